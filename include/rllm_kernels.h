@@ -530,6 +530,90 @@ int32_t rllm_cache_swap_in(const uint64_t *key_caches, const uint64_t *value_cac
                            int64_t num_blocks, int64_t block_nbytes, const int64_t *record_slots,
                            int64_t num_records, const void *host_records, uintptr_t stream);
 
+/* ======================================================================
+ * MXFP4 KV cache: 4-bit codes with a scale per 32 elements
+ * ==================================================================== */
+
+/* New (additive).  One layer's keys (and values) are uint8
+ * [num_blocks, num_kv_heads, page], page = rllm_mxfp4_page_bytes(head_dim,
+ * block_size) = block_size * head_dim * 17 / 32 bytes: block_size rows (one a
+ * token) of head_dim / 2 code bytes, then block_size rows of head_dim / 32 scale
+ * bytes.  Byte i of a code row holds elements 2i (low four bits) and 2i + 1: sign,
+ * two exponent bits, one mantissa bit (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6).  Scale
+ * byte j (E8M0) stands for 2^(e - 127), the factor of elements 32j .. 32j + 31; 255
+ * makes them NaN.  A block is num_kv_heads * page contiguous bytes, so
+ * rllm_cache_copy_blocks, rllm_cache_swap_out / _in, rllm_cache_block_copy and
+ * rllm_cache_zero move these caches as they are (zeroed pages read as zeros).
+ * Shapes: head_dim a multiple of 32 up to 256, block_size a multiple of 16 up to
+ * 4096, at most 1024 kv heads and 1024 q heads, caches 16-byte aligned; anything
+ * else returns hipErrorInvalidValue.  slot_mapping is as for the other cache
+ * writes; a block id of a table outside [0, num_blocks) is an unused entry. */
+
+/* Bytes of a (block, kv head) page; -1 for a shape outside the above. */
+int64_t rllm_mxfp4_page_bytes(int64_t head_dim, int64_t block_size);
+
+/* Slot-mapped write of new_key / new_value [num_tokens, num_kv_heads, head_dim]
+ * (input_dtype RLLM_DTYPE_F16 or RLLM_DTYPE_BF16, 16-byte aligned), quantised as it
+ * is written: of 32 elements with largest magnitude a, the scale byte is
+ * clamp(floor(log2 a) - 2 + 127, 1, 254) (the OCP microscaling rule) and each code the
+ * nearest to x / 2^(e - 127), ties to the even one, at most 6; 32 elements with an
+ * infinity or a NaN among them become NaN (byte 255).  Slots < 0 or of a block
+ * past the cache are skipped; the slots of one call must differ. */
+int32_t rllm_cache_write_mxfp4(uint8_t *key_cache, uint8_t *value_cache, const uint16_t *new_key,
+                               const uint16_t *new_value, const int64_t *slot_mapping,
+                               int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t block_size, int64_t num_blocks, int32_t input_dtype,
+                               uintptr_t stream);
+
+/* Reads rows back: out_key / out_value [num_tokens, num_kv_heads, head_dim] of
+ * output_dtype get the rows slot_mapping[t] of the caches, zeros where the slot is
+ * < 0 or of a block past the cache; a slot may be listed more than once.  Exact
+ * in bf16 up to its largest value; f16 rounds to nearest even (values past 65504
+ * become infinities, below 2^-14 subnormal). */
+int32_t rllm_cache_read_mxfp4(uint16_t *out_key, uint16_t *out_value, const uint8_t *key_cache,
+                              const uint8_t *value_cache, const int64_t *slot_mapping,
+                              int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t block_size, int64_t num_blocks, int32_t output_dtype,
+                              uintptr_t stream);
+
+/* Rotary embedding fused with the write: arguments as rllm_rope_cache_write.
+ * The rotation is in f32 (cos / sin as given, each product and the sum rounded to
+ * f32); q_out is rounded to dtype once, the rotated key is quantised from its f32
+ * value.  (rllm_rope_cache_write rounds every step to dtype, as the model does: its
+ * q_out differs from this one's by rounding.)  head_dim must be a multiple of 64. */
+int32_t rllm_rope_cache_write_mxfp4(void *q_out, const void *q, const void *k, const void *v,
+                                    uint8_t *key_cache, uint8_t *value_cache,
+                                    const int64_t *slot_mapping, const int32_t *positions,
+                                    const float *cos_cache, const float *sin_cache,
+                                    int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                                    int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                                    int64_t max_position, int32_t dtype, uintptr_t stream);
+
+/* Decode attention over the cache: arguments as rllm_paged_attention_decode_ex,
+ * with the cache's num_blocks.  output and query 4-byte aligned, of q_dtype
+ * (RLLM_DTYPE_F16 | RLLM_DTYPE_BF16).  Sums, maxima and weights are f32; the result
+ * does not depend on the q type's range (keys and values are not converted to
+ * it).  Keys or values that read as NaN make the outputs that see them NaN.
+ * workspace: at least rllm_paged_attention_decode_mxfp4_workspace_size(...) bytes,
+ * 16-byte aligned, zero-filled before its first such call (each completed call
+ * leaves it ready for the next); calls that share it must not overlap in time.
+ * NULL: a library-owned buffer per (device, stream); a capture on a stream that
+ * has none of the size yet runs a workgroup a (sequence, kv head) and needs none.
+ * Graphs captured on one stream share its buffer: replay them in order, or give
+ * each its own workspace. */
+int32_t rllm_paged_attention_decode_mxfp4(void *output, const void *query, const uint8_t *key_cache,
+                                          const uint8_t *value_cache, const int32_t *block_tables,
+                                          const int32_t *seq_lens, int64_t num_seqs,
+                                          int64_t num_q_heads, int64_t num_kv_heads,
+                                          int64_t head_dim, int64_t block_size,
+                                          int64_t max_num_blocks_per_seq, int64_t num_blocks,
+                                          float scale, int32_t q_dtype, void *workspace,
+                                          int64_t workspace_bytes, uintptr_t stream);
+int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64_t num_q_heads,
+                                                         int64_t num_kv_heads, int64_t head_dim,
+                                                         int64_t block_size,
+                                                         int64_t max_num_blocks_per_seq);
+
 /* Replace rllm_vector_add_f32(_sync) and rllm_block_copy(_sync),
  * smoke.cu:21-66; bound at cuda.rs:17-35.  out = a + b (f32); nbytes
  * contiguous bytes src -> dst. */

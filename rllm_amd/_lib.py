@@ -86,6 +86,14 @@ SIGNATURES = {
     "rllm_fused_silu_mul_f16_sync": [_P, _P, _P, _I64],
     "rllm_rmsnorm_ex": [_P, _P, _P, _I64, _I64, _F, _I32, _U],
     "rllm_silu_mul_ex": [_P, _P, _P, _I64, _I32, _U],
+    "rllm_mxfp4_page_bytes": [_I64, _I64],
+    "rllm_cache_write_mxfp4": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _U],
+    "rllm_cache_read_mxfp4": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _U],
+    "rllm_rope_cache_write_mxfp4": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+                                    _I64, _I64, _I32, _U],
+    "rllm_paged_attention_decode_mxfp4": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F,
+                                          _I32, _P, _I64, _U],
+    "rllm_paged_attention_decode_mxfp4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64],
     "rllm_vector_add_f32": [_P, _P, _P, _I64, _U],
     "rllm_vector_add_f32_sync": [_P, _P, _P, _I64],
     "rllm_block_copy": [_P, _P, _I64, _U],
@@ -101,7 +109,8 @@ SIGNATURES = {
     "rllm_gpu_alloc_host": [ctypes.POINTER(ctypes.c_void_p), _I64],
     "rllm_gpu_free_host": [_P],
 }
-_RESTYPE = {"rllm_paged_attention_decode_workspace_size": _I64}
+_RESTYPE = {"rllm_paged_attention_decode_workspace_size": _I64, "rllm_mxfp4_page_bytes": _I64,
+            "rllm_paged_attention_decode_mxfp4_workspace_size": _I64}
 
 
 def lib() -> ctypes.CDLL:

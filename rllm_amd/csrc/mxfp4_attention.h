@@ -1,0 +1,102 @@
+// Pieces of the attention kernels over the MXFP4 KV cache (mxfp4_decode.hip,
+// mxfp4_prefill.hip).
+//
+// Scores.  S = K Q^T runs on the block-scaled matrix product with K as it lies in
+// the cache: a lane's 16 bytes are the 32 codes of one scale, its scale byte the
+// product's E8M0 scale, so K is never converted.  The other operand is 8 bits a
+// value; a query row is split into E4M3 terms that add up to it: x0 = e4m3(x),
+// x1 = e4m3(16 (x - x0)), x2 = e4m3(16 (16 (x - x0) - x1)), with a power of two per row
+// (largest element in [128, 256)) and 2^-4 more per term in the scale operand.
+// Four significant bits a term: two hold a bf16 (8 bits), three an f16 (11),
+// exactly for elements down to 2^-13 of the row's largest, below that within 2^-21
+// (bf16; f16 2^-25) of it.  Against 64 bits the summed products of such terms are
+// off by 4e-6 of the scores' rms (200 random 128-wide tiles; 3e-5 with 30-fold
+// outlier channels): the product's own sums carry about 17 bits below its largest
+// terms.
+//
+// Values.  O^T = V^T P^T runs in bf16: code * 2^(e - 127) is exact in bf16 (two
+// significant bits, the f32 exponent range), whatever the query's type.
+#pragma once
+
+#include "mxfp4.h"
+
+namespace rllm {
+namespace {
+
+// terms of a query element
+template <int QKIND> constexpr int mx4_terms() { return QKIND == KIND_BF16 ? 2 : 3; }
+
+__device__ __forceinline__ mx_f32x4 mx4_mma16(const uint4& k, const mx_i32x8& q, const mx_f32x4& c, int ks, int qs) {
+    const mx_i32x8 a = {static_cast<int>(k.x), static_cast<int>(k.y), static_cast<int>(k.z), static_cast<int>(k.w), 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4, 0, 0, ks, 0, qs);
+}
+__device__ __forceinline__ mx_f32x16 mx4_mma32(const uint4& k, const mx_i32x8& q, const mx_f32x16& c, int ks, int qs) {
+    const mx_i32x8 a = {static_cast<int>(k.x), static_cast<int>(k.y), static_cast<int>(k.z), static_cast<int>(k.w), 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q, c, 4, 0, 0, ks, 0, qs);
+}
+__device__ __forceinline__ mx_f32x4 mx4_mma_bf16(const uint4& a, const uint4& b, const mx_f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, a), __builtin_bit_cast(mx_bf16x8, b), c,
+                                                   0, 0, 0);
+}
+__device__ __forceinline__ mx_f32x16 mx4_mma32_bf16(const uint4& a, const uint4& b, const mx_f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(mx_bf16x8, a), __builtin_bit_cast(mx_bf16x8, b), c,
+                                                   0, 0, 0);
+}
+
+// Transposing LDS read: in each group of 16 lanes, lane j addresses 4
+// consecutive 16-bit values M[j][0..3]; lane i receives M[4k + i/4][i%4] for k = 0..3.
+__device__ __forceinline__ uint2 mx4_read_tr16(const uint16_t* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mx_i16x4*)(p)));
+}
+
+__device__ __forceinline__ uint32_t mx4_pack_bf16(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(mx_f32x2{lo, hi}, mx_bf16x2));
+}
+template <int QKIND> __device__ __forceinline__ uint32_t mx4_pack16(float lo, float hi) {
+    if constexpr (QKIND == KIND_BF16) return mx4_pack_bf16(lo, hi);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(mx_f32x2{lo, hi}, mx_f16x2));
+}
+
+// four values -> four E4M3 bytes, and the remainders times 16
+__device__ __forceinline__ uint32_t mx4_term4(float (&x)[4]) {
+    int w = 0;
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    x[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * 16.f;
+    x[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * 16.f;
+    x[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * 16.f;
+    x[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * 16.f;
+    return static_cast<uint32_t>(w);
+}
+
+// max / sum over the lanes that share l % 16 (XOR 16, 32), or l % 32 (XOR 32 alone)
+__device__ __forceinline__ float mx4_max_32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float mx4_sum_32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float mx4_max_16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return mx4_max_32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float mx4_sum_16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return mx4_sum_32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// The power of two of a query row (its largest element in [128, 256)) as the
+// scale byte of its first term; the terms' bytes are this less 4 each and stay
+// at 0 or more.  255 (NaN) for a row with an infinity or a NaN.
+__device__ __forceinline__ int mx4_query_byte(float amax) {
+    const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // 127 + floor(log2)
+    return amax < INFINITY ? max(e - 7, 8) : 255;
+}
+
+// the block scales of a term: 255 stays NaN
+__device__ __forceinline__ int mx4_term_byte(int byte0, int term) { return byte0 == 255 ? 255 : byte0 - 4 * term; }
+
+}  // namespace
+}  // namespace rllm

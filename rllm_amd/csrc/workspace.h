@@ -33,7 +33,8 @@
 
 namespace rllm {
 
-enum WorkspaceRole : int { WS_DECODE_STREAM = 0, WS_DECODE_PARTS = 1, WS_PREFILL_SPLITS = 2, WS_DECODE_PREFIX = 3, WS_GENERIC = 4 };
+enum WorkspaceRole : int { WS_DECODE_STREAM = 0, WS_DECODE_PARTS = 1, WS_PREFILL_SPLITS = 2, WS_DECODE_PREFIX = 3, WS_GENERIC = 4,
+                           WS_MX4_DECODE = 5, WS_MX4_PREFILL = 6 };
 
 // The sole right to queue launches on one buffer, until it is destroyed.
 using WorkspaceHold = std::unique_lock<std::mutex>;

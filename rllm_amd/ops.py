@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import DTYPE_BF16, DTYPE_F16, DTYPE_FP8_E4M3, DTYPE_FP8_E5M2, FP8_ROUND_TOWARD_ZERO, call
+from ._lib import DTYPE_BF16, DTYPE_F16, DTYPE_FP8_E4M3, DTYPE_FP8_E5M2, FP8_ROUND_TOWARD_ZERO, call, lib
 
 _TORCH_16 = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
@@ -340,6 +340,157 @@ def rope_and_cache(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
          _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), _ptr(positions), _ptr(cos), _ptr(sin),
          n, hq, hkv, d, bs, nb, cos.shape[0], dt, kv, k_scale, v_scale, fp8_rounding, _stream(stream))
     return q_out if q is not None else None
+
+
+def mxfp4_cache(num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int, device) -> torch.Tensor:
+    """A zeroed MXFP4 cache uint8 [num_blocks, num_kv_heads, page] (keys or values
+    of one layer; layout in include/rllm_kernels.h)."""
+    page = lib().rllm_mxfp4_page_bytes(head_dim, block_size)
+    if page < 0:
+        raise ValueError("head_dim must be a multiple of 32 up to 256, block_size a multiple of 16 up to 4096")
+    return torch.zeros((num_blocks, num_kv_heads, page), dtype=torch.uint8, device=device)
+
+
+def _mxfp4_block_size(k_cache: torch.Tensor, v_cache: torch.Tensor, hkv: int, d: int) -> int:
+    """Block size of a pair of MXFP4 caches of hkv heads and head_dim d."""
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or k_cache.dim() != 3 \
+            or k_cache.shape != v_cache.shape:
+        raise ValueError("MXFP4 caches are uint8 [num_blocks, Hkv, page] of equal shape")
+    row = d // 32 * 17
+    bs = k_cache.shape[2] // row if row else 0
+    if d % 32 or k_cache.shape[1] != hkv or bs < 16 or bs % 16 or bs * row != k_cache.shape[2]:
+        raise ValueError("the caches' heads and page do not fit the heads and head_dim")
+    return bs
+
+
+def _mxfp4_rows(key, value, k_cache, v_cache, slot_mapping):
+    """Checks of the row operators; returns (n, Hkv, D, block size, blocks, dtype code)."""
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError("key and value rows must be [num_tokens, Hkv, D] of one shape")
+    n, hkv, d = key.shape
+    bs = _mxfp4_block_size(k_cache, v_cache, hkv, d)
+    dt = _TORCH_16.get(key.dtype)
+    if dt is None or value.dtype != key.dtype:
+        raise TypeError("key and value rows must be float16 or bfloat16")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (n,):
+        raise ValueError("slot_mapping must be int64 [num_tokens]")
+    return n, hkv, d, bs, k_cache.shape[0], dt
+
+
+def _all_dense(*tensors: torch.Tensor) -> None:
+    if not _dense_on_one_gpu(*tensors):
+        raise ValueError("tensors must be contiguous and on one GPU")
+    if tensors[0].get_device() != torch.cuda.current_device():
+        raise ValueError("the tensors' GPU must be the current device")
+
+
+def reshape_and_cache_mxfp4(new_key: torch.Tensor, new_value: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, slot_mapping: torch.Tensor, *,
+                            stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Slot-mapped write into MXFP4 caches, quantising as it writes, through
+    rllm_cache_write_mxfp4."""
+    n, hkv, d, bs, nb, dt = _mxfp4_rows(new_key, new_value, k_cache, v_cache, slot_mapping)
+    _all_dense(new_key, new_value, k_cache, v_cache, slot_mapping)
+    call("rllm_cache_write_mxfp4", _ptr(k_cache), _ptr(v_cache), _ptr(new_key), _ptr(new_value), _ptr(slot_mapping),
+         n, hkv, d, bs, nb, dt, _stream(stream))
+
+
+def read_cache_mxfp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, *,
+                     head_dim: Optional[int] = None, dtype: Optional[torch.dtype] = None,
+                     out_key: Optional[torch.Tensor] = None, out_value: Optional[torch.Tensor] = None,
+                     stream: Optional[torch.cuda.Stream] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows slot_mapping names of MXFP4 caches as 16-bit (key, value)
+    [num_tokens, Hkv, D], through rllm_cache_read_mxfp4; rows of negative slots are
+    zeros.  Give out_key and out_value, or head_dim and dtype."""
+    if (out_key is None) != (out_value is None):
+        raise ValueError("give both out_key and out_value or neither")
+    if out_key is None:
+        if head_dim is None or dtype is None or k_cache.dim() != 3 or slot_mapping.dim() != 1:
+            raise ValueError("without outputs, head_dim and dtype are needed, 3-d caches and 1-d slots")
+        out_key = torch.empty((slot_mapping.shape[0], k_cache.shape[1], head_dim), dtype=dtype, device=k_cache.device)
+        out_value = torch.empty_like(out_key)
+    elif (head_dim is not None and head_dim != out_key.shape[-1]) or (dtype is not None and dtype != out_key.dtype):
+        raise ValueError("head_dim and dtype disagree with the outputs")
+    n, hkv, d, bs, nb, dt = _mxfp4_rows(out_key, out_value, k_cache, v_cache, slot_mapping)
+    _all_dense(out_key, out_value, k_cache, v_cache, slot_mapping)
+    call("rllm_cache_read_mxfp4", _ptr(out_key), _ptr(out_value), _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping),
+         n, hkv, d, bs, nb, dt, _stream(stream))
+    return out_key, out_value
+
+
+def rope_and_cache_mxfp4(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, slot_mapping: torch.Tensor, positions: torch.Tensor,
+                         cos: torch.Tensor, sin: torch.Tensor, *, q_out: Optional[torch.Tensor] = None,
+                         stream: Optional[torch.cuda.Stream] = None) -> Optional[torch.Tensor]:
+    """rope_and_cache over MXFP4 caches, through rllm_rope_cache_write_mxfp4: q and
+    k rotated in f32, q rounded once, k quantised from f32.  Returns the rotated q
+    (``q_out``, which may be ``q`` itself), or None when q is None."""
+    n, hkv, d, bs, nb, dt = _mxfp4_rows(k, v, k_cache, v_cache, slot_mapping)
+    if positions.dtype != torch.int32 or positions.shape != (n,):
+        raise ValueError("positions must be int32 [num_tokens]")
+    if cos.dtype != torch.float32 or sin.shape != cos.shape or sin.dtype != cos.dtype \
+            or cos.dim() != 2 or cos.shape[1] != d // 2:
+        raise ValueError("cos/sin must be float32 [max_position, head_dim // 2]")
+    tensors = [k, v, k_cache, v_cache, slot_mapping, positions, cos, sin]
+    hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
+            raise ValueError("q must be [num_tokens, Hq, D] of the k dtype")
+        hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError("q_out must match q")
+        tensors += [q, q_out]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _all_dense(*tensors)
+    call("rllm_rope_cache_write_mxfp4", _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache),
+         _ptr(slot_mapping), _ptr(positions), _ptr(cos), _ptr(sin), n, hq, hkv, d, bs, nb, cos.shape[0], dt,
+         _stream(stream))
+    return q_out
+
+
+def _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out):
+    """Checks the attention operators share; returns (Hq, Hkv, D, block size, blocks, dtype code, out)."""
+    if q.dim() != 3 or k_cache.dim() != 3:
+        raise ValueError("q [*, Hq, D] and MXFP4 caches [nb, Hkv, page] required")
+    _, hq, d = q.shape
+    hkv = k_cache.shape[1]
+    bs = _mxfp4_block_size(k_cache, v_cache, hkv, d)
+    dt = _TORCH_16.get(q.dtype)
+    if dt is None:
+        raise TypeError("q must be float16 or bfloat16")
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("block_tables and seq_lens must be int32")
+    if seq_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0]:
+        raise ValueError("block_tables [num_seqs, max_blocks] and seq_lens [num_seqs] required")
+    if out is None:
+        out = torch.empty_like(q)
+    elif not _like(out, q):
+        raise ValueError("out must be a contiguous tensor like q")
+    _all_dense(q, k_cache, v_cache, block_tables, seq_lens)
+    return hq, hkv, d, bs, k_cache.shape[0], dt, out
+
+
+def paged_decode_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                       seq_lens: torch.Tensor, scale: float, *, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None, validate: bool = True,
+                       stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Decode attention over MXFP4 caches through rllm_paged_attention_decode_mxfp4."""
+    hq, hkv, d, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
+    if q.shape[0] != seq_lens.shape[0]:
+        raise ValueError("one query a sequence required")
+    if validate:
+        validate_tables(block_tables, seq_lens, nb, bs)
+    ws_bytes = 0
+    if workspace is not None:
+        _all_dense(q, workspace)
+        ws_bytes = workspace.numel() * workspace.element_size()
+    call("rllm_paged_attention_decode_mxfp4", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+         _ptr(seq_lens), q.shape[0], hq, hkv, d, bs, block_tables.shape[1], nb, scale, dt, _ptr(workspace), ws_bytes,
+         _stream(stream))
+    return out
 
 
 def layer_table(caches, device) -> torch.Tensor:
