@@ -593,7 +593,8 @@ int32_t rllm_rope_cache_write_mxfp4(void *q_out, const void *q, const void *k, c
  * with the cache's num_blocks.  output and query 4-byte aligned, of q_dtype
  * (RLLM_DTYPE_F16 | RLLM_DTYPE_BF16).  Sums, maxima and weights are f32; the result
  * does not depend on the q type's range (keys and values are not converted to
- * it).  Keys or values that read as NaN make the outputs that see them NaN.
+ * it).  Keys or values that read as NaN make the outputs that see them NaN, and no
+ * others (values with scale bytes 253 and 254, which no write makes, count as NaN).
  * workspace: at least rllm_paged_attention_decode_mxfp4_workspace_size(...) bytes,
  * 16-byte aligned, zero-filled before its first such call (each completed call
  * leaves it ready for the next); calls that share it must not overlap in time.
@@ -613,6 +614,22 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
                                                          int64_t num_kv_heads, int64_t head_dim,
                                                          int64_t block_size,
                                                          int64_t max_num_blocks_per_seq);
+
+/* Chunked-prefill attention over the cache: arguments as
+ * rllm_paged_attention_prefill_ex (causal at absolute positions; the new tokens'
+ * rows must be in the cache already), with the cache's num_blocks.  query 16-byte,
+ * output 8-byte aligned.  bf16 queries: the weights are rounded to bf16 before they
+ * meet the values, as for 16-bit caches; f16: to 16 bits.  Rows of output that
+ * query_start_loc leaves out stay as they are. */
+int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,
+                                           const uint8_t *key_cache, const uint8_t *value_cache,
+                                           const int32_t *block_tables, const int32_t *seq_lens,
+                                           const int32_t *query_start_loc, int64_t num_seqs,
+                                           int64_t num_tokens, int64_t num_q_heads,
+                                           int64_t num_kv_heads, int64_t head_dim,
+                                           int64_t block_size, int64_t max_num_blocks_per_seq,
+                                           int64_t num_blocks, float scale, int32_t q_dtype,
+                                           uintptr_t stream);
 
 /* Replace rllm_vector_add_f32(_sync) and rllm_block_copy(_sync),
  * smoke.cu:21-66; bound at cuda.rs:17-35.  out = a + b (f32); nbytes

@@ -94,6 +94,8 @@ SIGNATURES = {
     "rllm_paged_attention_decode_mxfp4": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F,
                                           _I32, _P, _I64, _U],
     "rllm_paged_attention_decode_mxfp4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64],
+    "rllm_paged_attention_prefill_mxfp4": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                           _F, _I32, _U],
     "rllm_vector_add_f32": [_P, _P, _P, _I64, _U],
     "rllm_vector_add_f32_sync": [_P, _P, _P, _I64],
     "rllm_block_copy": [_P, _P, _I64, _U],

@@ -23,6 +23,8 @@ namespace rllm {
 constexpr int MX4_BLOCK = 32;       // elements of one scale
 constexpr int MX4_TOKENS = 16;      // block_size is a multiple of this
 constexpr int64_t MX4_MAX_DIM = 256;
+// the largest scale byte a write makes (bf16 values up to 2^128): 6 * 2^125 is finite in f32
+constexpr uint32_t MX4_TOP_SCALE = 252;
 constexpr float MX4_LOG2E = 1.4426950408889634f;
 
 __host__ __device__ inline int64_t mx4_page_bytes(int64_t d, int64_t bs) { return bs * (d / 32) * 17; }
@@ -31,6 +33,12 @@ __host__ __device__ inline int64_t mx4_page_bytes(int64_t d, int64_t bs) { retur
 inline bool mx4_shape_ok(int64_t hkv, int64_t d, int64_t bs, int64_t nb) {
     return hkv > 0 && hkv <= 1024 && d >= MX4_BLOCK && d % MX4_BLOCK == 0 && d <= MX4_MAX_DIM && bs >= MX4_TOKENS &&
            bs % MX4_TOKENS == 0 && bs <= 4096 && nb >= 0 && nb <= (int64_t(1) << 31) - 1;
+}
+
+// the tables and heads of the two attention operators
+inline bool mx4_attention_ok(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t bs, int64_t maxb) {
+    return hq > 0 && hq <= 1024 && hq % hkv == 0 && num_seqs <= (int64_t(1) << 20) && maxb >= 0 &&
+           maxb <= (int64_t(1) << 24) && maxb * bs <= (int64_t(1) << 27);
 }
 
 inline bool mx4_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -87,6 +87,16 @@ __device__ __forceinline__ float mx4_sum_16(float v) {
     return mx4_sum_32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// inclusive prefix sum over the wave
+__device__ __forceinline__ int mx4_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);   // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);   // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1, 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2, 3
+}
+
 // The power of two of a query row (its largest element in [128, 256)) as the
 // scale byte of its first term; the terms' bytes are this less 4 each and stay
 // at 0 or more.  255 (NaN) for a row with an infinity or a NaN.

@@ -54,15 +54,6 @@ struct MxDecodeArgs {
     float* part_ml;                      // [2 * workgroups][16][2]
 };
 
-__device__ __forceinline__ int mxd_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // row_shr:2
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);   // row_shr:4
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);   // row_shr:8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1, 3
-    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2, 3
-}
-
 __device__ __forceinline__ int64_t mxd_uniform(int64_t v) {
     const int lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
     const int hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
@@ -127,7 +118,7 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
         int longest = 1;
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
             const int n = s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
-            total += __builtin_amdgcn_readlane(mxd_scan(n), 63);
+            total += __builtin_amdgcn_readlane(mx4_scan(n), 63);
             int m = n;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) m = max(m, __shfl_xor(m, off));
@@ -143,7 +134,7 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
         int64_t before = 0;   // items of one row of each earlier sequence
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
             const int n = s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
-            const int incl = mxd_scan(n);
+            const int incl = mx4_scan(n);
             const int64_t first = (before + incl - n) * rows_seq;
             const uint64_t hit =
                 __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos < first + static_cast<int64_t>(n) * rows_seq);
@@ -342,7 +333,7 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
                     w = ok ? w : make_uint4(0, 0, 0, 0);
                     e = ok ? e : 127u;
                 }
-                const float f = mx4_factor(e);
+                const float f = e > MX4_TOP_SCALE ? INFINITY : mx4_factor(e);   // NaN
                 if (NB % 2 == 0 || idx < 2 * MX4_TOKENS * NB) {
                     uint4* dst = reinterpret_cast<uint4*>(v_lds + tok * ROW + 32 * b);
                     dst[0] = make_uint4(mx4_dec_bf16<0>(w.x, f), mx4_dec_bf16<1>(w.x, f), mx4_dec_bf16<2>(w.x, f), mx4_dec_bf16<3>(w.x, f));
@@ -513,8 +504,7 @@ int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t bs, in
 
 int32_t mxd_check(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t nb) {
     RLLM_CHECK_ARG(mx4_shape_ok(hkv, d, bs, nb));
-    RLLM_CHECK_ARG(hq > 0 && hq <= 1024 && hq % hkv == 0);
-    RLLM_CHECK_ARG(num_seqs <= (int64_t(1) << 20) && maxb >= 0 && maxb <= (int64_t(1) << 24) && maxb * bs <= (int64_t(1) << 27));
+    RLLM_CHECK_ARG(mx4_attention_ok(num_seqs, hq, hkv, bs, maxb));
     return 0;
 }
 

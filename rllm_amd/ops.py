@@ -493,6 +493,27 @@ def paged_decode_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     return out
 
 
+def paged_prefill_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                        seq_lens: torch.Tensor, query_start_loc: torch.Tensor, scale: float, *,
+                        out: Optional[torch.Tensor] = None, validate: bool = True,
+                        stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Chunked-prefill attention over MXFP4 caches through rllm_paged_attention_prefill_mxfp4."""
+    hq, hkv, d, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
+    b, t = seq_lens.shape[0], q.shape[0]
+    if query_start_loc.dtype != torch.int32 or query_start_loc.shape != (b + 1,) or \
+            query_start_loc.device != q.device or not query_start_loc.is_contiguous():
+        raise ValueError("query_start_loc must be contiguous int32 [num_seqs + 1] on the device of q")
+    if validate:
+        validate_tables(block_tables, seq_lens, nb, bs)
+        qsl = query_start_loc.detach().cpu()
+        if int(qsl[0]) != 0 or int(qsl[-1]) != t or bool((qsl[1:] < qsl[:-1]).any()):
+            raise ValueError("query_start_loc must rise from 0 to num_tokens")
+    call("rllm_paged_attention_prefill_mxfp4", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+         _ptr(seq_lens), _ptr(query_start_loc), b, t, hq, hkv, d, bs, block_tables.shape[1], nb, scale, dt,
+         _stream(stream))
+    return out
+
+
 def layer_table(caches, device) -> torch.Tensor:
     """DEVICE uint64 array of the per-layer cache base addresses, the form
     rllm_cache_copy_blocks / rllm_cache_swap_{out,in} take.  Build it once per

@@ -55,6 +55,21 @@ def test_decode_refuses():
     assert decode(b=0, o=0) == 0 and decode(b=-1) == 0
 
 
+def prefill(b=2, t=10, hq=32, hkv=8, d=128, bs=16, maxb=4, nb=10, scale=0.1, dt=1, o=P, q=P, kc=P, vc=P, bt=P, sl=P,
+            qsl=P):
+    return rllm_amd.lib().rllm_paged_attention_prefill_mxfp4(o, q, kc, vc, bt, sl, qsl, b, t, hq, hkv, d, bs, maxb, nb,
+                                                             scale, dt, 0)
+
+
+def test_prefill_refuses():
+    for bad in (dict(hkv=0), dict(hq=0), dict(hq=30), dict(d=40), dict(d=512), dict(bs=8), dict(maxb=-1),
+                dict(maxb=1 << 25), dict(nb=0), dict(b=(1 << 20) + 1), dict(t=(1 << 26) + 1), dict(scale=float("nan")),
+                dict(dt=3), dict(o=0), dict(q=0), dict(kc=0), dict(vc=0), dict(bt=0), dict(sl=0), dict(qsl=0),
+                dict(kc=P + 8), dict(vc=P + 8), dict(q=P + 8), dict(o=P + 4)):
+        assert prefill(**bad) == 1, bad
+    assert prefill(b=0, o=0) == 0 and prefill(t=0) == 0
+
+
 def test_sizes():
     L = rllm_amd.lib()
     assert L.rllm_mxfp4_page_bytes(128, 16) == 16 * (64 + 4) == M.page_bytes(128, 16)
@@ -90,6 +105,8 @@ def test_front_end_refuses():
               (q, kc, kc, bt, sl, 1.0)):
         with pytest.raises(ValueError):
             ops.paged_decode_mxfp4(*a)
+        with pytest.raises(ValueError):
+            ops.paged_prefill_mxfp4(*a[:5], torch.zeros(3, dtype=torch.int32), 1.0)
     with pytest.raises(TypeError):
         ops.paged_decode_mxfp4(q, kc, kc, bt.long(), sl, 1.0)
 
