@@ -97,6 +97,17 @@ __device__ __forceinline__ int mx4_scan(int v) {
     return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2, 3
 }
 
+// largest value (>= 0) of the wave
+__device__ __forceinline__ int mx4_wave_max(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // The power of two of a query row (its largest element in [128, 256)) as the
 // scale byte of its first term; the terms' bytes are this less 4 each and stay
 // at 0 or more.  255 (NaN) for a row with an infinity or a NaN.

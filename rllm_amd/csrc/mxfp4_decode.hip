@@ -38,6 +38,9 @@ constexpr int MXD_ITEM = 32;          // tokens
 constexpr int MXD_HEADS = 16;         // query heads a row
 constexpr int MXD_MAX_PIECES = 64;    // of a row
 
+// workgroups a CU: two waves a SIMD, one where a wave needs more than half its registers
+__host__ __device__ constexpr int mxd_per_cu(int64_t d) { return d <= 128 ? 2 : 1; }
+
 struct MxDecodeArgs {
     uint16_t* out;
     const uint16_t* q;
@@ -54,15 +57,9 @@ struct MxDecodeArgs {
     float* part_ml;                      // [2 * workgroups][16][2]
 };
 
-__device__ __forceinline__ int64_t mxd_uniform(int64_t v) {
-    const int lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
-    const int hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
-    return (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
-}
-
-// bf16 elements of a V row in LDS: 32 bytes of padding put 8 consecutive rows of a
-// transposing read (4 a lane group) on different banks
-template <int NB> constexpr int mxd_row() { return 32 * NB + 16; }
+// bf16 elements of a V row in LDS (a multiple of 64 bytes apart in the banks, see
+// the transposing read)
+template <int NB> constexpr int mxd_row() { return 32 * NB + (NB % 2 ? 0 : 32); }
 
 template <int NB>
 constexpr int mxd_lds_words() {   // 4-byte words: the waves' V tiles, or their outputs at a row's end
@@ -71,7 +68,7 @@ constexpr int mxd_lds_words() {   // 4-byte words: the waves' V tiles, or their 
                : MXD_WAVES * MXD_HEADS * 32 * NB;
 }
 
-// ---- one item's operands as loaded ----
+// One item's operands as loaded.
 template <int NB>
 struct MxItem {
     static constexpr int NK = (NB + 3) / 4;     // 128-wide steps of head_dim
@@ -80,8 +77,14 @@ struct MxItem {
     uint32_t ke[2][NK], ve[NV];
 };
 
+// A row at hand: row r of sequence s, its first item in the list of all, its items
+// (all of them, and lo .. hi - 1 of this workgroup) and keys.
+struct MxRow {
+    int s, r, first, items, lo, hi, ctx;
+};
+
 template <int QKIND, int NB>
-__global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs a) {
+__global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_kernel(MxDecodeArgs a) {
     constexpr int D = 32 * NB;
     constexpr int NK = MxItem<NB>::NK, NV = MxItem<NB>::NV;
     constexpr int NT = mx4_terms<QKIND>();
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
     const int l16 = lane & 15, grp = lane >> 4;
     uint16_t* const v_lds = reinterpret_cast<uint16_t*>(lds) + wave * MXD_ITEM * ROW;
     const int rows_seq = a.hkv * a.groups;      // rows of a sequence
-    const int64_t page_bytes = mx4_page_bytes(D, a.bs);
+    const int page_bytes = static_cast<int>(mx4_page_bytes(D, a.bs));
     const int code_bytes = a.bs * (D / 2);      // of a page
     const int width = a.maxb * a.bs;            // tokens a table can hold
 
@@ -104,121 +107,178 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
         return max((min(len, width) + MXD_ITEM - 1) / MXD_ITEM, 1);
     };
 
-    int s = 0, r = 0, row_items = 0;   // the row at hand: row r of sequence s
-    int64_t row0 = 0, pos = 0, end, share;   // its first item, the next item, the share's end and length
+    MxRow row{};
+    int end, share;   // the end of this workgroup's items in the list, and the items of a workgroup
     if (!a.counters) {
         // no scratch: a workgroup a row
-        s = blockIdx.x / rows_seq;
-        r = blockIdx.x % rows_seq;
-        row_items = items_of(a.seq_lens[s]);
-        end = share = row_items;
+        row.s = blockIdx.x / rows_seq;
+        row.r = blockIdx.x % rows_seq;
+        row.items = items_of(a.seq_lens[row.s]);
+        end = share = row.items;
     } else {
-        // ---- the share: every wave works it out from the lengths ----
-        int64_t total = 0;
-        int longest = 1;
+        // ---- the share: every wave works it out from the lengths.  The lengths of
+        // up to 64 sequences are read once ----
+        int len0 = lane < a.num_seqs ? items_of(a.seq_lens[lane]) : 0;
+        int total = 0, longest = 1;
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int n = s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
+            const int n = s0 == 0 ? len0 : s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
             total += __builtin_amdgcn_readlane(mx4_scan(n), 63);
-            int m = n;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) m = max(m, __shfl_xor(m, off));
-            longest = max(longest, __builtin_amdgcn_readfirstlane(m));
+            longest = max(longest, mx4_wave_max(n));
         }
-        total = mxd_uniform(total * rows_seq);
+        total *= rows_seq;
         // n items span at most ceil(n / share) + 1 pieces
-        const int64_t least = max(MXD_WAVES, (longest + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
-        share = mxd_uniform(max((total + gridDim.x - 1) / gridDim.x, least));
-        pos = share * blockIdx.x;
-        end = min(pos + share, total);
-        if (pos >= end) return;   // whole workgroup
-        int64_t before = 0;   // items of one row of each earlier sequence
+        const int least = max(MXD_WAVES, (longest + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
+        share = __builtin_amdgcn_readfirstlane(max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), least));
+        const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
+        if (pos64 >= total) return;   // whole workgroup
+        const int pos = static_cast<int>(pos64);
+        end = static_cast<int>(min<int64_t>(pos64 + share, total));
+        int before = 0;   // items of one row of each earlier sequence
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int n = s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
+            const int n = s0 == 0 ? len0 : s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
             const int incl = mx4_scan(n);
-            const int64_t first = (before + incl - n) * rows_seq;
-            const uint64_t hit =
-                __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos < first + static_cast<int64_t>(n) * rows_seq);
+            const int first = (before + incl - n) * rows_seq;
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos - first < n * rows_seq);
             if (hit) {
                 const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-                s = s0 + j;
-                row_items = __builtin_amdgcn_readlane(n, j);
-                const int64_t f = (before + __builtin_amdgcn_readlane(incl, j) - row_items) * rows_seq;
-                r = static_cast<int>((pos - f) / row_items);
-                row0 = f + static_cast<int64_t>(r) * row_items;
+                row.s = s0 + j;
+                row.items = __builtin_amdgcn_readlane(n, j);
+                const int f = __builtin_amdgcn_readlane(first, j);
+                row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(row.items));
+                row.first = f + row.r * row.items;
                 break;
             }
             before += __builtin_amdgcn_readlane(incl, 63);
         }
-        s = __builtin_amdgcn_readfirstlane(s);
-        r = __builtin_amdgcn_readfirstlane(r);
-        row_items = __builtin_amdgcn_readfirstlane(row_items);
-        row0 = mxd_uniform(row0);
+        row.s = __builtin_amdgcn_readfirstlane(row.s);
+        row.r = __builtin_amdgcn_readfirstlane(row.r);
+        row.first = __builtin_amdgcn_readfirstlane(row.first);
+        row.items = __builtin_amdgcn_readfirstlane(row.items);
+        row.lo = pos - row.first;
     }
+    row.hi = min(end - row.first, row.items);
+    row.ctx = min(max(a.seq_lens[row.s], 0), width);
 
-    while (pos < end) {
-        const int ctx = min(max(a.seq_lens[s], 0), width);
-        const int h = r / a.groups, hg = r % a.groups;
-        const int g_all = a.hq / a.hkv;
-        const int heads = min(g_all - hg * MXD_HEADS, MXD_HEADS);           // of this row
-        const int64_t q_row = static_cast<int64_t>(s) * a.hq + h * g_all + hg * MXD_HEADS;
-        const int i_lo = static_cast<int>(pos - row0);
-        const int i_hi = static_cast<int>(min<int64_t>(end - row0, row_items));
-        const int32_t* bt_row = a.bt + static_cast<int64_t>(s) * a.maxb;
+    // the row after this one, empty (lo == hi) past the share
+    auto next_row = [&](const MxRow& x) __attribute__((always_inline)) -> MxRow {
+        MxRow y = x;
+        y.first = x.first + x.items;
+        y.lo = 0;
+        y.hi = 0;
+        if (y.first >= end) return y;
+        if (++y.r == rows_seq) {
+            y.r = 0;
+            ++y.s;   // within the batch: the list goes on
+            const int len = a.seq_lens[y.s];
+            y.items = items_of(len);
+            y.ctx = min(max(len, 0), width);
+        }
+        y.hi = min(end - y.first, y.items);
+        return y;
+    };
 
-        // 16-token part u of the context: its page (-1: none) and byte offset of
-        // its first code row, both uniform
-        struct Part { const uint8_t *k, *v; int row; bool ok; };
-        auto part_of = [&](int u) __attribute__((always_inline)) -> Part {
-            const int blk = static_cast<int>((static_cast<uint32_t>(u) * a.subs_mul) >> 32);
-            const bool in = u * MX4_TOKENS < ctx;
-            const int id = in ? bt_row[min(blk, a.maxb - 1)] : -1;
-            Part p;
-            p.ok = id >= 0 && id < a.nb;
-            const int64_t at = ((p.ok ? id : 0) * static_cast<int64_t>(a.hkv) + h) * page_bytes;
-            p.k = a.kc + at;
-            p.v = a.vc + at;
-            p.row = p.ok ? (u - blk * a.subs) * MX4_TOKENS : 0;
-            return p;
-        };
-        // loads of item i (every address lies in a page of the cache)
-        auto load = [&](int i, MxItem<NB>& x, uint32_t& present) __attribute__((always_inline)) {
-            const Part p0 = part_of(2 * i), p1 = part_of(2 * i + 1);
-            present = (p0.ok ? 1u : 0u) | (p1.ok ? 2u : 0u);
+    // ---- this wave's items of a row are lo + wave + 4 k.  Lane j holds what 16-token
+    // part j % 2 of item k0 + j / 2 needs of the table: its page (-1: none, a key
+    // past the context among it) and row in the page ----
+    struct Ids { int id, row; };
+    auto load_ids = [&](const MxRow& x, int k0) __attribute__((always_inline)) -> Ids {
+        const int i = x.lo + wave + MXD_WAVES * (k0 + (lane >> 1));
+        const int u = 2 * i + (lane & 1);
+        const int blk = static_cast<int>((static_cast<uint32_t>(u) * a.subs_mul) >> 32);
+        Ids y{-1, 0};
+        if (i < x.hi && u * MX4_TOKENS < x.ctx) {
+            const int id = a.bt[static_cast<int64_t>(x.s) * a.maxb + min(blk, a.maxb - 1)];
+            y.id = id < a.nb ? id : -1;
+            y.row = (u - blk * a.subs) * MX4_TOKENS;
+        }
+        return y;
+    };
+    struct Part { const uint8_t *k, *v; int codes, scales; bool ok; };   // pages and byte offsets, uniform
+    auto part_of = [&](const Ids& ids, int at, int h) __attribute__((always_inline)) -> Part {
+        const int id = __builtin_amdgcn_readlane(ids.id, at), r0 = __builtin_amdgcn_readlane(ids.row, at);
+        Part p;
+        p.ok = id >= 0;
+        const int64_t page = (static_cast<int64_t>(max(id, 0)) * a.hkv + h) * page_bytes;
+        p.k = a.kc + page;
+        p.v = a.vc + page;
+        p.codes = r0 * (D / 2);
+        p.scales = code_bytes + r0 * NB;
+        return p;
+    };
+    // loads of an item's keys and values; `at` its lane in ids.  Every address lies in a page of the cache
+    const uint32_t k_off = l16 * (D / 2) + 16 * grp, ke_off = l16 * NB + grp;
+    auto load_k = [&](const Ids& ids, int at, int h, MxItem<NB>& x) __attribute__((always_inline)) {
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const Part& p = sub ? p1 : p0;
-                const int row = p.row + l16;
+        for (int sub = 0; sub < 2; ++sub) {
+            const Part p = part_of(ids, at + sub, h);
+            const uint8_t *codes = p.k + p.codes, *scales = p.k + p.scales;
 #pragma unroll
-                for (int kk = 0; kk < NK; ++kk) {
-                    const int b = 4 * kk + grp;
-                    const bool have = NB % 4 == 0 || b < NB;
-                    x.k[sub][kk] = make_uint4(0, 0, 0, 0);
-                    x.ke[sub][kk] = 127;
-                    if (have) {
-                        x.k[sub][kk] = *reinterpret_cast<const uint4*>(p.k + row * (D / 2) + 16 * b);
-                        x.ke[sub][kk] = p.k[code_bytes + row * NB + b];
-                    }
+            for (int kk = 0; kk < NK; ++kk) {
+                x.k[sub][kk] = make_uint4(0, 0, 0, 0);
+                x.ke[sub][kk] = 127;
+                if (4 * (kk + 1) <= NB || 4 * kk + grp < NB) {
+                    x.k[sub][kk] = *reinterpret_cast<const uint4*>(codes + (k_off + 64 * kk));
+                    x.ke[sub][kk] = scales[ke_off + 4 * kk];
                 }
             }
+        }
+    };
+    auto load_v = [&](const Ids& ids, int at, int h, MxItem<NB>& x) __attribute__((always_inline)) -> uint32_t {
+        const Part p0 = part_of(ids, at, h), p1 = part_of(ids, at + 1, h);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
+        for (int j = 0; j < NV; ++j) {
+            constexpr int SUB = MX4_TOKENS * NB;   // chunks of a 16-token part
+            if constexpr (NB % 4 == 0) {           // a load lies in one part
+                const Part& p = 64 * j >= SUB ? p1 : p0;
+                const uint32_t at_c = (64 * j) % SUB + lane;
+                x.v[j] = *reinterpret_cast<const uint4*>(p.v + p.codes + 16 * at_c);
+                x.ve[j] = (p.v + p.scales)[at_c];
+            } else {
                 const int idx = 64 * j + lane;
-                const bool second = idx >= MX4_TOKENS * NB;
-                const int at = second ? idx - MX4_TOKENS * NB : idx;
-                const Part& p = second ? p1 : p0;
+                const bool second = idx >= SUB;
+                const int at_c = second ? idx - SUB : idx;
+                const uint8_t* page = second ? p1.v : p0.v;
                 x.v[j] = make_uint4(0, 0, 0, 0);
                 x.ve[j] = 127;
-                if (NB % 2 == 0 || idx < 2 * MX4_TOKENS * NB) {
-                    x.v[j] = *reinterpret_cast<const uint4*>(p.v + p.row * (D / 2) + 16 * at);
-                    x.ve[j] = p.v[code_bytes + p.row * NB + at];
+                if (NB % 2 == 0 || idx < 2 * SUB) {
+                    x.v[j] = *reinterpret_cast<const uint4*>(page + (second ? p1.codes : p0.codes) + 16 * at_c);
+                    x.ve[j] = page[(second ? p1.scales : p0.scales) + at_c];
                 }
             }
-        };
+        }
+        return (p0.ok ? 1u : 0u) | (p1.ok ? 2u : 0u);
+    };
 
-        MxItem<NB> cur, nxt;
-        uint32_t cur_present = 0, nxt_present = 0;
-        int i = i_lo + wave;
-        if (i < i_hi) load(i, cur, cur_present);
+    // transposing V read: lane's row 4 grp + l16 / 4 (and 16 more); 16-byte chunk i of
+    // block b of row t lies at i ^ (b % 4) ^ (2 (t / 4 % 2)).  With rows a multiple of 64
+    // bytes apart, the stores of 16 lanes (4 rows x 4 blocks) and the reads of 32 (8
+    // rows x 32 bytes) are then spread over all banks.
+    const int vr_row = 4 * grp + (l16 >> 2), vr_sw = 2 * (grp & 1);
+    const uint16_t* const vr = v_lds + vr_row * ROW + 4 * (l16 & 1);
+    const int vr_half = (l16 & 3) >> 1;
+
+    Ids ids = load_ids(row, 0);
+    MxItem<NB> set[2];
+    uint32_t present[2] = {0, 0};
+    // the first two items of a row
+    auto start = [&](const MxRow& x, const Ids& y) __attribute__((always_inline)) {
+        const int h = x.r / a.groups;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if (x.lo + wave + MXD_WAVES * b < x.hi) {
+                load_k(y, 2 * b, h, set[b]);
+                present[b] = load_v(y, 2 * b, h, set[b]);
+            }
+    };
+    start(row, ids);
+
+    while (row.lo < row.hi) {
+        const int h = row.r / a.groups, hg = row.r % a.groups;
+        const int g_all = a.hq / a.hkv;
+        const int heads = min(g_all - hg * MXD_HEADS, MXD_HEADS);           // of this row
+        const int64_t q_row = static_cast<int64_t>(row.s) * a.hq + h * g_all + hg * MXD_HEADS;
+        const MxRow nxt = next_row(row);
+        const Ids nxt_ids = load_ids(nxt, 0);
 
         // ---- the query rows as E4M3 terms: lane group g holds elements 16 g.. and
         // 64 + 16 g.. of each 128-wide step (the 8-bit operand's order) ----
@@ -273,11 +333,12 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
 #pragma unroll
         for (int j = 0; j < 2 * NB; ++j) o[j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;   // l: this lane's tokens only
+        const int count = (row.hi - row.lo - wave + MXD_WAVES - 1) / MXD_WAVES;   // this wave's items
 
-        for (; i < i_hi; i += MXD_WAVES) {
-            const bool more = i + MXD_WAVES < i_hi;
-            if (more) load(i + MXD_WAVES, nxt, nxt_present);
-
+        // item k from set x; the set's loads of item k + 2 go out as its registers come free
+        auto item = [&](int k, MxItem<NB>& x, uint32_t& here) __attribute__((always_inline)) {
+            const bool more = k + 2 < count;
+            const int at = 2 * ((k + 2) & 31);
             // ---- scores, in units of log2 ----
             float sc[8];
 #pragma unroll
@@ -287,23 +348,27 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
                 for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
-                        acc = mx4_mma16(cur.k[sub][kk], qt[t][kk], acc, static_cast<int>(cur.ke[sub][kk]), qs[t]);
+                        acc = mx4_mma16(x.k[sub][kk], qt[t][kk], acc, static_cast<int>(x.ke[sub][kk]), qs[t]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[4 * sub + e] = acc[e] * a.c;
             }
-            const int t0 = i * MXD_ITEM;
-            const bool full = cur_present == 3u && t0 + MXD_ITEM <= ctx;
+            if (more) {
+                if (at == 0) ids = load_ids(row, k + 2);   // every 32 items
+                load_k(ids, at, h, x);
+            }
+            const int t0 = (row.lo + wave + MXD_WAVES * k) * MXD_ITEM;
+            const bool full = here == 3u && t0 + MXD_ITEM <= row.ctx;
             if (!full) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const bool ok = ((cur_present >> (e >> 2)) & 1u) && t0 + 16 * (e >> 2) + 4 * grp + (e & 3) < ctx;
+                    const bool ok = ((here >> (e >> 2)) & 1u) && t0 + 16 * (e >> 2) + 4 * grp + (e & 3) < row.ctx;
                     sc[e] = ok ? sc[e] : -INFINITY;
                 }
             }
             // ---- weights against a running max that moves only when a score
             // passes it by 2^8: no weight passes 2^8, and the outputs are rarely
             // rescaled ----
-            float top = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+            const float top = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
             if (__builtin_amdgcn_ballot_w64(top > m + 8.f || m == -INFINITY)) {
                 const float m_new = fmaxf(m, mx4_max_16(top));
                 const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
@@ -326,37 +391,44 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
             for (int j = 0; j < NV; ++j) {
                 const int idx = 64 * j + lane;
                 const int tok = idx / NB, b = idx % NB;
-                uint4 w = cur.v[j];
-                uint32_t e = cur.ve[j];
+                uint4 w = x.v[j];
+                uint32_t e = x.ve[j];
                 if (!full) {   // rows that no query sees may hold anything: zeros
-                    const bool ok = ((cur_present >> (tok >> 4)) & 1u) && t0 + tok < ctx;
+                    const bool ok = ((here >> (tok >> 4)) & 1u) && t0 + tok < row.ctx;
                     w = ok ? w : make_uint4(0, 0, 0, 0);
                     e = ok ? e : 127u;
                 }
                 const float f = e > MX4_TOP_SCALE ? INFINITY : mx4_factor(e);   // NaN
                 if (NB % 2 == 0 || idx < 2 * MX4_TOKENS * NB) {
                     uint4* dst = reinterpret_cast<uint4*>(v_lds + tok * ROW + 32 * b);
-                    dst[0] = make_uint4(mx4_dec_bf16<0>(w.x, f), mx4_dec_bf16<1>(w.x, f), mx4_dec_bf16<2>(w.x, f), mx4_dec_bf16<3>(w.x, f));
-                    dst[1] = make_uint4(mx4_dec_bf16<0>(w.y, f), mx4_dec_bf16<1>(w.y, f), mx4_dec_bf16<2>(w.y, f), mx4_dec_bf16<3>(w.y, f));
-                    dst[2] = make_uint4(mx4_dec_bf16<0>(w.z, f), mx4_dec_bf16<1>(w.z, f), mx4_dec_bf16<2>(w.z, f), mx4_dec_bf16<3>(w.z, f));
-                    dst[3] = make_uint4(mx4_dec_bf16<0>(w.w, f), mx4_dec_bf16<1>(w.w, f), mx4_dec_bf16<2>(w.w, f), mx4_dec_bf16<3>(w.w, f));
+                    const int sw = (b & 3) ^ (2 * ((tok >> 2) & 1));
+                    dst[0 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.x, f), mx4_dec_bf16<1>(w.x, f), mx4_dec_bf16<2>(w.x, f), mx4_dec_bf16<3>(w.x, f));
+                    dst[1 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.y, f), mx4_dec_bf16<1>(w.y, f), mx4_dec_bf16<2>(w.y, f), mx4_dec_bf16<3>(w.y, f));
+                    dst[2 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.z, f), mx4_dec_bf16<1>(w.z, f), mx4_dec_bf16<2>(w.z, f), mx4_dec_bf16<3>(w.z, f));
+                    dst[3 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.w, f), mx4_dec_bf16<1>(w.w, f), mx4_dec_bf16<2>(w.w, f), mx4_dec_bf16<3>(w.w, f));
                 }
             }
+            if (more) here = load_v(ids, at, h, x);
             // a wave's LDS accesses stay in order; the fence keeps the compiler's too
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            const uint16_t* vr = v_lds + (4 * grp + (l16 >> 2)) * ROW + 4 * (l16 & 3);
 #pragma unroll
-            for (int j = 0; j < 2 * NB; ++j) {
-                const uint2 v0 = mx4_read_tr16(vr + 16 * j), v1 = mx4_read_tr16(vr + 16 * ROW + 16 * j);
+            for (int j = 0; j < 2 * NB; ++j) {   // 16 elements: half j % 2 of block j / 2
+                const uint16_t* src = vr + 32 * (j >> 1) + 8 * ((2 * (j & 1) + vr_half) ^ ((j >> 1) & 3) ^ vr_sw);
+                const uint2 v0 = mx4_read_tr16(src), v1 = mx4_read_tr16(src + 16 * ROW);
                 const uint4 vv = make_uint4(v0.x, v0.y, v1.x, v1.y);
                 o[j] = mx4_mma_bf16(vv, ph, o[j]);
                 o[j] = mx4_mma_bf16(vv, pl, o[j]);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            cur = nxt;
-            cur_present = nxt_present;
+        };
+        for (int k = 0; k < count; k += 2) {
+            item(k, set[0], present[0]);
+            if (k + 1 < count) item(k + 1, set[1], present[1]);
         }
+        // the next row's first loads travel while the waves join
+        ids = nxt_ids;
+        start(nxt, ids);
 
         // ---- the waves join ----
         l = mx4_sum_16(l);
@@ -391,10 +463,10 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
         }
         __syncthreads();
         const float* o_lds = reinterpret_cast<const float*>(lds);
-        const int64_t first_wg = row0 / share, last_wg = (row0 + row_items - 1) / share;
-        const int pieces = static_cast<int>(last_wg - first_wg) + 1;
+        const int first_wg = static_cast<int>(static_cast<uint32_t>(row.first) / static_cast<uint32_t>(share));
+        const int pieces = static_cast<int>(static_cast<uint32_t>(row.first + row.items - 1) / static_cast<uint32_t>(share)) - first_wg + 1;
         const bool whole = pieces == 1;
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (i_lo == 0 ? 1 : 0);
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (row.lo == 0 ? 1 : 0);
         for (int e = 2 * tid; e < heads * D; e += 2 * MXD_THREADS) {
             const int hd = e / D;
             float y0 = 0.f, y1 = 0.f;
@@ -429,7 +501,7 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
                 if (tid == 0) __hip_atomic_store(a.counters + first_wg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 // piece p's slot: the row starts in its first workgroup's last
                 // piece (slot 2 wg + 1) and goes on in the others' first
-                auto slot_of = [&](int p) __attribute__((always_inline)) { return 2 * (first_wg + p) + (p == 0 ? 1 : 0); };
+                auto slot_of = [&](int p) __attribute__((always_inline)) { return 2 * static_cast<int64_t>(first_wg + p) + (p == 0 ? 1 : 0); };
                 // a wave a head, a lane a piece: the pieces' factors and the row's sum
                 for (int hd = wave; hd < heads; hd += MXD_WAVES) {
                     float mp = -INFINITY, lp = 0.f;
@@ -470,17 +542,9 @@ __global__ __launch_bounds__(MXD_THREADS, 2) void mx4_decode_kernel(MxDecodeArgs
             }
         }
         __syncthreads();   // LDS is free for the next row
-        pos = row0 + i_hi;
-        if (i_hi == row_items) {
-            row0 += row_items;
-            if (++r == rows_seq) {
-                r = 0;
-                if (++s < a.num_seqs) row_items = items_of(a.seq_lens[s]);
-            }
-        }
+        row = nxt;
     }
 }
-
 
 // ---- host ----
 
@@ -490,21 +554,25 @@ int64_t mxd_scratch_bytes(int64_t wgs, int64_t d) {
     return mxd_counter_bytes(wgs) + 2 * wgs * MXD_HEADS * (d + 2) * 4;
 }
 
-// Workgroups: two a CU, fewer where the tables hold less than one item a wave.
-int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t bs, int64_t maxb, int64_t* wgs) {
+// Workgroups: what the device holds, fewer where the tables hold less than one item a wave.
+int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t* wgs) {
     int dev = 0, cus = 0;
     RLLM_TRY(hipGetDevice(&dev));
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t groups = (hq / hkv + MXD_HEADS - 1) / MXD_HEADS, rows = num_seqs * hkv * groups;
     const int64_t items = (maxb * bs + MXD_ITEM - 1) / MXD_ITEM;
     const int64_t most = rows * ((items + MXD_WAVES - 1) / MXD_WAVES > 0 ? (items + MXD_WAVES - 1) / MXD_WAVES : 1);
-    *wgs = most < 2 * cus ? most : 2 * cus;
+    const int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d);
+    *wgs = most < held ? most : held;
     return 0;
 }
 
 int32_t mxd_check(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t nb) {
     RLLM_CHECK_ARG(mx4_shape_ok(hkv, d, bs, nb));
     RLLM_CHECK_ARG(mx4_attention_ok(num_seqs, hq, hkv, bs, maxb));
+    // the items of all rows are counted in 32 bits
+    const int64_t rows = num_seqs * hkv * ((hq / hkv + MXD_HEADS - 1) / MXD_HEADS);
+    RLLM_CHECK_ARG(rows * ((maxb * bs + MXD_ITEM - 1) / MXD_ITEM + 1) <= INT32_MAX);
     return 0;
 }
 
@@ -533,7 +601,7 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
     if (num_seqs <= 0) return 0;
     if (mxd_check(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, 0)) return -1;
     int64_t wgs = 0;
-    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, block_size, max_num_blocks_per_seq, &wgs)) return -1;
+    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs)) return -1;
     return mxd_scratch_bytes(wgs, head_dim);
 }
 
@@ -554,7 +622,7 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
     RLLM_CHECK_ARG(mx4_aligned16(key_cache) && mx4_aligned16(value_cache));
     RLLM_CHECK_ARG(((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(output)) & 3) == 0);
     int64_t wgs = 0;
-    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, block_size, max_num_blocks_per_seq, &wgs);
+    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs);
     if (rc) return rc;
     const int64_t need = mxd_scratch_bytes(wgs, head_dim);
     void* ws = workspace;
