@@ -46,8 +46,10 @@ inline bool mx4_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p
 typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 typedef short mx_i16x4 __attribute__((ext_vector_type(4)));
+typedef short mx_i16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short mx_u16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 mx_bf16x8 __attribute__((ext_vector_type(8)));

@@ -23,6 +23,22 @@
 namespace rllm {
 namespace {
 
+// x / factor as four E4M3 bytes, and x less what they stand for (wrappers of target
+// builtins, not templates)
+__device__ __forceinline__ uint32_t mx4_enc_e4m3(const float (&x)[4], float factor) {
+    mx_i16x2 w = {0, 0};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[0], x[1], factor, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[2], x[3], factor, true);
+    return __builtin_bit_cast(uint32_t, w);
+}
+__device__ __forceinline__ void mx4_sub_e4m3(float (&x)[4], uint32_t w, float factor) {
+    const mx_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, factor, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, factor, true);
+    x[0] -= a[0];
+    x[1] -= a[1];
+    x[2] -= b[0];
+    x[3] -= b[1];
+}
+
 // terms of a query element
 template <int QKIND> constexpr int mx4_terms() { return QKIND == KIND_BF16 ? 2 : 3; }
 
@@ -57,16 +73,42 @@ template <int QKIND> __device__ __forceinline__ uint32_t mx4_pack16(float lo, fl
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(mx_f32x2{lo, hi}, mx_f16x2));
 }
 
-// four values -> four E4M3 bytes, and the remainders times 16
-__device__ __forceinline__ uint32_t mx4_term4(float (&x)[4]) {
-    int w = 0;
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], w, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
-    x[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * 16.f;
-    x[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * 16.f;
-    x[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * 16.f;
-    x[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * 16.f;
-    return static_cast<uint32_t>(w);
+// Four query elements (two packed pairs) as E4M3 terms, byte t of w[t]: term t is in
+// units of factor * 2^-4t.  Every step is exact but the conversions to E4M3 (nearest,
+// ties to even; in range, see mx4_query_byte).
+template <int QKIND>
+__device__ __forceinline__ void mx4_split4(uint32_t p0, uint32_t p1, float factor, uint32_t (&w)[mx4_terms<QKIND>()]) {
+    constexpr int NT = mx4_terms<QKIND>();
+    float x[4];
+    x[0] = QKIND == KIND_BF16 ? bf16_lo(p0) : f16_lo(p0);
+    x[1] = QKIND == KIND_BF16 ? bf16_hi(p0) : f16_hi(p0);
+    x[2] = QKIND == KIND_BF16 ? bf16_lo(p1) : f16_lo(p1);
+    x[3] = QKIND == KIND_BF16 ? bf16_hi(p1) : f16_hi(p1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        w[t] = mx4_enc_e4m3(x, factor);
+        if (t + 1 < NT) {
+            mx4_sub_e4m3(x, w[t], factor);
+            factor *= 0.0625f;
+        }
+    }
+}
+
+// largest 15-bit pattern of 8 16-bit floats (patterns rise with the magnitude,
+// infinities and NaNs above every finite value)
+__device__ __forceinline__ uint32_t mx4_amax8(const uint4& w) {
+    const mx_u16x2 a = __builtin_bit_cast(mx_u16x2, w.x & 0x7fff7fffu), b = __builtin_bit_cast(mx_u16x2, w.y & 0x7fff7fffu);
+    const mx_u16x2 c = __builtin_bit_cast(mx_u16x2, w.z & 0x7fff7fffu), d = __builtin_bit_cast(mx_u16x2, w.w & 0x7fff7fffu);
+    const mx_u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(a, b), __builtin_elementwise_max(c, d));
+    return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
+}
+__device__ __forceinline__ uint32_t mx4_umax_32(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+}
+__device__ __forceinline__ uint32_t mx4_umax_16(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return mx4_umax_32(max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1])));
 }
 
 // max / sum over the lanes that share l % 16 (XOR 16, 32), or l % 32 (XOR 32 alone)
@@ -109,11 +151,17 @@ __device__ __forceinline__ int mx4_wave_max(int v) {
 }
 
 // The power of two of a query row (its largest element in [128, 256)) as the
-// scale byte of its first term; the terms' bytes are this less 4 each and stay
-// at 0 or more.  255 (NaN) for a row with an infinity or a NaN.
-__device__ __forceinline__ int mx4_query_byte(float amax) {
-    const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // 127 + floor(log2)
-    return amax < INFINITY ? max(e - 7, 8) : 255;
+// scale byte of its first term, from the row's largest pattern; the terms' bytes are
+// this less 4 each and stay above 0.  255 (NaN) for a row with an infinity or a NaN.
+template <int QKIND>
+__device__ __forceinline__ int mx4_query_byte(uint32_t amax) {
+    const float x = QKIND == KIND_BF16 ? __uint_as_float(amax << 16) : f16_bits_to_f32(static_cast<uint16_t>(amax));
+    const int e = static_cast<int>(__float_as_uint(x) >> 23);   // 127 + floor(log2)
+    return amax < (QKIND == KIND_BF16 ? 0x7f80u : 0x7c00u) ? max(e - 7, 9) : 255;
+}
+// the terms' unit; of a NaN row any will do, its scales make it NaN
+__device__ __forceinline__ float mx4_query_factor(int byte0) {
+    return __uint_as_float(static_cast<uint32_t>(byte0 == 255 ? 127 : byte0) << 23);
 }
 
 // the block scales of a term: 255 stays NaN

@@ -37,6 +37,11 @@ constexpr int MXD_THREADS = 64 * MXD_WAVES;
 constexpr int MXD_ITEM = 32;          // tokens
 constexpr int MXD_HEADS = 16;         // query heads a row
 constexpr int MXD_MAX_PIECES = 64;    // of a row
+// What a row's start and join cost beside its items, in items: a workgroup whose share
+// starts more rows gets fewer.  64 contexts of 128-4096 tokens (32/8 heads, head_dim
+// 128): 53.6 us without, 44 with 4, 39.5 with 8, 41 with 12.  Equal contexts do not change.
+// Where a workgroup has under MXD_VIRT_MIN items the waves of a row have little to share.
+constexpr int MXD_VIRT = 8, MXD_VIRT_MIN = 24;
 
 // workgroups a CU: two waves a SIMD, one where a wave needs more than half its registers
 __host__ __device__ constexpr int mxd_per_cu(int64_t d) { return d <= 128 ? 2 : 1; }
@@ -61,13 +66,6 @@ struct MxDecodeArgs {
 // the transposing read)
 template <int NB> constexpr int mxd_row() { return 32 * NB + (NB % 2 ? 0 : 32); }
 
-template <int NB>
-constexpr int mxd_lds_words() {   // 4-byte words: the waves' V tiles, or their outputs at a row's end
-    return MXD_WAVES * MXD_ITEM * mxd_row<NB>() / 2 > MXD_WAVES * MXD_HEADS * 32 * NB
-               ? MXD_WAVES * MXD_ITEM * mxd_row<NB>() / 2
-               : MXD_WAVES * MXD_HEADS * 32 * NB;
-}
-
 // One item's operands as loaded.
 template <int NB>
 struct MxItem {
@@ -83,16 +81,32 @@ struct MxRow {
     int s, r, first, items, lo, hi, ctx;
 };
 
+// A piece of a row cut between workgroups: the row, its first workgroup and its pieces.
+struct Piece {
+    int s, r, first_wg, count;
+};
+
+// two floats past the XCD's own L2, as one access
+__device__ __forceinline__ void store2(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void load2(const float* p, float& x, float& y) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float(static_cast<uint32_t>(w));
+    y = __uint_as_float(static_cast<uint32_t>(w >> 32));
+}
+
 template <int QKIND, int NB>
 __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_kernel(MxDecodeArgs a) {
     constexpr int D = 32 * NB;
     constexpr int NK = MxItem<NB>::NK, NV = MxItem<NB>::NV;
     constexpr int NT = mx4_terms<QKIND>();
     constexpr int ROW = mxd_row<NB>();
-    __shared__ __align__(16) uint32_t lds[mxd_lds_words<NB>()];
+    __shared__ __align__(16) uint32_t lds[MXD_WAVES * MXD_ITEM * ROW / 2];   // a V tile a wave
     __shared__ float ml_lds[MXD_WAVES][MXD_HEADS][2];
     __shared__ float w_lds[MXD_MAX_PIECES][MXD_HEADS];
-    __shared__ int last_lds;
+    __shared__ int last_lds[2];
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -108,26 +122,36 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
     };
 
     MxRow row{};
+    int virt = 0;     // items a row's start counts for in the list
     int end, share;   // the end of this workgroup's items in the list, and the items of a workgroup
     if (!a.counters) {
         // no scratch: a workgroup a row
         row.s = blockIdx.x / rows_seq;
         row.r = blockIdx.x % rows_seq;
         row.items = items_of(a.seq_lens[row.s]);
+        row.ctx = min(max(a.seq_lens[row.s], 0), width);
         end = share = row.items;
     } else {
         // ---- the share: every wave works it out from the lengths.  The lengths of
         // up to 64 sequences are read once ----
-        int len0 = lane < a.num_seqs ? items_of(a.seq_lens[lane]) : 0;
+        const int len0 = a.seq_lens[min(lane, a.num_seqs - 1)];
+        auto len_at = [&](int s0) __attribute__((always_inline)) {
+            return s0 == 0 ? len0 : a.seq_lens[min(s0 + lane, a.num_seqs - 1)];
+        };
         int total = 0, longest = 1;
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int n = s0 == 0 ? len0 : s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
+            const int n = s0 + lane < a.num_seqs ? items_of(len_at(s0)) : 0;
             total += __builtin_amdgcn_readlane(mx4_scan(n), 63);
             longest = max(longest, mx4_wave_max(n));
         }
         total *= rows_seq;
+        const int all_rows = a.num_seqs * rows_seq;
+        if (total >= MXD_VIRT_MIN * static_cast<int>(gridDim.x)) {
+            virt = MXD_VIRT;
+            total += virt * all_rows;
+        }
         // n items span at most ceil(n / share) + 1 pieces
-        const int least = max(MXD_WAVES, (longest + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
+        const int least = max(MXD_WAVES, (longest + virt + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
         share = __builtin_amdgcn_readfirstlane(max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), least));
         const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
         if (pos64 >= total) return;   // whole workgroup
@@ -135,17 +159,20 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         end = static_cast<int>(min<int64_t>(pos64 + share, total));
         int before = 0;   // items of one row of each earlier sequence
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int n = s0 == 0 ? len0 : s0 + lane < a.num_seqs ? items_of(a.seq_lens[s0 + lane]) : 0;
+            const int raw = len_at(s0);
+            const int n = s0 + lane < a.num_seqs ? items_of(raw) + virt : 0;
             const int incl = mx4_scan(n);
             const int first = (before + incl - n) * rows_seq;
             const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos - first < n * rows_seq);
             if (hit) {
                 const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
                 row.s = s0 + j;
-                row.items = __builtin_amdgcn_readlane(n, j);
+                const int len = __builtin_amdgcn_readlane(n, j);
+                row.items = len - virt;
+                row.ctx = min(max(__builtin_amdgcn_readlane(raw, j), 0), width);
                 const int f = __builtin_amdgcn_readlane(first, j);
-                row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(row.items));
-                row.first = f + row.r * row.items;
+                row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(len));
+                row.first = f + row.r * len + virt;
                 break;
             }
             before += __builtin_amdgcn_readlane(incl, 63);
@@ -154,15 +181,15 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         row.r = __builtin_amdgcn_readfirstlane(row.r);
         row.first = __builtin_amdgcn_readfirstlane(row.first);
         row.items = __builtin_amdgcn_readfirstlane(row.items);
-        row.lo = pos - row.first;
+        row.ctx = __builtin_amdgcn_readfirstlane(row.ctx);
+        row.lo = max(pos - row.first, 0);
     }
     row.hi = min(end - row.first, row.items);
-    row.ctx = min(max(a.seq_lens[row.s], 0), width);
 
     // the row after this one, empty (lo == hi) past the share
     auto next_row = [&](const MxRow& x) __attribute__((always_inline)) -> MxRow {
         MxRow y = x;
-        y.first = x.first + x.items;
+        y.first = x.first + x.items + virt;
         y.lo = 0;
         y.hi = 0;
         if (y.first >= end) return y;
@@ -177,41 +204,43 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         return y;
     };
 
-    // ---- this wave's items of a row are lo + wave + 4 k.  Lane j holds what 16-token
-    // part j % 2 of item k0 + j / 2 needs of the table: its page (-1: none, a key
-    // past the context among it) and row in the page ----
+    // ---- this wave's items of a row are lo + wave + 4 k.  Lane j holds the table entry
+    // of 16-token part j % 2 of item k0 + j / 2, and the part's row in the page (-1: past
+    // the context).  Nothing looks at the entry here: its load, a row ahead, would have
+    // to be waited for ----
     struct Ids { int id, row; };
     auto load_ids = [&](const MxRow& x, int k0) __attribute__((always_inline)) -> Ids {
         const int i = x.lo + wave + MXD_WAVES * (k0 + (lane >> 1));
         const int u = 2 * i + (lane & 1);
         const int blk = static_cast<int>((static_cast<uint32_t>(u) * a.subs_mul) >> 32);
-        Ids y{-1, 0};
-        if (i < x.hi && u * MX4_TOKENS < x.ctx) {
-            const int id = a.bt[static_cast<int64_t>(x.s) * a.maxb + min(blk, a.maxb - 1)];
-            y.id = id < a.nb ? id : -1;
-            y.row = (u - blk * a.subs) * MX4_TOKENS;
-        }
+        Ids y{-1, i < x.hi && u * MX4_TOKENS < x.ctx ? (u - blk * a.subs) * MX4_TOKENS : -1};
+        if (a.maxb > 0) y.id = a.bt[static_cast<int64_t>(x.s) * a.maxb + min(blk, a.maxb - 1)];
         return y;
     };
-    struct Part { const uint8_t *k, *v; int codes, scales; bool ok; };   // pages and byte offsets, uniform
-    auto part_of = [&](const Ids& ids, int at, int h) __attribute__((always_inline)) -> Part {
-        const int id = __builtin_amdgcn_readlane(ids.id, at), r0 = __builtin_amdgcn_readlane(ids.row, at);
-        Part p;
-        p.ok = id >= 0;
-        const int64_t page = (static_cast<int64_t>(max(id, 0)) * a.hkv + h) * page_bytes;
-        p.k = a.kc + page;
-        p.v = a.vc + page;
-        p.codes = r0 * (D / 2);
-        p.scales = code_bytes + r0 * NB;
-        return p;
+    // The same resolved for kv head h: lane j's byte offset of the part's first code
+    // row in a cache, the distance from there to its first scale row, and which of the
+    // parts exist (the others point to page 0, and get no weight)
+    struct Parts { uint32_t lo, hi; int scales; uint64_t ok; };
+    auto resolve = [&](const Ids& x, int h) __attribute__((always_inline)) -> Parts {
+        const bool ok = x.row >= 0 && x.id >= 0 && x.id < a.nb;
+        const int r0 = ok ? x.row : 0;
+        const int64_t at = (static_cast<int64_t>(ok ? x.id : 0) * a.hkv + h) * page_bytes + r0 * (D / 2);
+        return Parts{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32), code_bytes + r0 * (NB - D / 2),
+                     __builtin_amdgcn_ballot_w64(ok)};
     };
-    // loads of an item's keys and values; `at` its lane in ids.  Every address lies in a page of the cache
+    struct Part { int64_t at; int scales; };   // uniform
+    auto part_of = [&](const Parts& x, int j) __attribute__((always_inline)) -> Part {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x.lo), j);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x.hi), j);
+        return Part{static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo), __builtin_amdgcn_readlane(x.scales, j)};
+    };
+    // loads of an item's keys and values from its parts.  Every address lies in a page of the cache
     const uint32_t k_off = l16 * (D / 2) + 16 * grp, ke_off = l16 * NB + grp;
-    auto load_k = [&](const Ids& ids, int at, int h, MxItem<NB>& x) __attribute__((always_inline)) {
+    auto load_k = [&](const Part& p0, const Part& p1, MxItem<NB>& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
-            const Part p = part_of(ids, at + sub, h);
-            const uint8_t *codes = p.k + p.codes, *scales = p.k + p.scales;
+            const Part& p = sub ? p1 : p0;
+            const uint8_t *codes = a.kc + p.at, *scales = codes + p.scales;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
                 x.k[sub][kk] = make_uint4(0, 0, 0, 0);
@@ -223,30 +252,29 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
             }
         }
     };
-    auto load_v = [&](const Ids& ids, int at, int h, MxItem<NB>& x) __attribute__((always_inline)) -> uint32_t {
-        const Part p0 = part_of(ids, at, h), p1 = part_of(ids, at + 1, h);
+    auto load_v = [&](const Part& p0, const Part& p1, MxItem<NB>& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             constexpr int SUB = MX4_TOKENS * NB;   // chunks of a 16-token part
             if constexpr (NB % 4 == 0) {           // a load lies in one part
                 const Part& p = 64 * j >= SUB ? p1 : p0;
+                const uint8_t* codes = a.vc + p.at;
                 const uint32_t at_c = (64 * j) % SUB + lane;
-                x.v[j] = *reinterpret_cast<const uint4*>(p.v + p.codes + 16 * at_c);
-                x.ve[j] = (p.v + p.scales)[at_c];
+                x.v[j] = *reinterpret_cast<const uint4*>(codes + 16 * at_c);
+                x.ve[j] = (codes + p.scales)[at_c];
             } else {
                 const int idx = 64 * j + lane;
                 const bool second = idx >= SUB;
                 const int at_c = second ? idx - SUB : idx;
-                const uint8_t* page = second ? p1.v : p0.v;
+                const uint8_t* codes = a.vc + (second ? p1.at : p0.at);
                 x.v[j] = make_uint4(0, 0, 0, 0);
                 x.ve[j] = 127;
                 if (NB % 2 == 0 || idx < 2 * SUB) {
-                    x.v[j] = *reinterpret_cast<const uint4*>(page + (second ? p1.codes : p0.codes) + 16 * at_c);
-                    x.ve[j] = page[(second ? p1.scales : p0.scales) + at_c];
+                    x.v[j] = *reinterpret_cast<const uint4*>(codes + 16 * at_c);
+                    x.ve[j] = codes[(second ? p1.scales : p0.scales) + at_c];
                 }
             }
         }
-        return (p0.ok ? 1u : 0u) | (p1.ok ? 2u : 0u);
     };
 
     // transposing V read: lane's row 4 grp + l16 / 4 (and 16 more); 16-byte chunk i of
@@ -257,75 +285,93 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
     const uint16_t* const vr = v_lds + vr_row * ROW + 4 * (l16 & 1);
     const int vr_half = (l16 & 3) >> 1;
 
-    Ids ids = load_ids(row, 0);
+    // a row's first workgroup and pieces: one that lies in this share needs no division
+    auto piece_of = [&](const MxRow& x) __attribute__((always_inline)) -> Piece {
+        Piece y{x.s, x.r, static_cast<int>(blockIdx.x), 1};
+        if (x.lo > 0) y.first_wg = static_cast<int>(static_cast<uint32_t>(x.first) / static_cast<uint32_t>(share));
+        if (x.lo > 0 || x.hi < x.items)
+            y.count = static_cast<int>(static_cast<uint32_t>(x.first + x.items - 1) / static_cast<uint32_t>(share)) - y.first_wg + 1;
+        return y;
+    };
+    Piece head{}, tail{};   // pieces of rows cut at the share's start and end
+
+    // a row's first query row and its number of query heads
+    auto q_row_of = [&](int s, int r, int& heads) __attribute__((always_inline)) -> int64_t {
+        const int g_all = a.hq / a.hkv, hg = r % a.groups;
+        heads = min(g_all - hg * MXD_HEADS, MXD_HEADS);
+        return static_cast<int64_t>(s) * a.hq + r / a.groups * g_all + hg * MXD_HEADS;
+    };
+    // the query rows, 4-byte aligned: lane group g holds elements 16 g.. and 64 + 16 g..
+    // of each 128-wide step (the order of the 8-bit operand)
+    uint4 q_raw[NK][4];
+    auto load_q = [&](const MxRow& x) __attribute__((always_inline)) {
+        int heads;
+        const int64_t q_row = q_row_of(x.s, x.r, heads);
+        const uint16_t* src = a.q + (q_row + min(l16, heads - 1)) * D;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d0 = 128 * kk + 64 * (i >> 1) + 16 * grp + 8 * (i & 1);
+                q_raw[kk][i] = make_uint4(0, 0, 0, 0);
+                if (NB % 4 == 0 || d0 < D) {
+                    const mx_u32x4 w = *reinterpret_cast<const mx_u32x4*>(src + d0);
+                    q_raw[kk][i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+    };
+
     MxItem<NB> set[2];
-    uint32_t present[2] = {0, 0};
+    uint32_t present[2] = {0, 0};   // an item's parts that exist
+    Parts parts;                    // of the items whose loads go out next
     // the first two items of a row
-    auto start = [&](const MxRow& x, const Ids& y) __attribute__((always_inline)) {
-        const int h = x.r / a.groups;
+    auto start = [&](const MxRow& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
             if (x.lo + wave + MXD_WAVES * b < x.hi) {
-                load_k(y, 2 * b, h, set[b]);
-                present[b] = load_v(y, 2 * b, h, set[b]);
+                const Part p0 = part_of(parts, 2 * b), p1 = part_of(parts, 2 * b + 1);
+                load_k(p0, p1, set[b]);
+                load_v(p0, p1, set[b]);
+                present[b] = static_cast<uint32_t>(parts.ok >> (2 * b)) & 3u;
             }
     };
-    start(row, ids);
+    parts = resolve(load_ids(row, 0), row.r / a.groups);
+    load_q(row);
+    start(row);
 
     while (row.lo < row.hi) {
-        const int h = row.r / a.groups, hg = row.r % a.groups;
-        const int g_all = a.hq / a.hkv;
-        const int heads = min(g_all - hg * MXD_HEADS, MXD_HEADS);           // of this row
-        const int64_t q_row = static_cast<int64_t>(row.s) * a.hq + h * g_all + hg * MXD_HEADS;
+        const int h = row.r / a.groups;
+        int heads;   // of this row
+        const int64_t q_row = q_row_of(row.s, row.r, heads);
         const MxRow nxt = next_row(row);
+        const int nxt_h = nxt.r / a.groups;
         const Ids nxt_ids = load_ids(nxt, 0);
 
-        // ---- the query rows as E4M3 terms: lane group g holds elements 16 g.. and
-        // 64 + 16 g.. of each 128-wide step (the 8-bit operand's order) ----
+        // ---- the query rows as E4M3 terms ----
         mx_i32x8 qt[NT][NK];
         int qs[NT];
         {
-            const uint16_t* src = a.q + (q_row + min(l16, heads - 1)) * D;
-            uint32_t raw[NK][16];
-            float amax = 0.f;
-            bool finite = true;
+            uint32_t amax = 0;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int d0 = 128 * kk + 64 * hf + 16 * grp;
-                    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (NB % 4 == 0 || d0 < D) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint32_t*>(src + d0 + 2 * j);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        raw[kk][8 * hf + j] = w[j];
-                        const float lo = QKIND == KIND_BF16 ? bf16_lo(w[j]) : f16_lo(w[j]);
-                        const float hi = QKIND == KIND_BF16 ? bf16_hi(w[j]) : f16_hi(w[j]);
-                        finite = finite && __builtin_fabsf(lo) < INFINITY && __builtin_fabsf(hi) < INFINITY;
-                        amax = fmaxf(amax, fmaxf(__builtin_fabsf(lo), __builtin_fabsf(hi)));
-                    }
-                }
-            amax = mx4_max_16(finite ? amax : INFINITY);
-            const int byte0 = mx4_query_byte(amax);
-            const int shift = byte0 == 255 ? 0 : 127 - byte0;
+                for (int i = 0; i < 4; ++i) amax = max(amax, mx4_amax8(q_raw[kk][i]));
+            const int byte0 = mx4_query_byte<QKIND>(mx4_umax_16(amax));
+            const float factor = mx4_query_factor(byte0);
 #pragma unroll
             for (int t = 0; t < NT; ++t) qs[t] = mx4_term_byte(byte0, t);
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float x[4];
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t x[NT], y[NT];
+                    mx4_split4<QKIND>(q_raw[kk][i].x, q_raw[kk][i].y, factor, x);
+                    mx4_split4<QKIND>(q_raw[kk][i].z, q_raw[kk][i].w, factor, y);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = raw[kk][2 * j + e];
-                        x[2 * e] = ldexpf(QKIND == KIND_BF16 ? bf16_lo(w) : f16_lo(w), shift);
-                        x[2 * e + 1] = ldexpf(QKIND == KIND_BF16 ? bf16_hi(w) : f16_hi(w), shift);
+                    for (int t = 0; t < NT; ++t) {
+                        qt[t][kk][2 * i] = static_cast<int>(x[t]);
+                        qt[t][kk][2 * i + 1] = static_cast<int>(y[t]);
                     }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) qt[t][kk][j] = static_cast<int>(mx4_term4(x));
                 }
         }
 
@@ -335,10 +381,15 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         float m = -INFINITY, l = 0.f;   // l: this lane's tokens only
         const int count = (row.hi - row.lo - wave + MXD_WAVES - 1) / MXD_WAVES;   // this wave's items
 
-        // item k from set x; the set's loads of item k + 2 go out as its registers come free
+        // item k from set x.  As the set's registers come free, the loads of item k + 2
+        // go out, or, at a row's end, of the next row's first two items
+        const int nxt_count = count < 2 ? 0 : (nxt.hi - nxt.lo - wave + MXD_WAVES - 1) / MXD_WAVES;
         auto item = [&](int k, MxItem<NB>& x, uint32_t& here) __attribute__((always_inline)) {
-            const bool more = k + 2 < count;
-            const int at = 2 * ((k + 2) & 31);
+            const bool last2 = k + 2 >= count;
+            const int ahead = last2 ? k + 2 - count : k + 2;
+            const bool more = !last2 || ahead < nxt_count;
+            const int at = 2 * (ahead & 31);
+            Part p0{}, p1{};
             // ---- scores, in units of log2 ----
             float sc[8];
 #pragma unroll
@@ -352,9 +403,12 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[4 * sub + e] = acc[e] * a.c;
             }
+            if (last2 && ahead == 0) parts = resolve(nxt_ids, nxt_h);
             if (more) {
-                if (at == 0) ids = load_ids(row, k + 2);   // every 32 items
-                load_k(ids, at, h, x);
+                if (!last2 && at == 0) parts = resolve(load_ids(row, ahead), h);   // every 32 items
+                p0 = part_of(parts, at);
+                p1 = part_of(parts, at + 1);
+                load_k(p0, p1, x);
             }
             const int t0 = (row.lo + wave + MXD_WAVES * k) * MXD_ITEM;
             const bool full = here == 3u && t0 + MXD_ITEM <= row.ctx;
@@ -408,7 +462,10 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
                     dst[3 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.w, f), mx4_dec_bf16<1>(w.w, f), mx4_dec_bf16<2>(w.w, f), mx4_dec_bf16<3>(w.w, f));
                 }
             }
-            if (more) here = load_v(ids, at, h, x);
+            if (more) {
+                load_v(p0, p1, x);
+                here = static_cast<uint32_t>(parts.ok >> at) & 3u;
+            }
             // a wave's LDS accesses stay in order; the fence keeps the compiler's too
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -427,122 +484,128 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
             if (k + 1 < count) item(k + 1, set[1], present[1]);
         }
         // the next row's first loads travel while the waves join
-        ids = nxt_ids;
-        start(nxt, ids);
+        if (nxt.lo < nxt.hi) load_q(nxt);
+        if (count < 2) {
+            parts = resolve(nxt_ids, nxt_h);
+            start(nxt);
+        } else if (count & 1) {
+            const MxItem<NB> x = set[0];
+            set[0] = set[1];
+            set[1] = x;
+            const uint32_t p = present[0];
+            present[0] = present[1];
+            present[1] = p;
+        }
 
-        // ---- the waves join ----
+        // ---- the waves join: outputs and sums in LDS (each in its own V tile) ----
         l = mx4_sum_16(l);
-        if (grp == 0) {
-            ml_lds[wave][l16][0] = m;
-            ml_lds[wave][l16][1] = l;
-        }
-        __syncthreads();   // every wave has also left its V tile
-        float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < MXD_WAVES; ++w) mm = fmaxf(mm, ml_lds[w][l16][0]);
-#pragma unroll
-        for (int w = 0; w < MXD_WAVES; ++w) {
-            const float mw = ml_lds[w][l16][0], lw = ml_lds[w][l16][1];
-            ll += lw == 0.f ? 0.f : lw * __builtin_amdgcn_exp2f(mw - mm);
-        }
-        {
-            const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-            float* dst = reinterpret_cast<float*>(lds) + (wave * MXD_HEADS + l16) * D + 4 * grp;
-            if (l16 < heads) {
-#pragma unroll
-                for (int j = 0; j < 2 * NB; ++j) {
-                    const mx_f32x4 y = f == 0.f ? mx_f32x4{0.f, 0.f, 0.f, 0.f} : o[j] * f;
-                    *reinterpret_cast<mx_f32x4*>(dst + 16 * j) = y;
-                }
+        if (l16 < heads) {
+            if (grp == 0) {
+                ml_lds[wave][l16][0] = m;
+                ml_lds[wave][l16][1] = l;
             }
-        }
-        // sums of the row's heads beside the outputs
-        if (wave == 0 && grp == 0) {
-            w_lds[0][l16] = mm;
-            w_lds[1][l16] = ll;
+            float* dst = reinterpret_cast<float*>(v_lds) + l16 * D + 4 * grp;
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) *reinterpret_cast<mx_f32x4*>(dst + 16 * j) = o[j];
         }
         __syncthreads();
-        const float* o_lds = reinterpret_cast<const float*>(lds);
-        const int first_wg = static_cast<int>(static_cast<uint32_t>(row.first) / static_cast<uint32_t>(share));
-        const int pieces = static_cast<int>(static_cast<uint32_t>(row.first + row.items - 1) / static_cast<uint32_t>(share)) - first_wg + 1;
-        const bool whole = pieces == 1;
+        const Piece piece = piece_of(row);
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (row.lo == 0 ? 1 : 0);
         for (int e = 2 * tid; e < heads * D; e += 2 * MXD_THREADS) {
             const int hd = e / D;
-            float y0 = 0.f, y1 = 0.f;
+            float mw[MXD_WAVES], lw[MXD_WAVES], mm = -INFINITY, ll = 0.f, y0 = 0.f, y1 = 0.f;
 #pragma unroll
             for (int w = 0; w < MXD_WAVES; ++w) {
-                const mx_f32x2 y = *reinterpret_cast<const mx_f32x2*>(o_lds + w * MXD_HEADS * D + e);
-                y0 += y[0];
-                y1 += y[1];
+                mw[w] = ml_lds[w][hd][0];
+                lw[w] = ml_lds[w][hd][1];
+                mm = fmaxf(mm, mw[w]);
             }
-            if (whole) {
-                const float L = w_lds[1][hd];
-                const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+            for (int w = 0; w < MXD_WAVES; ++w) {
+                const mx_f32x2 y = *reinterpret_cast<const mx_f32x2*>(lds + w * MXD_ITEM * ROW / 2 + e);
+                if (lw[w] != 0.f) {   // a wave that saw nothing adds nothing, NaN goes on
+                    const float f = __builtin_amdgcn_exp2f(mw[w] - mm);
+                    ll += f * lw[w];
+                    y0 += f * y[0];
+                    y1 += f * y[1];
+                }
+            }
+            if (piece.count == 1) {
+                const float inv = ll == 0.f ? 0.f : 1.f / ll;
                 *reinterpret_cast<uint32_t*>(a.out + q_row * D + e) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
             } else {
-                __hip_atomic_store(reinterpret_cast<uint64_t*>(a.part_o + slot * (MXD_HEADS * D) + e),
-                                   static_cast<uint64_t>(__float_as_uint(y1)) << 32 | __float_as_uint(y0),
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                store2(a.part_o + slot * (MXD_HEADS * D) + e, y0, y1);
+                if (e == hd * D) store2(a.part_ml + slot * (2 * MXD_HEADS) + 2 * hd, mm, ll);
             }
         }
-        if (!whole) {
-            if (tid < 2 * MXD_HEADS)
-                __hip_atomic_store(a.part_ml + slot * (2 * MXD_HEADS) + tid, w_lds[tid & 1][tid >> 1], __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's stores have arrived
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t n = __hip_atomic_fetch_add(a.counters + first_wg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                last_lds = n + 1 == static_cast<uint32_t>(pieces);
-            }
-            __syncthreads();
-            if (last_lds) {
-                if (tid == 0) __hip_atomic_store(a.counters + first_wg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // piece p's slot: the row starts in its first workgroup's last
-                // piece (slot 2 wg + 1) and goes on in the others' first
-                auto slot_of = [&](int p) __attribute__((always_inline)) { return 2 * static_cast<int64_t>(first_wg + p) + (p == 0 ? 1 : 0); };
-                // a wave a head, a lane a piece: the pieces' factors and the row's sum
-                for (int hd = wave; hd < heads; hd += MXD_WAVES) {
-                    float mp = -INFINITY, lp = 0.f;
-                    if (lane < pieces) {
-                        const float* src = a.part_ml + slot_of(lane) * (2 * MXD_HEADS) + 2 * hd;
-                        mp = __hip_atomic_load(src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        lp = __hip_atomic_load(src + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    }
-                    const float top = wave_max(mp);
-                    const float f = lp == 0.f ? 0.f : __builtin_amdgcn_exp2f(mp - top);
-                    const float L = wave_sum(lp == 0.f ? 0.f : f * lp);
-                    if (lane < pieces) w_lds[lane][hd] = f;
-                    if (lane == 0) ml_lds[0][hd][0] = L == 0.f ? 0.f : 1.f / L;
-                }
-                __syncthreads();
-                for (int e = 2 * tid; e < heads * D; e += 2 * MXD_THREADS) {
-                    const int hd = e / D;
-                    float y0 = 0.f, y1 = 0.f;
-                    for (int p0 = 0; p0 < pieces; p0 += 8) {
-                        uint64_t w[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            w[k] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(
-                                                         a.part_o + slot_of(min(p0 + k, pieces - 1)) * (MXD_HEADS * D) + e),
-                                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float f = p0 + k < pieces ? w_lds[p0 + k][hd] : 0.f;
-                            if (f != 0.f) {   // a piece that saw nothing adds nothing, NaN goes on
-                                y0 += f * __uint_as_float(static_cast<uint32_t>(w[k]));
-                                y1 += f * __uint_as_float(static_cast<uint32_t>(w[k] >> 32));
-                            }
-                        }
-                    }
-                    const float inv = ml_lds[0][hd][0];
-                    *reinterpret_cast<uint32_t*>(a.out + q_row * D + e) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
-                }
-            }
+        if (piece.count > 1) {
+            if (row.lo == 0) tail = piece;
+            else head = piece;
         }
         __syncthreads();   // LDS is free for the next row
         row = nxt;
+    }
+
+    // ---- the share's (at most two) pieces of cut rows are counted; whoever completes
+    // a row adds its pieces ----
+    if (head.count == 0 && tail.count == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's stores have arrived
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t n0 = 0, n1 = 0;
+        if (head.count) n0 = __hip_atomic_fetch_add(a.counters + head.first_wg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tail.count) n1 = __hip_atomic_fetch_add(a.counters + tail.first_wg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_lds[0] = head.count && n0 + 1 == static_cast<uint32_t>(head.count);
+        last_lds[1] = tail.count && n1 + 1 == static_cast<uint32_t>(tail.count);
+    }
+    __syncthreads();
+    for (int side = 0; side < 2; ++side) {
+        if (!last_lds[side]) continue;   // uniform
+        const Piece x = side ? tail : head;
+        int heads;
+        const int64_t q_row = q_row_of(x.s, x.r, heads);
+        if (tid == 0) __hip_atomic_store(a.counters + x.first_wg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // piece p's slot: the row starts in its first workgroup's last piece
+        // (slot 2 wg + 1) and goes on in the others' first
+        auto slot_of = [&](int p) __attribute__((always_inline)) { return 2 * static_cast<int64_t>(x.first_wg + p) + (p == 0 ? 1 : 0); };
+        // the first pieces' outputs travel with the factors
+        const int e0 = 2 * tid;
+        float u[8], v[8];
+        auto load8 = [&](int p0, int e) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                load2(a.part_o + slot_of(min(p0 + k, x.count - 1)) * (MXD_HEADS * D) + e, u[k], v[k]);
+        };
+        if (e0 < heads * D) load8(0, e0);
+        // a wave a head, a lane a piece: the pieces' factors and the row's sum
+        for (int hd = wave; hd < heads; hd += MXD_WAVES) {
+            float mp = -INFINITY, lp = 0.f;
+            if (lane < x.count) load2(a.part_ml + slot_of(lane) * (2 * MXD_HEADS) + 2 * hd, mp, lp);
+            const float top = wave_max(mp);
+            const float f = lp == 0.f ? 0.f : __builtin_amdgcn_exp2f(mp - top);
+            const float L = wave_sum(lp == 0.f ? 0.f : f * lp);
+            if (lane < x.count) w_lds[lane][hd] = f;
+            if (lane == 0) ml_lds[0][hd][0] = L == 0.f ? 0.f : 1.f / L;
+        }
+        __syncthreads();
+        for (int e = e0; e < heads * D; e += 2 * MXD_THREADS) {
+            const int hd = e / D;
+            float y0 = 0.f, y1 = 0.f;
+            for (int p0 = 0; p0 < x.count; p0 += 8) {
+                if (p0 > 0 || e > e0) load8(p0, e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float f = p0 + k < x.count ? w_lds[p0 + k][hd] : 0.f;
+                    if (f != 0.f) {
+                        y0 += f * u[k];
+                        y1 += f * v[k];
+                    }
+                }
+            }
+            const float inv = ml_lds[0][hd][0];
+            *reinterpret_cast<uint32_t*>(a.out + q_row * D + e) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
+        }
+        __syncthreads();   // before the other row's factors
     }
 }
 
@@ -572,7 +635,7 @@ int32_t mxd_check(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t 
     RLLM_CHECK_ARG(mx4_attention_ok(num_seqs, hq, hkv, bs, maxb));
     // the items of all rows are counted in 32 bits
     const int64_t rows = num_seqs * hkv * ((hq / hkv + MXD_HEADS - 1) / MXD_HEADS);
-    RLLM_CHECK_ARG(rows * ((maxb * bs + MXD_ITEM - 1) / MXD_ITEM + 1) <= INT32_MAX);
+    RLLM_CHECK_ARG(rows * ((maxb * bs + MXD_ITEM - 1) / MXD_ITEM + 1 + MXD_VIRT) <= INT32_MAX);
     return 0;
 }
 

@@ -217,8 +217,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
     {
         const uint16_t* src = a.q + orow * D;
         uint4 w[NKS][4];
-        float amax = 0.f;
-        bool finite = true;
+        uint32_t amax = 0;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
@@ -226,36 +225,23 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
                 const int d0 = 64 * ks + 32 * (i >> 1) + 16 * hl + 8 * (i & 1);
                 w[ks][i] = make_uint4(0, 0, 0, 0);
                 if (NB % 2 == 0 || 64 * ks + 32 * (i >> 1) < D) w[ks][i] = *reinterpret_cast<const uint4*>(src + d0);
-                const uint32_t u[4] = {w[ks][i].x, w[ks][i].y, w[ks][i].z, w[ks][i].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float lo = QKIND == KIND_BF16 ? bf16_lo(u[k]) : f16_lo(u[k]);
-                    const float hi = QKIND == KIND_BF16 ? bf16_hi(u[k]) : f16_hi(u[k]);
-                    finite = finite && __builtin_fabsf(lo) < INFINITY && __builtin_fabsf(hi) < INFINITY;
-                    amax = fmaxf(amax, fmaxf(__builtin_fabsf(lo), __builtin_fabsf(hi)));
-                }
+                amax = max(amax, mx4_amax8(w[ks][i]));
             }
-        amax = mx4_max_32(finite ? amax : INFINITY);
-        const int byte0 = mx4_query_byte(amax);
-        const int shift = byte0 == 255 ? 0 : 127 - byte0;
+        const int byte0 = mx4_query_byte<QKIND>(mx4_umax_32(amax));
+        const float factor = mx4_query_factor(byte0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) qs[t] = mx4_term_byte(byte0, t);
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t u[4] = {w[ks][i].x, w[ks][i].y, w[ks][i].z, w[ks][i].w};
+                uint32_t x[NT], y[NT];
+                mx4_split4<QKIND>(w[ks][i].x, w[ks][i].y, factor, x);
+                mx4_split4<QKIND>(w[ks][i].z, w[ks][i].w, factor, y);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t v = u[2 * k + e];
-                        x[2 * e] = ldexpf(QKIND == KIND_BF16 ? bf16_lo(v) : f16_lo(v), shift);
-                        x[2 * e + 1] = ldexpf(QKIND == KIND_BF16 ? bf16_hi(v) : f16_hi(v), shift);
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) qt[t][ks][2 * i + k] = static_cast<int>(mx4_term4(x));
+                for (int t = 0; t < NT; ++t) {
+                    qt[t][ks][2 * i] = static_cast<int>(x[t]);
+                    qt[t][ks][2 * i + 1] = static_cast<int>(y[t]);
                 }
             }
     }
