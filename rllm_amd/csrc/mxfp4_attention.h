@@ -150,6 +150,19 @@ __device__ __forceinline__ int mx4_wave_max(int v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+// The softmax's exponents are score * c, c = scale * log2(e) > 0: a negative scale
+// turns the query's sign, and of scale 0 the query is 0 and c 1.
+struct MxScale {
+    uint32_t keep, flip;   // of a packed pair of query elements
+    float c;
+};
+__device__ __forceinline__ MxScale mx4_scale(float c) {
+    return MxScale{c == 0.f ? 0u : 0xffffffffu, c < 0.f ? 0x80008000u : 0u, c == 0.f ? 1.f : __builtin_fabsf(c)};
+}
+__device__ __forceinline__ uint4 mx4_scaled(const uint4& w, const MxScale& x) {
+    return make_uint4((w.x & x.keep) ^ x.flip, (w.y & x.keep) ^ x.flip, (w.z & x.keep) ^ x.flip, (w.w & x.keep) ^ x.flip);
+}
+
 // The power of two of a query row (its largest element in [128, 256)) as the
 // scale byte of its first term, from the row's largest pattern; the terms' bytes are
 // this less 4 each and stay above 0.  255 (NaN) for a row with an infinity or a NaN.

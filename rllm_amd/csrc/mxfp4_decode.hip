@@ -55,7 +55,7 @@ struct MxDecodeArgs {
     int32_t bs, subs;                    // tokens, 16-token parts of a block
     uint64_t subs_mul;                   // ceil(2^32 / subs)
     int32_t maxb;
-    int64_t nb;
+    int32_t nb;
     float c;                             // scale * log2(e)
     uint32_t* counters;                  // [workgroups]
     float* part_o;                       // [2 * workgroups][16][D]
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
     // parts exist (the others point to page 0, and get no weight)
     struct Parts { uint32_t lo, hi; int scales; uint64_t ok; };
     auto resolve = [&](const Ids& x, int h) __attribute__((always_inline)) -> Parts {
-        const bool ok = x.row >= 0 && x.id >= 0 && x.id < a.nb;
+        const bool ok = x.row >= 0 && static_cast<uint32_t>(x.id) < static_cast<uint32_t>(a.nb);
         const int r0 = ok ? x.row : 0;
         const int64_t at = (static_cast<int64_t>(ok ? x.id : 0) * a.hkv + h) * page_bytes + r0 * (D / 2);
         return Parts{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32), code_bytes + r0 * (NB - D / 2),
@@ -713,7 +713,7 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
     a.subs = static_cast<int32_t>(block_size / MX4_TOKENS);
     a.subs_mul = ((uint64_t(1) << 32) + a.subs - 1) / a.subs;   // exact quotients below 2^23
     a.maxb = static_cast<int32_t>(max_num_blocks_per_seq);
-    a.nb = num_blocks;
+    a.nb = static_cast<int32_t>(num_blocks);
     a.c = scale * MX4_LOG2E;
     if (ws) {
         a.counters = static_cast<uint32_t*>(ws);

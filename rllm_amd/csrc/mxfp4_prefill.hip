@@ -25,6 +25,9 @@ namespace {
 
 constexpr int MXP_TILE = 64;    // keys
 constexpr int MXP_SUBS = MXP_TILE / MX4_TOKENS;
+// Rounds of workgroups up to which the query tiles go by falling key counts: with
+// more, the last round is a small part.
+constexpr int MXP_SORTED_ROUNDS = 4;
 
 // 8 waves, two a SIMD, up to head_dim 128; past it a wave needs the registers of two
 template <int NB> constexpr int mxp_waves() { return NB <= 4 ? 8 : 4; }
@@ -36,11 +39,11 @@ struct MxPrefillArgs {
     const int32_t *bt, *seq_lens, *qsl;
     int32_t num_seqs, num_tokens, hq, hkv;
     int32_t bs, subs;       // tokens, 16-token parts of a block
-    uint64_t subs_mul;      // ceil(2^32 / subs)
     int32_t maxb;
-    int64_t nb;
+    int32_t nb;
     float c;                // scale * log2(e)
     int32_t splits, base_wgs;
+    int32_t longest_first;  // query tiles by falling key counts
     float* part_o;          // [num_tokens * hq][splits][D], relative to the part's max
     float* part_ml;         // [num_tokens * hq][splits][2]
 };
@@ -49,33 +52,72 @@ struct MxPrefillArgs {
 // (64 bytes each) on different banks
 template <int NB> constexpr int mxp_row() { return 32 * NB + (NB % 2 ? 0 : 32); }
 
+// Tile `rank` of the batch by falling key counts, in steps of MXP_TILE keys: the
+// workgroups of a launch start in order, so the long ones run first and the short
+// ones fill the last round.  Lane i brings sequence i's new tokens n (nt query tiles)
+// and context ctx.  The step is searched for: a sequence's tiles with more than T steps
+// of keys are its last ones, and their number is a shift away.  -1 past the last tile.
+template <int ROWS>
+__device__ __forceinline__ int mxp_longest(int n, int ctx, int nt, int G, int rank, int& tile) {
+    static_assert((ROWS & (ROWS - 1)) == 0, "tiles are counted by shifts");
+    constexpr int SH = __builtin_ctz(ROWS);
+    ctx = min(max(ctx, 0), 1 << 27);
+    auto above = [&](int steps) __attribute__((always_inline)) {
+        // tile i's last token is (ROWS (i + 1) - 1) / G, and attends it and ctx - n more
+        const int x = min(max(steps * MXP_TILE - (ctx - n), 0), n);
+        return nt > 0 && (ctx > steps * MXP_TILE || steps < 0) ? nt - min(nt - 1, (x * G) >> SH) : 0;
+    };
+    auto all_above = [&](int steps) __attribute__((always_inline)) {
+        return __builtin_amdgcn_readlane(mx4_scan(above(steps)), 63);
+    };
+    int lo = -1, hi = (mx4_wave_max(ctx) + MXP_TILE - 1) / MXP_TILE;   // all_above(lo) counts every tile, (hi) none
+    if (rank >= all_above(lo)) return -1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (all_above(mid) > rank) lo = mid;
+        else hi = mid;
+    }
+    const int longer = above(hi), band = above(lo) - longer;
+    const int r = rank - all_above(hi);
+    const int before = mx4_scan(band) - band;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(before <= r && r < before + band);
+    const int s = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+    tile = __builtin_amdgcn_readlane(nt - longer - 1 - (r - before), s);
+    return s;
+}
+
+// LDS: K codes of two tiles, V rows of two, and beside them K's scales and marks of
+// NaN blocks of V (a tile's number where it has one).
 template <int NB>
-struct MxTile {   // one buffer
-    uint4 k[NB][MXP_TILE];
-    uint16_t v[MXP_TILE][mxp_row<NB>()];
-    uint8_t ke[NB][MXP_TILE];
-    uint8_t bad[NB][MXP_TILE];   // V blocks that are NaN
-    int32_t bad_tile;            // the last tile here that had one
+struct MxTiles {
+    uint4 k[2][NB][MXP_TILE];
+    uint16_t v[2][MXP_TILE][mxp_row<NB>()];
+    uint8_t ke[2][NB][MXP_TILE];
+    uint8_t bad[2][NB][MXP_TILE];
+    int32_t bad_tile[2];
 };
 
 template <int QKIND, int NB>
-__global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void mx4_prefill_kernel(
+__global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4_prefill_kernel(
     MxPrefillArgs a, const int32_t* __restrict__ bt) {
-    constexpr int D = 32 * NB, WAVES = mxp_waves<NB>(), THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+    constexpr int D = 32 * NB, WAVES = mxp_waves<NB>(), ROWS = 32 * WAVES;
+    constexpr int GROUP = 64 * (WAVES / 2);       // threads of a group
     constexpr int NKS = (NB + 1) / 2;             // 64-wide steps of head_dim
     constexpr int NT = mx4_terms<QKIND>();
     constexpr int PT = QKIND == KIND_BF16 ? 1 : 2;   // terms of a weight
-    constexpr int CHUNKS = 2 * MXP_TILE * NB;     // 16-byte chunks of a tile, K's then V's
-    constexpr int NCH = (CHUNKS + THREADS - 1) / THREADS;
+    constexpr int CHUNKS = MXP_TILE * NB;         // 16-byte chunks of a tile's K (V): group 1 (0) copies them
+    constexpr int NCH = (CHUNKS + GROUP - 1) / GROUP;
     constexpr int ROW = mxp_row<NB>();
-    __shared__ __align__(16) MxTile<NB> tiles[2];
+    constexpr int RING = NB <= 4 ? 2 : 1;         // V operands in registers: steps
+    __shared__ __align__(16) MxTiles<NB> tiles;
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int grp = wave / (WAVES / 2), gtid = tid - grp * GROUP;
     const int l32 = lane & 31, hl = lane >> 5;
     const int G = a.hq / a.hkv;
 
-    // ---- which (kv head, sequence, query tile): a sequence's last tile first ----
+    // ---- which (kv head, sequence, query tile) ----
     const int base = a.splits > 1 ? blockIdx.x % a.base_wgs : blockIdx.x;
     const int split = a.splits > 1 ? blockIdx.x / a.base_wgs : 0;
     const int h = base % a.hkv;
@@ -87,7 +129,17 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
             q0_l = min(max(a.qsl[s0 + lane], 0), a.num_tokens);
             n_l = min(max(a.qsl[s0 + lane + 1], q0_l), a.num_tokens) - q0_l;
         }
-        const int nt_l = static_cast<int>((static_cast<int64_t>(n_l) * G + ROWS - 1) / ROWS);
+        const int nt_l = (n_l * G + ROWS - 1) / ROWS;
+        if (a.longest_first) {   // at most 64 sequences
+            const int ctx_l = s0 + lane < a.num_seqs ? a.seq_lens[s0 + lane] : 0;
+            s = mxp_longest<ROWS>(n_l, ctx_l, nt_l, G, j, tile);
+            if (s >= 0) {
+                q0 = __builtin_amdgcn_readlane(q0_l, s);
+                n = __builtin_amdgcn_readlane(n_l, s);
+            }
+            break;
+        }
+        // sequence by sequence, a sequence's last tile (the most keys) first
         const int incl = mx4_scan(nt_l);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(incl - nt_l <= j && j < incl);
         if (hit) {
@@ -121,64 +173,84 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
     // the smallest position among the wave's rows: its first row's
     const int min_pos = __builtin_amdgcn_readfirstlane(pos);
 
-    // ---- staging ----
+    // ---- copies: group 0 brings V, group 1 K.  A thread's chunks are 16 bytes of codes
+    // and their scale; its table entries are loaded a tile before the chunks ----
     const int64_t page_bytes = mx4_page_bytes(D, a.bs);
     const int code_bytes = a.bs * (D / 2);
     const int32_t* bt_row = bt + static_cast<int64_t>(s) * a.maxb;
-    struct Ids { int id[MXP_SUBS]; int row[MXP_SUBS]; };
-    auto load_ids = [&](int t, Ids& x) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < MXP_SUBS; ++i) {
-            const int u = t * MXP_SUBS + i;
-            const int blk = static_cast<int>((static_cast<uint32_t>(u) * a.subs_mul) >> 32);
-            const bool in = u * MX4_TOKENS < kv_end;
-            const int id = in ? bt_row[min(blk, a.maxb - 1)] : -1;
-            x.id[i] = id >= 0 && id < a.nb ? id : -1;
-            x.row[i] = in ? (u - blk * a.subs) * MX4_TOKENS : 0;
-        }
+    const uint8_t* const cache = (grp == 0 ? a.vc : a.kc) + h * page_bytes;
+    const uint64_t block_bytes = static_cast<uint64_t>(a.hkv) * page_bytes;
+    // A place in the context: the 16-token part `rem` of table entry `blk`.  Four parts
+    // (a tile) further on by additions alone: this runs every tile, and integer
+    // products take four issue slots.
+    struct Place { int blk, rem; };
+    const int adv_blk = MXP_SUBS / a.subs, adv_rem = MXP_SUBS % a.subs;
+    auto place_of = [&](int u) __attribute__((always_inline)) { return Place{u / a.subs, u % a.subs}; };
+    auto advance = [&](Place& x) __attribute__((always_inline)) {
+        x.rem += adv_rem;
+        const bool over = x.rem >= a.subs;
+        x.rem -= over ? a.subs : 0;
+        x.blk += adv_blk + (over ? 1 : 0);
     };
-    auto presence = [&](const Ids& x) __attribute__((always_inline)) {
-        uint32_t m = 0;
+    // this thread's chunks: their places in the tile whose entries are loaded next and,
+    // for part lane % 4, what says whether it exists
+    Place at[NCH], at_part;
+    int id[NCH], id_part, rem[NCH];   // entries as loaded, and the chunks' parts of them
+    const int part = lane & (MXP_SUBS - 1);
+    auto begin_ids = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < MXP_SUBS; ++i) m |= x.id[i] >= 0 ? 1u << i : 0u;
-        return m;
+        for (int c = 0; c < NCH; ++c)
+            at[c] = place_of(t * MXP_SUBS + min((c * GROUP + gtid) / (MX4_TOKENS * NB), MXP_SUBS - 1));
+        at_part = place_of(t * MXP_SUBS + part);
     };
-    struct Raw { uint4 w[NCH]; uint32_t e[NCH]; };
-    auto fetch = [&](int t, const Ids& x, Raw& r) __attribute__((always_inline)) {
+    auto load_ids = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int idx = c * THREADS + tid;
-            const bool is_v = idx >= MXP_TILE * NB;
-            const int at = is_v ? idx - MXP_TILE * NB : idx;
-            const int sub = min(at / (MX4_TOKENS * NB), MXP_SUBS - 1), off = at - sub * (MX4_TOKENS * NB);
-            int id = x.id[0], r0 = x.row[0];
+            id[c] = bt_row[min(at[c].blk, a.maxb - 1)];
+            rem[c] = at[c].rem;
+            advance(at[c]);
+        }
+        id_part = bt_row[min(at_part.blk, a.maxb - 1)];
+        advance(at_part);
+    };
+    // bit i: part i of tile t exists
+    auto presence = [&](int t) __attribute__((always_inline)) {
+        const bool ok = static_cast<uint32_t>(id_part) < static_cast<uint32_t>(a.nb) && (t * MXP_SUBS + part) * MX4_TOKENS < kv_end;
+        return static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok)) & ((1u << MXP_SUBS) - 1);
+    };
+    // a chunk's byte offsets in its part's codes and scales, and its key in the tile
+    int c_off[NCH], c_key[NCH];
 #pragma unroll
-            for (int i = 1; i < MXP_SUBS; ++i) {
-                id = sub == i ? x.id[i] : id;
-                r0 = sub == i ? x.row[i] : r0;
-            }
+    for (int c = 0; c < NCH; ++c) {
+        const int idx = c * GROUP + gtid;
+        c_off[c] = idx % (MX4_TOKENS * NB);
+        c_key[c] = CHUNKS % GROUP == 0 || idx < CHUNKS ? idx / NB : 1 << 30;   // past any context
+    }
+    struct Raw { uint4 w[NCH]; uint32_t e[NCH]; };
+    auto fetch = [&](int t, Raw& r) __attribute__((always_inline)) {
+        const int room = kv_end - t * MXP_TILE;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
             r.w[c] = make_uint4(0, 0, 0, 0);
             r.e[c] = 127;
             // rows past the keys any query here sees may hold anything: zeros
-            const int key = t * MXP_TILE + sub * MX4_TOKENS + off / NB;
-            if ((CHUNKS % THREADS == 0 || idx < CHUNKS) && id >= 0 && key < kv_end) {
-                const uint8_t* page = (is_v ? a.vc : a.kc) + (static_cast<int64_t>(id) * a.hkv + h) * page_bytes;
-                r.w[c] = *reinterpret_cast<const uint4*>(page + r0 * (D / 2) + 16 * off);
-                r.e[c] = page[code_bytes + r0 * NB + off];
+            if (static_cast<uint32_t>(id[c]) < static_cast<uint32_t>(a.nb) && c_key[c] < room) {
+                const uint8_t* page = cache + static_cast<uint64_t>(static_cast<uint32_t>(id[c])) * block_bytes;
+                r.w[c] = *reinterpret_cast<const uint4*>(page + (rem[c] * (MX4_TOKENS * D / 2) + 16 * c_off[c]));
+                r.e[c] = page[code_bytes + rem[c] * (MX4_TOKENS * NB) + c_off[c]];
             }
         }
     };
-    auto store = [&](int t, const Raw& r, MxTile<NB>& buf) __attribute__((always_inline)) {
+    auto store = [&](int t, const Raw& r) __attribute__((always_inline)) {
+        const int buf = (t - t_lo) & 1;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const int idx = c * THREADS + tid;
-            if (CHUNKS % THREADS != 0 && idx >= CHUNKS) continue;
-            const bool is_v = idx >= MXP_TILE * NB;
-            const int at = is_v ? idx - MXP_TILE * NB : idx;
-            const int key = at / NB, b = at % NB;
-            if (!is_v) {
-                buf.k[b][key] = r.w[c];
-                buf.ke[b][key] = static_cast<uint8_t>(r.e[c]);
+            const int idx = c * GROUP + gtid;
+            if (CHUNKS % GROUP != 0 && idx >= CHUNKS) continue;
+            const int key = idx / NB, b = idx % NB;
+            if (grp == 1) {
+                tiles.k[buf][b][key] = r.w[c];
+                tiles.ke[buf][b][key] = static_cast<uint8_t>(r.e[c]);
             } else {
                 // A NaN block enters as zeros and marks its token: a weight of 0
                 // for a key that a row does not see would not keep it out.
@@ -188,26 +260,42 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
                 // 16-byte chunk i of block b lies at i ^ (b % 4): the 16 lanes of a
                 // store (4 keys x 4 blocks, rows 64 bytes apart in the banks) then
                 // cover all banks
-                uint4* dst = reinterpret_cast<uint4*>(&buf.v[key][32 * b]);
+                uint4* dst = reinterpret_cast<uint4*>(&tiles.v[buf][key][32 * b]);
                 const int sw = b & 3;
                 dst[0 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.x, f), mx4_dec_bf16<1>(w.x, f), mx4_dec_bf16<2>(w.x, f), mx4_dec_bf16<3>(w.x, f));
                 dst[1 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.y, f), mx4_dec_bf16<1>(w.y, f), mx4_dec_bf16<2>(w.y, f), mx4_dec_bf16<3>(w.y, f));
                 dst[2 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.z, f), mx4_dec_bf16<1>(w.z, f), mx4_dec_bf16<2>(w.z, f), mx4_dec_bf16<3>(w.z, f));
                 dst[3 ^ sw] = make_uint4(mx4_dec_bf16<0>(w.w, f), mx4_dec_bf16<1>(w.w, f), mx4_dec_bf16<2>(w.w, f), mx4_dec_bf16<3>(w.w, f));
-                buf.bad[b][key] = bad;
-                if (bad) buf.bad_tile = t;
+                tiles.bad[buf][b][key] = bad;
+                if (bad) tiles.bad_tile[buf] = t;
             }
         }
     };
-    if (tid == 0) tiles[0].bad_tile = tiles[1].bad_tile = -1;
 
-    Ids ids;
+    // presences of the tiles ahead, four bits each
+    uint32_t ring = 0;
+    auto note = [&](int t) __attribute__((always_inline)) {
+        const int sh = 4 * ((t - t_lo) & 7);
+        ring = (ring & ~(15u << sh)) | presence(t) << sh;
+    };
+    // the next tile's copy: stored from its registers, the one after it fetched and the
+    // table entries of one more asked for
     Raw raw;
-    uint32_t present = 0, next_present = 0;
+    auto copy = [&](int t) __attribute__((always_inline)) {
+        if (t < t_hi) store(t, raw);
+        if (t + 1 < t_hi) {
+            fetch(t + 1, raw);
+            note(t + 1);
+            if (t + 2 < t_hi) load_ids();
+        }
+    };
+    if (tid == 0) tiles.bad_tile[0] = tiles.bad_tile[1] = -1;
     if (t_lo < t_hi) {
-        load_ids(t_lo, ids);
-        fetch(t_lo, ids, raw);
-        present = presence(ids);
+        begin_ids(t_lo);
+        load_ids();
+        fetch(t_lo, raw);
+        note(t_lo);
+        if (t_lo + 1 < t_hi) load_ids();
     }
 
     // ---- the query row as E4M3 terms: lane group hl holds elements 16 hl.. and
@@ -216,6 +304,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
     int qs[NT];
     {
         const uint16_t* src = a.q + orow * D;
+        const MxScale sign = mx4_scale(a.c);
         uint4 w[NKS][4];
         uint32_t amax = 0;
 #pragma unroll
@@ -226,6 +315,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
                 w[ks][i] = make_uint4(0, 0, 0, 0);
                 if (NB % 2 == 0 || 64 * ks + 32 * (i >> 1) < D) w[ks][i] = *reinterpret_cast<const uint4*>(src + d0);
                 amax = max(amax, mx4_amax8(w[ks][i]));
+                w[ks][i] = mx4_scaled(w[ks][i], sign);
             }
         const int byte0 = mx4_query_byte<QKIND>(mx4_umax_32(amax));
         const float factor = mx4_query_factor(byte0);
@@ -252,118 +342,170 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
     float m = -INFINITY, l = 0.f;   // l: this lane's keys only
     uint32_t nan_blocks = 0;        // output blocks made NaN by a value the row sees
 
-    __syncthreads();   // bad_tile is set
-    if (t_lo < t_hi) store(t_lo, raw, tiles[0]);
-    if (t_lo + 1 < t_hi) {
-        load_ids(t_lo + 1, ids);
-        fetch(t_lo + 1, ids, raw);
-        next_present = presence(ids);
-    }
-    __syncthreads();
+    const float c = mx4_scale(a.c).c;
+    mx_f32x16 st[2];               // S^T of the tile's 32-key halves
+    uint32_t p[PT][2][8];          // the weights, packed pairs, same order
 
     // transposing V read: row 4 hl + (lane % 16) / 4, 16 elements from 16 ((lane / 16) & 1) of a block
     const int v_row = 4 * hl + ((lane & 15) >> 2);
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_in = 4 * (lane & 1);
 
-    for (int t = t_lo; t < t_hi; ++t) {
-        MxTile<NB>& buf = tiles[(t - t_lo) & 1];
-        if (wave_live) {
-            // ---- scores ----
-            mx_f32x16 st[2];
+    // ---- products ----
+    auto load_v = [&](int t, int k16, uint4 (&v)[NB]) __attribute__((always_inline)) {
+        const uint16_t* base = &tiles.v[(t - t_lo) & 1][16 * k16 + v_row][v_in];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                st[half] = mx_f32x16{};
+        for (int dt = 0; dt < NB; ++dt) {
+            const uint16_t* src = base + 32 * dt + 8 * (v_chunk ^ (dt & 3));
+            const uint2 v0 = mx4_read_tr16(src), v1 = mx4_read_tr16(src + 8 * ROW);
+            v[dt] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+        }
+    };
+    struct KOp { uint4 k[2]; int e[2]; };   // both halves of a 64-wide step
+    auto load_k = [&](int t, int ks, KOp& x) __attribute__((always_inline)) {
+        const int buf = (t - t_lo) & 1, b = 2 * ks + hl;
+        const bool have = NB % 2 == 0 || b < NB;
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) {
-                    const int b = 2 * ks + hl;
-                    const bool have = NB % 2 == 0 || b < NB;
-                    const uint4 kk = buf.k[have ? b : 0][32 * half + l32];
-                    const int e = have ? buf.ke[b][32 * half + l32] : 127;
+        for (int half = 0; half < 2; ++half) {
+            x.k[half] = tiles.k[buf][have ? b : 0][32 * half + l32];
+            x.e[half] = have ? tiles.ke[buf][b][32 * half + l32] : 127;
+        }
+    };
+    // O^T += V^T P^T over tile t, 16 keys a step; operands are read a step ahead
+    auto values = [&](int t, auto&& last) __attribute__((always_inline)) {
+        uint4 v[RING][NB];
+        if constexpr (RING == 2) load_v(t, 0, v[0]);
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) st[half] = mx4_mma32(kk, qt[i][ks], st[half], e, qs[i]);
-                }
+        for (int k16 = 0; k16 < MXP_TILE / 16; ++k16) {
+            if constexpr (RING == 1) load_v(t, k16, v[0]);
+            else if (k16 + 1 < MXP_TILE / 16) load_v(t, k16 + 1, v[(k16 + 1) & 1]);
+            if (k16 + 1 == MXP_TILE / 16) last();
+            if constexpr (RING == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < PT; ++i) {
+                const uint32_t* w = &p[i][k16 >> 1][4 * (k16 & 1)];
+                const uint4 pb = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int dt = 0; dt < NB; ++dt) o[dt] = mx4_mma32_bf16(v[k16 % RING][dt], pb, o[dt]);
             }
-            const int t0 = t * MXP_TILE;
-            const bool full = present == (1u << MXP_SUBS) - 1 && t0 + MXP_TILE <= kv_end && t0 + MXP_TILE - 1 <= min_pos;
-            float sc[2][16];
+        }
+    };
+    int bad_before = -1;   // bad_tile of the tile before, read where LDS is waited for anyway
+    auto products = [&](int t) __attribute__((always_inline)) {
+        KOp k[2];
+        if (t > t_lo) values(t - 1, [&]() __attribute__((always_inline)) { load_k(t, 0, k[0]); });
+        else load_k(t, 0, k[0]);
+        bad_before = tiles.bad_tile[(t - 1 - t_lo) & 1];
+        st[0] = st[1] = mx_f32x16{};
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+        for (int ks = 0; ks < NKS; ++ks) {
+            if (ks + 1 < NKS) load_k(t, ks + 1, k[(ks + 1) & 1]);
+            if constexpr (RING == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sc[half][i] = st[half][i] * a.c;
-            if (!full) {
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
+                    st[half] = mx4_mma32(k[ks & 1].k[half], qt[i][ks], st[half], k[ks & 1].e[half], qs[i]);
+        }
+    };
+    // value blocks of tile t that are NaN in a row that sees them
+    auto mark_nan = [&](int t, int bad_tile) __attribute__((always_inline)) {
+        const int buf = (t - t_lo) & 1;
+        if (t < t_lo || bad_tile != t) return;
+        for (int key = 0; key < MXP_TILE; ++key)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = 32 * half + 8 * (i >> 2) + 4 * hl + (i & 3);
-                        const bool ok = ((present >> (key >> 4)) & 1u) && t0 + key <= pos && t0 + key < kv_end;
-                        sc[half][i] = ok ? sc[half][i] : -INFINITY;
-                    }
-            }
-            if (buf.bad_tile == t) {
-                for (int key = 0; key < MXP_TILE; ++key)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        nan_blocks |= t0 + key <= pos ? static_cast<uint32_t>(buf.bad[b][key]) << b : 0u;
-            }
-            // ---- weights against a max that moves only when passed by 2^8 ----
-            float top = sc[0][0];
+            for (int b = 0; b < NB; ++b)
+                nan_blocks |= t * MXP_TILE + key <= pos ? static_cast<uint32_t>(tiles.bad[buf][b][key]) << b : 0u;
+    };
+    // ---- scores of tile t -> weights against the max as it stands, which moves only when
+    // a lane's weights sum past 2^8: the tile's own max is not looked for before ----
+    auto mask = [&](int t) __attribute__((always_inline)) {
+        const int t0 = t * MXP_TILE;
+        const uint32_t present = ring >> (4 * ((t - t_lo) & 7)) & ((1u << MXP_SUBS) - 1);
+        const bool full = present == (1u << MXP_SUBS) - 1 && t0 + MXP_TILE <= kv_end && t0 + MXP_TILE - 1 <= min_pos;
+        if (!full) {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[half][i]);
-            if (__builtin_amdgcn_ballot_w64(top > m + 8.f || m == -INFINITY)) {
-                const float m_new = fmaxf(m, mx4_max_32(top));
-                const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-                l *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < NB; ++dt) o[dt] *= alpha;
-                m = m_new;
-            }
-            const float mb = m == -INFINITY ? 0.f : m;
-            uint32_t p[PT][2][8];
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(sc[half][2 * i] - mb);
-                    const float p1 = __builtin_amdgcn_exp2f(sc[half][2 * i + 1] - mb);
-                    sum0 += p0;
-                    sum1 += p1;
-                    p[0][half][i] = mx4_pack_bf16(p0, p1);
-                    if constexpr (PT == 2)
-                        p[1][half][i] = mx4_pack_bf16(p0 - bf16_lo(p[0][half][i]), p1 - bf16_hi(p[0][half][i]));
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * half + 8 * (i >> 2) + 4 * hl + (i & 3);
+                    const bool ok = ((present >> (key >> 4)) & 1u) && t0 + key <= pos && t0 + key < kv_end;
+                    st[half][i] = ok ? st[half][i] : -INFINITY;
                 }
-            l += sum0 + sum1;
-            // ---- O^T += V^T P^T, 16 keys a step ----
-#pragma unroll
-            for (int k16 = 0; k16 < MXP_TILE / 16; ++k16) {
-                uint4 pb[PT];
-#pragma unroll
-                for (int i = 0; i < PT; ++i) {
-                    const uint32_t* w = &p[i][k16 >> 1][4 * (k16 & 1)];
-                    pb[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-#pragma unroll
-                for (int dt = 0; dt < NB; ++dt) {
-                    const uint16_t* src = &buf.v[16 * k16 + v_row][32 * dt + 8 * (v_chunk ^ (dt & 3)) + v_in];
-                    const uint2 v0 = mx4_read_tr16(src), v1 = mx4_read_tr16(src + 8 * ROW);
-                    const uint4 vv = make_uint4(v0.x, v0.y, v1.x, v1.y);
-#pragma unroll
-                    for (int i = 0; i < PT; ++i) o[dt] = mx4_mma32_bf16(vv, pb[i], o[dt]);
-                }
-            }
         }
-        MxTile<NB>& next = tiles[(t - t_lo + 1) & 1];
-        if (t + 1 < t_hi) store(t + 1, raw, next);
-        present = next_present;
-        if (t + 2 < t_hi) {
-            load_ids(t + 2, ids);
-            fetch(t + 2, ids, raw);
-            next_present = presence(ids);
-        }
+    };
+    auto rescale = [&]() __attribute__((always_inline)) {
+        float top = st[0][0];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, st[half][i]);
+        const float m_new = fmaxf(m, mx4_max_32(top));
+        const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NB; ++dt) o[dt] *= alpha;
+        m = m_new;
+    };
+    auto weights = [&]() __attribute__((always_inline)) -> float {   // their sum
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[half][2 * i], c, -mc));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[half][2 * i + 1], c, -mc));
+                sum0 += p0;
+                sum1 += p1;
+                p[0][half][i] = mx4_pack_bf16(p0, p1);
+                if constexpr (PT == 2) p[1][half][i] = mx4_pack_bf16(p0 - bf16_lo(p[0][half][i]), p1 - bf16_hi(p[0][half][i]));
+            }
+        return sum0 + sum1;
+    };
+
+    // ---- the turns.  In turn 2t group 0 issues tile t's products (and tile t-1's
+    // V products), in turn 2t + 1 its softmax and the copy of V(t); group 1 is one turn
+    // behind, with the copy of K(t + 2).  On every SIMD a wave of one group then keeps the
+    // matrix core while the other's works on the vector units.  K(t) is read in turns 2t
+    // and 2t + 1, V(t) in 2t + 2 and 2t + 3; K(t + 2) is written over K(t) in turn 2t + 2, V(t)
+    // over V(t - 2) in turn 2t + 1. ----
+    if (t_lo < t_hi) {
+        if (grp == 1) copy(t_lo);
         __syncthreads();
+        if (grp == 1) {   // while group 0 begins
+            copy(t_lo + 1);
+            __syncthreads();
+        }
+        // A tile that moves the max leaves the loop and comes back: a rescale in its body
+        // has the compiler copy the accumulators between two sets of registers every tile.
+        for (int t = t_lo; t < t_hi;) {
+            bool moves = false;
+            for (; t < t_hi; ++t) {
+                if (wave_live) products(t);
+                __syncthreads();
+                if (wave_live) {
+                    mark_nan(t - 1, bad_before);
+                    mask(t);
+                    const float sum = weights();
+                    moves = __builtin_amdgcn_ballot_w64(!(sum <= 256.f) || m == -INFINITY);
+                    if (moves) break;
+                    l += sum;
+                }
+                copy(grp == 0 ? t : t + 2);
+                __syncthreads();
+            }
+            if (!moves) break;
+            rescale();
+            l += weights();
+            copy(grp == 0 ? t : t + 2);
+            __syncthreads();
+            ++t;
+        }
+        if (grp == 0) __syncthreads();   // group 1's last softmax
+        if (wave_live) {
+            mark_nan(t_hi - 1, tiles.bad_tile[(t_hi - 1 - t_lo) & 1]);
+            values(t_hi - 1, [] {});
+        }
     }
     if (!wave_live) return;   // no barrier follows
 
@@ -381,7 +523,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), 8 / (NB <= 4 ? 4 : 8)) void m
                 if ((nan_blocks >> dt) & 1u) y = mx_f32x4{nan, nan, nan, nan};
                 *reinterpret_cast<mx_f32x4*>(dst + 32 * dt + 8 * jj) = y;
             }
-        if (hl == 0) *reinterpret_cast<mx_f32x2*>(a.part_ml + 2 * slot) = mx_f32x2{m, l};
+        if (hl == 0) *reinterpret_cast<mx_f32x2*>(a.part_ml + 2 * slot) = mx_f32x2{m * c, l};
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -464,8 +606,8 @@ extern "C" int32_t rllm_paged_attention_prefill_mxfp4(
     RLLM_CHECK_ARG(mx4_aligned16(key_cache) && mx4_aligned16(value_cache) && mx4_aligned16(query));
     RLLM_CHECK_ARG((reinterpret_cast<uintptr_t>(output) & 7) == 0);
     const int64_t group = num_q_heads / num_kv_heads, rows_wg = head_dim <= 128 ? 256 : 128;
-    // a sequence's tiles are at most rows / rows_wg + 1; workgroups past the last find none
-    const int64_t wgs = (num_tokens * group / rows_wg + num_seqs) * num_kv_heads;
+    // ceil(r / rows_wg) <= (r - 1) / rows_wg + 1 for every r >= 0; workgroups past the last tile find none
+    const int64_t wgs = ((num_tokens * group - num_seqs) / rows_wg + num_seqs) * num_kv_heads;
     RLLM_CHECK_ARG(wgs <= INT32_MAX);
     MxPrefillArgs a{};
     a.out = static_cast<uint16_t*>(output);
@@ -481,9 +623,8 @@ extern "C" int32_t rllm_paged_attention_prefill_mxfp4(
     a.hkv = static_cast<int32_t>(num_kv_heads);
     a.bs = static_cast<int32_t>(block_size);
     a.subs = static_cast<int32_t>(block_size / MX4_TOKENS);
-    a.subs_mul = ((uint64_t(1) << 32) + a.subs - 1) / a.subs;   // exact quotients below 2^23
     a.maxb = static_cast<int32_t>(max_num_blocks_per_seq);
-    a.nb = num_blocks;
+    a.nb = static_cast<int32_t>(num_blocks);
     a.c = scale * MX4_LOG2E;
     a.base_wgs = static_cast<int32_t>(wgs);
     a.splits = 1;
@@ -492,6 +633,7 @@ extern "C" int32_t rllm_paged_attention_prefill_mxfp4(
     RLLM_TRY(hipGetDevice(&dev));
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t tiles = (max_num_blocks_per_seq * block_size + MXP_TILE - 1) / MXP_TILE;
+    a.longest_first = num_seqs > 1 && num_seqs <= 64 && wgs > cus && wgs <= MXP_SORTED_ROUNDS * cus;
     int64_t splits = cus / wgs;
     if (splits > tiles / 4) splits = tiles / 4;
     if (splits > 64) splits = 64;
