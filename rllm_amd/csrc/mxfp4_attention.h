@@ -120,6 +120,12 @@ __device__ __forceinline__ float mx4_sum_32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// x: a of lanes < 32, then b of lanes < 32; y: a of lanes >= 32, then b of lanes >= 32
+__device__ __forceinline__ void mx4_swap_32(uint32_t a, uint32_t b, uint32_t& x, uint32_t& y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    x = r[0];
+    y = r[1];
+}
 __device__ __forceinline__ float mx4_max_16(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return mx4_max_32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));

@@ -108,7 +108,6 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
     constexpr int CHUNKS = MXP_TILE * NB;         // 16-byte chunks of a tile's K (V): group 1 (0) copies them
     constexpr int NCH = (CHUNKS + GROUP - 1) / GROUP;
     constexpr int ROW = mxp_row<NB>();
-    constexpr int RING = NB <= 4 ? 2 : 1;         // V operands in registers: steps
     __shared__ __align__(16) MxTiles<NB> tiles;
 
     const int tid = threadIdx.x;
@@ -370,47 +369,42 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
             x.e[half] = have ? tiles.ke[buf][b][32 * half + l32] : 127;
         }
     };
-    // O^T += V^T P^T over tile t, 16 keys a step; operands are read a step ahead
-    auto values = [&](int t, auto&& last) __attribute__((always_inline)) {
-        uint4 v[RING][NB];
-        if constexpr (RING == 2) load_v(t, 0, v[0]);
+    // O^T += V^T P^T over tile t, 16 keys a step
+    auto values = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int k16 = 0; k16 < MXP_TILE / 16; ++k16) {
-            if constexpr (RING == 1) load_v(t, k16, v[0]);
-            else if (k16 + 1 < MXP_TILE / 16) load_v(t, k16 + 1, v[(k16 + 1) & 1]);
-            if (k16 + 1 == MXP_TILE / 16) last();
-            if constexpr (RING == 2) __builtin_amdgcn_sched_barrier(0);
+            uint4 v[NB];
+            load_v(t, k16, v);
 #pragma unroll
             for (int i = 0; i < PT; ++i) {
                 const uint32_t* w = &p[i][k16 >> 1][4 * (k16 & 1)];
                 const uint4 pb = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
-                for (int dt = 0; dt < NB; ++dt) o[dt] = mx4_mma32_bf16(v[k16 % RING][dt], pb, o[dt]);
+                for (int dt = 0; dt < NB; ++dt) o[dt] = mx4_mma32_bf16(v[dt], pb, o[dt]);
             }
         }
     };
     int bad_before = -1;   // bad_tile of the tile before, read where LDS is waited for anyway
     auto products = [&](int t) __attribute__((always_inline)) {
-        KOp k[2];
-        if (t > t_lo) values(t - 1, [&]() __attribute__((always_inline)) { load_k(t, 0, k[0]); });
-        else load_k(t, 0, k[0]);
+        if (t > t_lo) values(t - 1);
         bad_before = tiles.bad_tile[(t - 1 - t_lo) & 1];
         st[0] = st[1] = mx_f32x16{};
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
-            if (ks + 1 < NKS) load_k(t, ks + 1, k[(ks + 1) & 1]);
-            if constexpr (RING == 2) __builtin_amdgcn_sched_barrier(0);
+            KOp k;
+            load_k(t, ks, k);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                    st[half] = mx4_mma32(k[ks & 1].k[half], qt[i][ks], st[half], k[ks & 1].e[half], qs[i]);
+                    st[half] = mx4_mma32(k.k[half], qt[i][ks], st[half], k.e[half], qs[i]);
         }
+        bad_before = __builtin_amdgcn_readfirstlane(bad_before);
     };
     // value blocks of tile t that are NaN in a row that sees them
-    auto mark_nan = [&](int t, int bad_tile) __attribute__((always_inline)) {
+    auto mark_nan = [&](int t) __attribute__((always_inline)) {
         const int buf = (t - t_lo) & 1;
-        if (t < t_lo || bad_tile != t) return;
+        if (t < t_lo || tiles.bad_tile[buf] != t) return;
         for (int key = 0; key < MXP_TILE; ++key)
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -476,25 +470,25 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
             copy(t_lo + 1);
             __syncthreads();
         }
-        // A tile that moves the max leaves the loop and comes back: a rescale in its body
-        // has the compiler copy the accumulators between two sets of registers every tile.
+        // A tile that moves the max or follows one with NaN values leaves the loop and comes
+        // back: what it needs, in the loop's body, costs every tile 5%.
         for (int t = t_lo; t < t_hi;) {
-            bool moves = false;
+            bool rare = false;
             for (; t < t_hi; ++t) {
                 if (wave_live) products(t);
                 __syncthreads();
                 if (wave_live) {
-                    mark_nan(t - 1, bad_before);
                     mask(t);
                     const float sum = weights();
-                    moves = __builtin_amdgcn_ballot_w64(!(sum <= 256.f) || m == -INFINITY);
-                    if (moves) break;
+                    rare = __builtin_amdgcn_ballot_w64(!(sum <= 256.f) || m == -INFINITY) || bad_before == t - 1;
+                    if (rare) break;
                     l += sum;
                 }
                 copy(grp == 0 ? t : t + 2);
                 __syncthreads();
             }
-            if (!moves) break;
+            if (!rare) break;
+            mark_nan(t - 1);
             rescale();
             l += weights();
             copy(grp == 0 ? t : t + 2);
@@ -503,8 +497,8 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
         }
         if (grp == 0) __syncthreads();   // group 1's last softmax
         if (wave_live) {
-            mark_nan(t_hi - 1, tiles.bad_tile[(t_hi - 1 - t_lo) & 1]);
-            values(t_hi - 1, [] {});
+            mark_nan(t_hi - 1);
+            values(t_hi - 1);
         }
     }
     if (!wave_live) return;   // no barrier follows
@@ -526,16 +520,24 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
         if (hl == 0) *reinterpret_cast<mx_f32x2*>(a.part_ml + 2 * slot) = mx_f32x2{m * c, l};
         return;
     }
+    // lanes l and l + 32 hold the two halves of each 8-element run; swapped in pairs of
+    // runs, lane l stores the whole of the first and lane l + 32 of the second
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* dst = a.out + orow * D + 4 * hl;
+    uint16_t* dst = a.out + orow * D + 8 * hl;
 #pragma unroll
     for (int dt = 0; dt < NB; ++dt) {
         const float f = (nan_blocks >> dt) & 1u ? nan : inv;
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
-            *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * jj) =
-                make_uint2(mx4_pack16<QKIND>(o[dt][4 * jj] * f, o[dt][4 * jj + 1] * f),
-                           mx4_pack16<QKIND>(o[dt][4 * jj + 2] * f, o[dt][4 * jj + 3] * f));
+        for (int jj = 0; jj < 4; jj += 2) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t even = mx4_pack16<QKIND>(o[dt][4 * jj + 2 * i] * f, o[dt][4 * jj + 2 * i + 1] * f);
+                const uint32_t odd = mx4_pack16<QKIND>(o[dt][4 * jj + 4 + 2 * i] * f, o[dt][4 * jj + 5 + 2 * i] * f);
+                mx4_swap_32(even, odd, w[i], w[2 + i]);
+            }
+            *reinterpret_cast<mx_out8*>(dst + 32 * dt + 8 * jj) = mx_out8{w[0], w[1], w[2], w[3]};
+        }
     }
 }
 
