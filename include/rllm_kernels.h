@@ -597,11 +597,12 @@ int32_t rllm_rope_cache_write_mxfp4(void *q_out, const void *q, const void *k, c
  * others (values with scale bytes 253 and 254, which no write makes, count as NaN).
  * workspace: at least rllm_paged_attention_decode_mxfp4_workspace_size(...) bytes,
  * 16-byte aligned, zero-filled before its first such call (each completed call
- * leaves it ready for the next); calls that share it must not overlap in time.
+ * leaves it ready for the next, of any size it is large enough for); calls that
+ * share it must not overlap in time.
  * NULL: a library-owned buffer per (device, stream); a capture on a stream that
  * has none of the size yet runs a workgroup a (sequence, kv head) and needs none.
- * Graphs captured on one stream share its buffer: replay them in order, or give
- * each its own workspace. */
+ * Graphs captured on one stream share its buffer with each other and with eager
+ * calls there: run them in order, or give each its own workspace. */
 int32_t rllm_paged_attention_decode_mxfp4(void *output, const void *query, const uint8_t *key_cache,
                                           const uint8_t *value_cache, const int32_t *block_tables,
                                           const int32_t *seq_lens, int64_t num_seqs,

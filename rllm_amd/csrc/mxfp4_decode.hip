@@ -611,10 +611,11 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
 
 // ---- host ----
 
-// Bytes of the arrival counters, and of all scratch, for `wgs` workgroups.
-int64_t mxd_counter_bytes(int64_t wgs) { return (wgs * 4 + 255) & ~int64_t(255); }
+// The arrival counters have a place of their own at the scratch's start, the same for
+// every call: what one call leaves in its partials never lies under another's counters.
+constexpr int64_t MXD_COUNTER_BYTES = 16384, MXD_MAX_WGS = MXD_COUNTER_BYTES / 4;
 int64_t mxd_scratch_bytes(int64_t wgs, int64_t d) {
-    return mxd_counter_bytes(wgs) + 2 * wgs * MXD_HEADS * (d + 2) * 4;
+    return MXD_COUNTER_BYTES + 2 * wgs * MXD_HEADS * (d + 2) * 4;
 }
 
 // Workgroups: what the device holds, fewer where the tables hold less than one item a wave.
@@ -625,7 +626,8 @@ int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int
     const int64_t groups = (hq / hkv + MXD_HEADS - 1) / MXD_HEADS, rows = num_seqs * hkv * groups;
     const int64_t items = (maxb * bs + MXD_ITEM - 1) / MXD_ITEM;
     const int64_t most = rows * ((items + MXD_WAVES - 1) / MXD_WAVES > 0 ? (items + MXD_WAVES - 1) / MXD_WAVES : 1);
-    const int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d);
+    int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d);
+    if (held > MXD_MAX_WGS) held = MXD_MAX_WGS;
     *wgs = most < held ? most : held;
     return 0;
 }
@@ -717,7 +719,7 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
     a.c = scale * MX4_LOG2E;
     if (ws) {
         a.counters = static_cast<uint32_t*>(ws);
-        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + mxd_counter_bytes(wgs));
+        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + MXD_COUNTER_BYTES);
         a.part_ml = a.part_o + 2 * wgs * MXD_HEADS * head_dim;
     }
     return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16>(a, head_dim, wgs, as_stream(stream))

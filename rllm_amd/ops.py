@@ -351,8 +351,8 @@ def mxfp4_cache(num_blocks: int, num_kv_heads: int, head_dim: int, block_size: i
     return torch.zeros((num_blocks, num_kv_heads, page), dtype=torch.uint8, device=device)
 
 
-def _mxfp4_block_size(k_cache: torch.Tensor, v_cache: torch.Tensor, hkv: int, d: int) -> int:
-    """Block size of a pair of MXFP4 caches of hkv heads and head_dim d."""
+def _check_mxfp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, hkv: int, d: int) -> None:
+    """A pair of MXFP4 caches of hkv heads and head_dim d, or an error."""
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or k_cache.dim() != 3 \
             or k_cache.shape != v_cache.shape:
         raise ValueError("MXFP4 caches are uint8 [num_blocks, Hkv, page] of equal shape")
@@ -360,28 +360,46 @@ def _mxfp4_block_size(k_cache: torch.Tensor, v_cache: torch.Tensor, hkv: int, d:
     bs = k_cache.shape[2] // row if row else 0
     if d % 32 or k_cache.shape[1] != hkv or bs < 16 or bs % 16 or bs * row != k_cache.shape[2]:
         raise ValueError("the caches' heads and page do not fit the heads and head_dim")
-    return bs
+
+
+def _on_current_gpu(*tensors: torch.Tensor) -> bool:
+    """Contiguous tensors of the current device (device numbers as ints: no device objects are made)."""
+    dev = tensors[0].get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        return False
+    for t in tensors:
+        if t.get_device() != dev or not t.is_contiguous():
+            return False
+    return True
+
+
+def _all_dense(*tensors: torch.Tensor) -> None:
+    if not _on_current_gpu(*tensors):
+        raise ValueError("tensors must be contiguous and on the current GPU")
 
 
 def _mxfp4_rows(key, value, k_cache, v_cache, slot_mapping):
     """Checks of the row operators; returns (n, Hkv, D, block size, blocks, dtype code)."""
+    shape, cache = key.shape, k_cache.shape
+    dt = _TORCH_16.get(key.dtype)
+    # at once, as for the other operators; what fails goes on to the error that says which
+    if (dt is not None and len(shape) == 3 and len(cache) == 3 and value.shape == shape and v_cache.shape == cache
+            and value.dtype is key.dtype and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8
+            and slot_mapping.dtype is torch.int64 and slot_mapping.shape == shape[:1]
+            and _on_current_gpu(key, value, k_cache, v_cache, slot_mapping)):
+        n, hkv, d = shape
+        nb, heads, page = cache
+        row = d // 32 * 17
+        if heads == hkv and d % 32 == 0 and row and page % (16 * row) == 0 and page:
+            return n, hkv, d, page // row, nb, dt
     if key.dim() != 3 or value.shape != key.shape:
         raise ValueError("key and value rows must be [num_tokens, Hkv, D] of one shape")
-    n, hkv, d = key.shape
-    bs = _mxfp4_block_size(k_cache, v_cache, hkv, d)
-    dt = _TORCH_16.get(key.dtype)
     if dt is None or value.dtype != key.dtype:
         raise TypeError("key and value rows must be float16 or bfloat16")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (n,):
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != shape[:1]:
         raise ValueError("slot_mapping must be int64 [num_tokens]")
-    return n, hkv, d, bs, k_cache.shape[0], dt
-
-
-def _all_dense(*tensors: torch.Tensor) -> None:
-    if not _dense_on_one_gpu(*tensors):
-        raise ValueError("tensors must be contiguous and on one GPU")
-    if tensors[0].get_device() != torch.cuda.current_device():
-        raise ValueError("the tensors' GPU must be the current device")
+    _check_mxfp4_caches(k_cache, v_cache, shape[1], shape[2])
+    raise ValueError("tensors must be contiguous and on the current GPU")
 
 
 def reshape_and_cache_mxfp4(new_key: torch.Tensor, new_value: torch.Tensor, k_cache: torch.Tensor,
@@ -390,7 +408,6 @@ def reshape_and_cache_mxfp4(new_key: torch.Tensor, new_value: torch.Tensor, k_ca
     """Slot-mapped write into MXFP4 caches, quantising as it writes, through
     rllm_cache_write_mxfp4."""
     n, hkv, d, bs, nb, dt = _mxfp4_rows(new_key, new_value, k_cache, v_cache, slot_mapping)
-    _all_dense(new_key, new_value, k_cache, v_cache, slot_mapping)
     call("rllm_cache_write_mxfp4", _ptr(k_cache), _ptr(v_cache), _ptr(new_key), _ptr(new_value), _ptr(slot_mapping),
          n, hkv, d, bs, nb, dt, _stream(stream))
 
@@ -412,7 +429,6 @@ def read_cache_mxfp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping:
     elif (head_dim is not None and head_dim != out_key.shape[-1]) or (dtype is not None and dtype != out_key.dtype):
         raise ValueError("head_dim and dtype disagree with the outputs")
     n, hkv, d, bs, nb, dt = _mxfp4_rows(out_key, out_value, k_cache, v_cache, slot_mapping)
-    _all_dense(out_key, out_value, k_cache, v_cache, slot_mapping)
     call("rllm_cache_read_mxfp4", _ptr(out_key), _ptr(out_value), _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping),
          n, hkv, d, bs, nb, dt, _stream(stream))
     return out_key, out_value
@@ -431,7 +447,6 @@ def rope_and_cache_mxfp4(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Te
     if cos.dtype != torch.float32 or sin.shape != cos.shape or sin.dtype != cos.dtype \
             or cos.dim() != 2 or cos.shape[1] != d // 2:
         raise ValueError("cos/sin must be float32 [max_position, head_dim // 2]")
-    tensors = [k, v, k_cache, v_cache, slot_mapping, positions, cos, sin]
     hq = 0
     if q is not None:
         if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
@@ -441,10 +456,11 @@ def rope_and_cache_mxfp4(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Te
             q_out = torch.empty_like(q)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out must match q")
-        tensors += [q, q_out]
+        _all_dense(positions, cos, sin, q, q_out)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _all_dense(*tensors)
+    else:
+        _all_dense(positions, cos, sin)
     call("rllm_rope_cache_write_mxfp4", _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache),
          _ptr(slot_mapping), _ptr(positions), _ptr(cos), _ptr(sin), n, hq, hkv, d, bs, nb, cos.shape[0], dt,
          _stream(stream))
@@ -452,25 +468,33 @@ def rope_and_cache_mxfp4(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Te
 
 
 def _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out):
-    """Checks the attention operators share; returns (Hq, Hkv, D, block size, blocks, dtype code, out)."""
+    """Checks the attention operators share; returns (rows, Hq, Hkv, D, sequences,
+    table width, block size, blocks, dtype code, out)."""
+    shape, cache, table = q.shape, k_cache.shape, block_tables.shape
+    dt = _TORCH_16.get(q.dtype)
+    if out is None:
+        out = torch.empty_like(q)
+    if (dt is not None and len(shape) == 3 and len(cache) == 3 and len(table) == 2 and v_cache.shape == cache
+            and out.shape == shape and out.dtype is q.dtype and k_cache.dtype is torch.uint8
+            and v_cache.dtype is torch.uint8 and block_tables.dtype is torch.int32 and seq_lens.dtype is torch.int32
+            and seq_lens.shape == table[:1] and _on_current_gpu(q, k_cache, v_cache, block_tables, seq_lens, out)):
+        rows, hq, d = shape
+        nb, hkv, page = cache
+        row = d // 32 * 17
+        if d % 32 == 0 and row and page % (16 * row) == 0 and page:
+            return rows, hq, hkv, d, table[0], table[1], page // row, nb, dt, out
     if q.dim() != 3 or k_cache.dim() != 3:
         raise ValueError("q [*, Hq, D] and MXFP4 caches [nb, Hkv, page] required")
-    _, hq, d = q.shape
-    hkv = k_cache.shape[1]
-    bs = _mxfp4_block_size(k_cache, v_cache, hkv, d)
-    dt = _TORCH_16.get(q.dtype)
     if dt is None:
         raise TypeError("q must be float16 or bfloat16")
     if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise TypeError("block_tables and seq_lens must be int32")
-    if seq_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0]:
+    if block_tables.dim() != 2 or seq_lens.shape != table[:1]:
         raise ValueError("block_tables [num_seqs, max_blocks] and seq_lens [num_seqs] required")
-    if out is None:
-        out = torch.empty_like(q)
-    elif not _like(out, q):
+    if not _like(out, q):
         raise ValueError("out must be a contiguous tensor like q")
-    _all_dense(q, k_cache, v_cache, block_tables, seq_lens)
-    return hq, hkv, d, bs, k_cache.shape[0], dt, out
+    _check_mxfp4_caches(k_cache, v_cache, cache[1], shape[2])
+    raise ValueError("tensors must be contiguous and on the current GPU")
 
 
 def paged_decode_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -478,8 +502,8 @@ def paged_decode_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                        workspace: Optional[torch.Tensor] = None, validate: bool = True,
                        stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Decode attention over MXFP4 caches through rllm_paged_attention_decode_mxfp4."""
-    hq, hkv, d, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
-    if q.shape[0] != seq_lens.shape[0]:
+    n, hq, hkv, d, b, maxb, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
+    if n != b:
         raise ValueError("one query a sequence required")
     if validate:
         validate_tables(block_tables, seq_lens, nb, bs)
@@ -488,7 +512,7 @@ def paged_decode_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         _all_dense(q, workspace)
         ws_bytes = workspace.numel() * workspace.element_size()
     call("rllm_paged_attention_decode_mxfp4", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
-         _ptr(seq_lens), q.shape[0], hq, hkv, d, bs, block_tables.shape[1], nb, scale, dt, _ptr(workspace), ws_bytes,
+         _ptr(seq_lens), b, hq, hkv, d, bs, maxb, nb, scale, dt, _ptr(workspace), ws_bytes,
          _stream(stream))
     return out
 
@@ -498,10 +522,9 @@ def paged_prefill_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         out: Optional[torch.Tensor] = None, validate: bool = True,
                         stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Chunked-prefill attention over MXFP4 caches through rllm_paged_attention_prefill_mxfp4."""
-    hq, hkv, d, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
-    b, t = seq_lens.shape[0], q.shape[0]
+    t, hq, hkv, d, b, maxb, bs, nb, dt, out = _mxfp4_attention(q, k_cache, v_cache, block_tables, seq_lens, out)
     if query_start_loc.dtype != torch.int32 or query_start_loc.shape != (b + 1,) or \
-            query_start_loc.device != q.device or not query_start_loc.is_contiguous():
+            query_start_loc.get_device() != q.get_device() or not query_start_loc.is_contiguous():
         raise ValueError("query_start_loc must be contiguous int32 [num_seqs + 1] on the device of q")
     if validate:
         validate_tables(block_tables, seq_lens, nb, bs)
@@ -509,7 +532,7 @@ def paged_prefill_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         if int(qsl[0]) != 0 or int(qsl[-1]) != t or bool((qsl[1:] < qsl[:-1]).any()):
             raise ValueError("query_start_loc must rise from 0 to num_tokens")
     call("rllm_paged_attention_prefill_mxfp4", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
-         _ptr(seq_lens), _ptr(query_start_loc), b, t, hq, hkv, d, bs, block_tables.shape[1], nb, scale, dt,
+         _ptr(seq_lens), _ptr(query_start_loc), b, t, hq, hkv, d, bs, maxb, nb, scale, dt,
          _stream(stream))
     return out
 
