@@ -47,6 +47,7 @@ typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t mx_u32x4a __attribute__((ext_vector_type(4)));
 typedef uint32_t mx_out8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 typedef short mx_i16x4 __attribute__((ext_vector_type(4)));

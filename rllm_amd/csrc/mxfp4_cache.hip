@@ -261,8 +261,11 @@ __global__ __launch_bounds__(MXC_THREADS) void mx4_read_kernel(uint4* __restrict
         k = values8<KIND>(ck, ek);
         v = values8<KIND>(cv, ev);
     }
-    ok[i] = k;
-    ov[i] = v;
+    // The rows go past the L2: written through it they take turns with the reads (128k
+    // rows of 8 x 128, 330 MB in all: 76 -> 58.5 us; 4000 rows 6.0 -> 4.9; 777 rows of 8 x 64
+    // 2.7 -> 2.9).
+    __builtin_nontemporal_store(mx_u32x4a{k.x, k.y, k.z, k.w}, reinterpret_cast<mx_u32x4a*>(ok + i));
+    __builtin_nontemporal_store(mx_u32x4a{v.x, v.y, v.z, v.w}, reinterpret_cast<mx_u32x4a*>(ov + i));
 }
 
 // arguments the write and the read share; *grid = the workgroups

@@ -477,6 +477,71 @@ inline Result<void> rope_cache_write(void* q_out, const void* q, const void* k, 
 }
 
 // ---------------------------------------------------------------------------
+// MXFP4 KV cache (additive entry points): pages of 4-bit codes with a scale per 32
+// elements, uint8 [num_blocks, num_kv_heads, mxfp4_page_bytes(head_dim, block_size)]
+// ---------------------------------------------------------------------------
+inline Result<size_t> mxfp4_page_bytes(size_t head_dim, size_t block_size) {
+    const int64_t n = rllm_mxfp4_page_bytes(static_cast<int64_t>(head_dim), static_cast<int64_t>(block_size));
+    if (n < 0) return Result<size_t>::err(CudaKernelError{CudaKernelError::Kind::KernelError, 1});   // hipErrorInvalidValue
+    return Result<size_t>::ok(static_cast<size_t>(n));
+}
+
+inline Result<void> cache_write_mxfp4(uint8_t* key_cache, uint8_t* value_cache, const uint16_t* new_key,
+                                      const uint16_t* new_value, const int64_t* slot_mapping, int64_t num_tokens,
+                                      int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                                      DType input_dtype, uintptr_t stream) {
+    return check(rllm_cache_write_mxfp4(key_cache, value_cache, new_key, new_value, slot_mapping, num_tokens,
+                                        num_kv_heads, head_dim, block_size, num_blocks, abi_dtype(input_dtype), stream));
+}
+
+inline Result<void> cache_read_mxfp4(uint16_t* out_key, uint16_t* out_value, const uint8_t* key_cache,
+                                     const uint8_t* value_cache, const int64_t* slot_mapping, int64_t num_tokens,
+                                     int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                                     DType output_dtype, uintptr_t stream) {
+    return check(rllm_cache_read_mxfp4(out_key, out_value, key_cache, value_cache, slot_mapping, num_tokens,
+                                       num_kv_heads, head_dim, block_size, num_blocks, abi_dtype(output_dtype), stream));
+}
+
+// q_out may equal q; dtype is F16 or BF16
+inline Result<void> rope_cache_write_mxfp4(void* q_out, const void* q, const void* k, const void* v,
+                                           uint8_t* key_cache, uint8_t* value_cache, const int64_t* slot_mapping,
+                                           const int32_t* positions, const float* cos_cache, const float* sin_cache,
+                                           int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                                           int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                                           int64_t max_position, DType dtype, uintptr_t stream) {
+    return check(rllm_rope_cache_write_mxfp4(q_out, q, k, v, key_cache, value_cache, slot_mapping, positions, cos_cache,
+                                             sin_cache, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                                             num_blocks, max_position, abi_dtype(dtype), stream));
+}
+
+// workspace null: library-owned scratch
+inline Result<void> paged_attention_decode_mxfp4(void* output, const void* query, const uint8_t* key_cache,
+                                                 const uint8_t* value_cache, const int32_t* block_tables,
+                                                 const int32_t* seq_lens, int64_t num_seqs, int64_t num_q_heads,
+                                                 int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                                 int64_t max_num_blocks_per_seq, int64_t num_blocks, float scale,
+                                                 DType q_dtype, uintptr_t stream, void* workspace = nullptr,
+                                                 int64_t workspace_bytes = 0) {
+    return check(rllm_paged_attention_decode_mxfp4(output, query, key_cache, value_cache, block_tables, seq_lens,
+                                                   num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                                                   max_num_blocks_per_seq, num_blocks, scale, abi_dtype(q_dtype),
+                                                   workspace, workspace_bytes, stream));
+}
+
+inline Result<void> paged_attention_prefill_mxfp4(void* output, const void* query, const uint8_t* key_cache,
+                                                  const uint8_t* value_cache, const int32_t* block_tables,
+                                                  const int32_t* seq_lens, const int32_t* query_start_loc,
+                                                  int64_t num_seqs, int64_t num_tokens, int64_t num_q_heads,
+                                                  int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                                  int64_t max_num_blocks_per_seq, int64_t num_blocks, float scale,
+                                                  DType q_dtype, uintptr_t stream) {
+    return check(rllm_paged_attention_prefill_mxfp4(output, query, key_cache, value_cache, block_tables, seq_lens,
+                                                    query_start_loc, num_seqs, num_tokens, num_q_heads, num_kv_heads,
+                                                    head_dim, block_size, max_num_blocks_per_seq, num_blocks, scale,
+                                                    abi_dtype(q_dtype), stream));
+}
+
+// ---------------------------------------------------------------------------
 // block lists: copy-on-write copies and swap records (additive entry points)
 // ---------------------------------------------------------------------------
 inline Result<void> cache_copy_blocks(const uint64_t* key_caches, const uint64_t* value_caches, int64_t num_layers,
