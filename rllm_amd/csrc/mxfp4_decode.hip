@@ -8,8 +8,8 @@
 // context is cut into items of 32 tokens (an empty context is one, so every output
 // is written).  The rows' items form one list, of which every workgroup takes an
 // equal share; the host sees only the tables' width, so the shares come from the
-// lengths on the device.  The four waves of a workgroup take a row's items in
-// turn and join at the row's end in LDS.  A row cut between workgroups leaves
+// lengths on the device.  The waves of a workgroup take a row's items in turn and
+// join at the row's end in LDS.  A row cut between workgroups leaves
 // partials (sum of p v relative to the piece's max, max, sum of p); the workgroup
 // that completes the row's arrival counter adds the pieces in their order, so
 // repeated calls give the same bits whichever comes last.  Partials are written
@@ -32,19 +32,17 @@
 namespace rllm {
 namespace {
 
-constexpr int MXD_WAVES = 4;
-constexpr int MXD_THREADS = 64 * MXD_WAVES;
 constexpr int MXD_ITEM = 32;          // tokens
 constexpr int MXD_HEADS = 16;         // query heads a row
 constexpr int MXD_MAX_PIECES = 64;    // of a row
 // What a row's start and join cost beside its items, in items: a workgroup whose share
 // starts more rows gets fewer.  64 contexts of 128-4096 tokens (32/8 heads, head_dim
-// 128): 53.6 us without, 44 with 4, 39.5 with 8, 41 with 12.  Equal contexts do not change.
-// Where a workgroup has under MXD_VIRT_MIN items the waves of a row have little to share.
-constexpr int MXD_VIRT = 8, MXD_VIRT_MIN = 24;
+// 128): 53.6 us without, 44 with 4, 39.5 with 8, 41 with 12.
+constexpr int MXD_VIRT = 8;
 
-// workgroups a CU: two waves a SIMD, one where a wave needs more than half its registers
-__host__ __device__ constexpr int mxd_per_cu(int64_t d) { return d <= 128 ? 2 : 1; }
+// waves a SIMD: two, one where a wave needs more than half its registers; and workgroups a CU
+__host__ __device__ constexpr int mxd_per_simd(int64_t d) { return d <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int mxd_per_cu(int64_t d, int waves) { return 4 * mxd_per_simd(d) / waves; }
 
 struct MxDecodeArgs {
     uint16_t* out;
@@ -97,14 +95,15 @@ __device__ __forceinline__ void load2(const float* p, float& x, float& y) {
     y = __uint_as_float(static_cast<uint32_t>(w >> 32));
 }
 
-template <int QKIND, int NB>
-__global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_kernel(MxDecodeArgs a) {
+template <int QKIND, int NB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_kernel(MxDecodeArgs a) {
+    constexpr int THREADS = 64 * WAVES;
     constexpr int D = 32 * NB;
     constexpr int NK = MxItem<NB>::NK, NV = MxItem<NB>::NV;
     constexpr int NT = mx4_terms<QKIND>();
     constexpr int ROW = mxd_row<NB>();
-    __shared__ __align__(16) uint32_t lds[MXD_WAVES * MXD_ITEM * ROW / 2];   // a V tile a wave
-    __shared__ float ml_lds[MXD_WAVES][MXD_HEADS][2];
+    __shared__ __align__(16) uint32_t lds[WAVES * MXD_ITEM * ROW / 2];   // a V tile a wave
+    __shared__ float ml_lds[WAVES][MXD_HEADS][2];
     __shared__ float w_lds[MXD_MAX_PIECES][MXD_HEADS];
     __shared__ int last_lds[2];
 
@@ -145,44 +144,64 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
             longest = max(longest, mx4_wave_max(n));
         }
         total *= rows_seq;
-        const int all_rows = a.num_seqs * rows_seq;
-        if (total >= MXD_VIRT_MIN * static_cast<int>(gridDim.x)) {
-            virt = MXD_VIRT;
+        const uint32_t grid = gridDim.x, all_rows = a.num_seqs * rows_seq;
+        // Where each row can have `own` workgroups of its own and the longest row's part is
+        // no more than an equal share of the list, starts and joins counted, every row is cut
+        // at multiples of that part and no workgroup touches two rows.  Else the list is
+        // cut into equal shares, a row's start in it as `virt` items.
+        const int even = static_cast<int>((total + MXD_VIRT * all_rows + grid - 1) / grid);
+        const uint32_t own = grid / all_rows;
+        const int part = own ? max(static_cast<int>((longest + own - 1) / own), max(WAVES, (longest + MXD_MAX_PIECES - 1) / MXD_MAX_PIECES)) : 0;
+        if (own && part <= max(even, WAVES)) {
+            const uint32_t parts = (longest + part - 1) / part, at = blockIdx.x / parts;
+            if (at >= all_rows) return;   // whole workgroup
+            share = __builtin_amdgcn_readfirstlane(part);
+            row.s = __builtin_amdgcn_readfirstlane(static_cast<int>(at / static_cast<uint32_t>(rows_seq)));
+            row.r = __builtin_amdgcn_readfirstlane(static_cast<int>(at)) - row.s * rows_seq;
+            const int len = a.num_seqs <= 64 ? __builtin_amdgcn_readlane(len0, row.s) : a.seq_lens[row.s];
+            row.items = items_of(len);
+            row.ctx = min(max(len, 0), width);
+            virt = __builtin_amdgcn_readfirstlane(static_cast<int>(parts)) * share;   // the next row begins past this share
+            row.first = __builtin_amdgcn_readfirstlane(static_cast<int>(at)) * virt;
+            row.lo = blockIdx.x * share - row.first;
+            end = blockIdx.x * share + share;
+        } else {
+            virt = __builtin_amdgcn_readfirstlane(min(MXD_VIRT, even / 2));
             total += virt * all_rows;
-        }
-        // n items span at most ceil(n / share) + 1 pieces
-        const int least = max(MXD_WAVES, (longest + virt + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
-        share = __builtin_amdgcn_readfirstlane(max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), least));
-        const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
-        if (pos64 >= total) return;   // whole workgroup
-        const int pos = static_cast<int>(pos64);
-        end = static_cast<int>(min<int64_t>(pos64 + share, total));
-        int before = 0;   // items of one row of each earlier sequence
-        for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int raw = len_at(s0);
-            const int n = s0 + lane < a.num_seqs ? items_of(raw) + virt : 0;
-            const int incl = mx4_scan(n);
-            const int first = (before + incl - n) * rows_seq;
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos - first < n * rows_seq);
-            if (hit) {
-                const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-                row.s = s0 + j;
-                const int len = __builtin_amdgcn_readlane(n, j);
-                row.items = len - virt;
-                row.ctx = min(max(__builtin_amdgcn_readlane(raw, j), 0), width);
-                const int f = __builtin_amdgcn_readlane(first, j);
-                row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(len));
-                row.first = f + row.r * len + virt;
-                break;
+            // n items span at most ceil(n / share) + 1 pieces
+            const int least = max(WAVES, (longest + virt + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
+            share = __builtin_amdgcn_readfirstlane(max(static_cast<int>((total + grid - 1) / grid), least));
+            const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
+            if (pos64 >= total) return;   // whole workgroup
+            const int pos = static_cast<int>(pos64);
+            end = static_cast<int>(min<int64_t>(pos64 + share, total));
+            int before = 0;   // items of one row of each earlier sequence
+            for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+                const int raw = len_at(s0);
+                const int n = s0 + lane < a.num_seqs ? items_of(raw) + virt : 0;
+                const int incl = mx4_scan(n);
+                const int first = (before + incl - n) * rows_seq;
+                const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos - first < n * rows_seq);
+                if (hit) {
+                    const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+                    row.s = s0 + j;
+                    const int len = __builtin_amdgcn_readlane(n, j);
+                    row.items = len - virt;
+                    row.ctx = min(max(__builtin_amdgcn_readlane(raw, j), 0), width);
+                    const int f = __builtin_amdgcn_readlane(first, j);
+                    row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(len));
+                    row.first = f + row.r * len + virt;
+                    break;
+                }
+                before += __builtin_amdgcn_readlane(incl, 63);
             }
-            before += __builtin_amdgcn_readlane(incl, 63);
+            row.s = __builtin_amdgcn_readfirstlane(row.s);
+            row.r = __builtin_amdgcn_readfirstlane(row.r);
+            row.first = __builtin_amdgcn_readfirstlane(row.first);
+            row.items = __builtin_amdgcn_readfirstlane(row.items);
+            row.ctx = __builtin_amdgcn_readfirstlane(row.ctx);
+            row.lo = max(pos - row.first, 0);
         }
-        row.s = __builtin_amdgcn_readfirstlane(row.s);
-        row.r = __builtin_amdgcn_readfirstlane(row.r);
-        row.first = __builtin_amdgcn_readfirstlane(row.first);
-        row.items = __builtin_amdgcn_readfirstlane(row.items);
-        row.ctx = __builtin_amdgcn_readfirstlane(row.ctx);
-        row.lo = max(pos - row.first, 0);
     }
     row.hi = min(end - row.first, row.items);
 
@@ -204,13 +223,13 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         return y;
     };
 
-    // ---- this wave's items of a row are lo + wave + 4 k.  Lane j holds the table entry
+    // ---- this wave's items of a row are lo + wave + WAVES k.  Lane j holds the table entry
     // of 16-token part j % 2 of item k0 + j / 2, and the part's row in the page (-1: past
     // the context).  Nothing looks at the entry here: its load, a row ahead, would have
     // to be waited for ----
     struct Ids { int id, row; };
     auto load_ids = [&](const MxRow& x, int k0) __attribute__((always_inline)) -> Ids {
-        const int i = x.lo + wave + MXD_WAVES * (k0 + (lane >> 1));
+        const int i = x.lo + wave + WAVES * (k0 + (lane >> 1));
         const int u = 2 * i + (lane & 1);
         const int blk = static_cast<int>((static_cast<uint32_t>(u) * a.subs_mul) >> 32);
         Ids y{-1, i < x.hi && u * MX4_TOKENS < x.ctx ? (u - blk * a.subs) * MX4_TOKENS : -1};
@@ -328,7 +347,7 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
     auto start = [&](const MxRow& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            if (x.lo + wave + MXD_WAVES * b < x.hi) {
+            if (x.lo + wave + WAVES * b < x.hi) {
                 const Part p0 = part_of(parts, 2 * b), p1 = part_of(parts, 2 * b + 1);
                 load_k(p0, p1, set[b]);
                 load_v(p0, p1, set[b]);
@@ -379,11 +398,11 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
 #pragma unroll
         for (int j = 0; j < 2 * NB; ++j) o[j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;   // l: this lane's tokens only
-        const int count = (row.hi - row.lo - wave + MXD_WAVES - 1) / MXD_WAVES;   // this wave's items
+        const int count = (row.hi - row.lo - wave + WAVES - 1) / WAVES;   // this wave's items
 
         // item k from set x.  As the set's registers come free, the loads of item k + 2
         // go out, or, at a row's end, of the next row's first two items
-        const int nxt_count = count < 2 ? 0 : (nxt.hi - nxt.lo - wave + MXD_WAVES - 1) / MXD_WAVES;
+        const int nxt_count = count < 2 ? 0 : (nxt.hi - nxt.lo - wave + WAVES - 1) / WAVES;
         auto item = [&](int k, MxItem<NB>& x, uint32_t& here) __attribute__((always_inline)) {
             const bool last2 = k + 2 >= count;
             const int ahead = last2 ? k + 2 - count : k + 2;
@@ -410,7 +429,7 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
                 p1 = part_of(parts, at + 1);
                 load_k(p0, p1, x);
             }
-            const int t0 = (row.lo + wave + MXD_WAVES * k) * MXD_ITEM;
+            const int t0 = (row.lo + wave + WAVES * k) * MXD_ITEM;
             const bool full = here == 3u && t0 + MXD_ITEM <= row.ctx;
             if (!full) {
 #pragma unroll
@@ -511,17 +530,17 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         __syncthreads();
         const Piece piece = piece_of(row);
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (row.lo == 0 ? 1 : 0);
-        for (int e = 2 * tid; e < heads * D; e += 2 * MXD_THREADS) {
+        for (int e = 2 * tid; e < heads * D; e += 2 * THREADS) {
             const int hd = e / D;
-            float mw[MXD_WAVES], lw[MXD_WAVES], mm = -INFINITY, ll = 0.f, y0 = 0.f, y1 = 0.f;
+            float mw[WAVES], lw[WAVES], mm = -INFINITY, ll = 0.f, y0 = 0.f, y1 = 0.f;
 #pragma unroll
-            for (int w = 0; w < MXD_WAVES; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 mw[w] = ml_lds[w][hd][0];
                 lw[w] = ml_lds[w][hd][1];
                 mm = fmaxf(mm, mw[w]);
             }
 #pragma unroll
-            for (int w = 0; w < MXD_WAVES; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const mx_f32x2 y = *reinterpret_cast<const mx_f32x2*>(lds + w * MXD_ITEM * ROW / 2 + e);
                 if (lw[w] != 0.f) {   // a wave that saw nothing adds nothing, NaN goes on
                     const float f = __builtin_amdgcn_exp2f(mw[w] - mm);
@@ -578,7 +597,7 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
         };
         if (e0 < heads * D) load8(0, e0);
         // a wave a head, a lane a piece: the pieces' factors and the row's sum
-        for (int hd = wave; hd < heads; hd += MXD_WAVES) {
+        for (int hd = wave; hd < heads; hd += WAVES) {
             float mp = -INFINITY, lp = 0.f;
             if (lane < x.count) load2(a.part_ml + slot_of(lane) * (2 * MXD_HEADS) + 2 * hd, mp, lp);
             const float top = wave_max(mp);
@@ -588,7 +607,7 @@ __global__ __launch_bounds__(MXD_THREADS, mxd_per_cu(32 * NB)) void mx4_decode_k
             if (lane == 0) ml_lds[0][hd][0] = L == 0.f ? 0.f : 1.f / L;
         }
         __syncthreads();
-        for (int e = e0; e < heads * D; e += 2 * MXD_THREADS) {
+        for (int e = e0; e < heads * D; e += 2 * THREADS) {
             const int hd = e / D;
             float y0 = 0.f, y1 = 0.f;
             for (int p0 = 0; p0 < x.count; p0 += 8) {
@@ -618,15 +637,25 @@ int64_t mxd_scratch_bytes(int64_t wgs, int64_t d) {
     return MXD_COUNTER_BYTES + 2 * wgs * MXD_HEADS * (d + 2) * 4;
 }
 
+// Waves a workgroup: four share a row's items, two where rows are many and short, so
+// that a workgroup joins less often for the same waves on the chip.  With a
+// row or more for every pair of waves, us of four / two: 256 contexts (32/8 heads,
+// head_dim 128) of 64 tokens 20.0 / 13.8, 256 28.0 / 23.1, 512 39.3 / 34.2, 2048 132 / 133, of
+// 32-512 38 / 35; 128 of 4096 126 / 130.  With fewer rows two cut them more often: 64 of
+// 512 12.5 / 17.0.
+constexpr int64_t MXD_SHORT = 2048;   // tokens
+
 // Workgroups: what the device holds, fewer where the tables hold less than one item a wave.
-int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t* wgs) {
+int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t* wgs,
+                       int* waves) {
     int dev = 0, cus = 0;
     RLLM_TRY(hipGetDevice(&dev));
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t groups = (hq / hkv + MXD_HEADS - 1) / MXD_HEADS, rows = num_seqs * hkv * groups;
+    *waves = rows >= static_cast<int64_t>(cus) * mxd_per_cu(d, 2) && maxb * bs <= MXD_SHORT ? 2 : 4;
     const int64_t items = (maxb * bs + MXD_ITEM - 1) / MXD_ITEM;
-    const int64_t most = rows * ((items + MXD_WAVES - 1) / MXD_WAVES > 0 ? (items + MXD_WAVES - 1) / MXD_WAVES : 1);
-    int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d);
+    const int64_t most = rows * (items > *waves ? (items + *waves - 1) / *waves : 1);
+    int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d, *waves);
     if (held > MXD_MAX_WGS) held = MXD_MAX_WGS;
     *wgs = most < held ? most : held;
     return 0;
@@ -641,11 +670,11 @@ int32_t mxd_check(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t 
     return 0;
 }
 
-template <int QKIND>
+template <int QKIND, int WAVES>
 int32_t mxd_launch(const MxDecodeArgs& a, int64_t d, int64_t wgs, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(wgs)), block(MXD_THREADS);
+    const dim3 grid(static_cast<unsigned>(wgs)), block(64 * WAVES);
     switch (d / 32) {
-#define MXD_CASE(NB) case NB: hipLaunchKernelGGL((mx4_decode_kernel<QKIND, NB>), grid, block, 0, st, a); break;
+#define MXD_CASE(NB) case NB: hipLaunchKernelGGL((mx4_decode_kernel<QKIND, NB, WAVES>), grid, block, 0, st, a); break;
         MXD_CASE(1) MXD_CASE(2) MXD_CASE(3) MXD_CASE(4) MXD_CASE(5) MXD_CASE(6) MXD_CASE(7) MXD_CASE(8)
 #undef MXD_CASE
         default: return static_cast<int32_t>(hipErrorInvalidValue);
@@ -666,7 +695,8 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
     if (num_seqs <= 0) return 0;
     if (mxd_check(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, 0)) return -1;
     int64_t wgs = 0;
-    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs)) return -1;
+    int waves = 0;
+    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves)) return -1;
     return mxd_scratch_bytes(wgs, head_dim);
 }
 
@@ -687,7 +717,8 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
     RLLM_CHECK_ARG(mx4_aligned16(key_cache) && mx4_aligned16(value_cache));
     RLLM_CHECK_ARG(((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(output)) & 3) == 0);
     int64_t wgs = 0;
-    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs);
+    int waves = 0;
+    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves);
     if (rc) return rc;
     const int64_t need = mxd_scratch_bytes(wgs, head_dim);
     void* ws = workspace;
@@ -722,8 +753,12 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
         a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + MXD_COUNTER_BYTES);
         a.part_ml = a.part_o + 2 * wgs * MXD_HEADS * head_dim;
     }
-    return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16>(a, head_dim, wgs, as_stream(stream))
-                                      : mxd_launch<KIND_F16>(a, head_dim, wgs, as_stream(stream));
+    hipStream_t st = as_stream(stream);
+    if (waves == 2)
+        return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 2>(a, head_dim, wgs, st)
+                                          : mxd_launch<KIND_F16, 2>(a, head_dim, wgs, st);
+    return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 4>(a, head_dim, wgs, st)
+                                      : mxd_launch<KIND_F16, 4>(a, head_dim, wgs, st);
 }
 
 }  // extern "C"

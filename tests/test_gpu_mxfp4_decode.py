@@ -80,6 +80,22 @@ def test_many_sequences(dev):
     run_and_check(rng, lens, 4, 2, 64, 16, "bf16", dev)
 
 
+@pytest.mark.parametrize("lo", [1, 150])
+def test_many_short_rows(dev, lo):
+    # a row or more for every two waves of the chip: workgroups of two waves, several rows each
+    rng = np.random.default_rng(22)
+    lens = rng.integers(lo, 150, 150, endpoint=True).tolist()
+    run_and_check(rng, lens, 16, 8, 64, 16, "bf16", dev)
+    run_and_check(rng, lens[:140], 16, 8, 160, 32, "f16", dev)
+
+
+@pytest.mark.parametrize("lens", [[64] * 9, [1, 700, 33, 64, 2], [3000] + [40] * 20, [0, 0, 5000]])
+def test_equal_and_unequal_parts(dev, lens):
+    # rows cut at multiples of one part, and a list cut into equal shares
+    rng = np.random.default_rng(23)
+    run_and_check(rng, lens, 8, 2, 128, 16, "bf16", dev)
+
+
 def test_long_row_cut_between_workgroups(dev):
     rng = np.random.default_rng(10)
     run_and_check(rng, [9001, 40], 4, 1, 128, 16, "bf16", dev)
