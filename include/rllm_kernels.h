@@ -620,8 +620,12 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
  * rllm_paged_attention_prefill_ex (causal at absolute positions; the new tokens'
  * rows must be in the cache already), with the cache's num_blocks.  query 16-byte,
  * output 8-byte aligned.  bf16 queries: the weights are rounded to bf16 before they
- * meet the values, as for 16-bit caches; f16: to 16 bits.  Rows of output that
- * query_start_loc leaves out stay as they are. */
+ * meet the values, as for 16-bit caches (to 16 bits where a sequence has few new
+ * tokens); f16: to 16 bits.  Rows of output that query_start_loc leaves out stay as
+ * they are; its entries must not fall or pass num_tokens (sequences of one that does
+ * may be left unwritten).  Calls of few new tokens use library-owned buffers per
+ * (device, stream), the decode call's among them, on its terms for captured graphs; a
+ * capture on a stream that has none of the size yet runs without. */
 int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,
                                            const uint8_t *key_cache, const uint8_t *value_cache,
                                            const int32_t *block_tables, const int32_t *seq_lens,

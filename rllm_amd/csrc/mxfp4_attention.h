@@ -39,6 +39,9 @@ __device__ __forceinline__ void mx4_sub_e4m3(float (&x)[4], uint32_t w, float fa
     x[3] -= b[1];
 }
 
+// the least factor of a part of a row that saw a key (f32's smallest normal)
+constexpr float MX4_LEAST = 1.17549435e-38f;
+
 // terms of a query element
 template <int QKIND> constexpr int mx4_terms() { return QKIND == KIND_BF16 ? 2 : 3; }
 
@@ -186,5 +189,18 @@ __device__ __forceinline__ float mx4_query_factor(int byte0) {
 // the block scales of a term: 255 stays NaN
 __device__ __forceinline__ int mx4_term_byte(int byte0, int term) { return byte0 == 255 ? 255 : byte0 - 4 * term; }
 
+// waves a SIMD of the decode kernel: two, one where a wave needs more than half its registers
+__host__ __device__ constexpr int mxd_per_simd(int64_t d) { return d <= 128 ? 2 : 1; }
 }  // namespace
+
+// Chunks of few new tokens on the decode kernel, a (token, query head) pair a column: sequences of
+// at most most_cols columns a kv head; the others' outputs stay.  Its rows, at most (a workgroup's
+// least work), or -1 where the batch passes its counters, which the launch refuses.
+int64_t mx4_short_rows(int64_t num_seqs, int64_t num_tokens, int64_t hq, int64_t hkv, int64_t bs, int64_t maxb,
+                       int64_t most_cols);
+int32_t mx4_short_chunks(void* out, const void* q, const uint8_t* kc, const uint8_t* vc, const int32_t* bt,
+                         const int32_t* seq_lens, const int32_t* qsl, int64_t num_seqs, int64_t num_tokens, int64_t hq,
+                         int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t nb, float scale, int32_t q_dtype,
+                         int64_t most_cols, uintptr_t stream);
+
 }  // namespace rllm

@@ -1,18 +1,21 @@
-// Decode attention (one query token a sequence) over the MXFP4 KV cache, for
-// gfx950: o = softmax(scale q K^T) V per (sequence, query head).
+// Decode attention over the MXFP4 KV cache, for gfx950: o = softmax(scale q K^T) V per
+// (sequence, query head), for one query token a sequence, and for chunks of few (see
+// mxfp4_prefill.hip, which sends them here): a sequence's query token i of n attends keys
+// 0 .. seq_len - n + i.
 //
 // Bound by HBM: a context token of one kv head is 2 * D * 17 / 32 bytes (136 at D
-// 128) against 4 D G operations for its G query heads.
+// 128) against 4 D operations for each of its columns, a column being a (query token,
+// query head of the group) pair.
 //
-// Work.  A row is a (sequence, kv head, group of up to 16 of its query heads); its
-// context is cut into items of 32 tokens (an empty context is one, so every output
-// is written).  The rows' items form one list, of which every workgroup takes an
-// equal share; the host sees only the tables' width, so the shares come from the
-// lengths on the device.  The waves of a workgroup take a row's items in turn and
-// join at the row's end in LDS.  A row cut between workgroups leaves
-// partials (sum of p v relative to the piece's max, max, sum of p); the workgroup
-// that completes the row's arrival counter adds the pieces in their order, so
-// repeated calls give the same bits whichever comes last.  Partials are written
+// Work.  A row is up to 16 columns of a (sequence, kv head), the width of the product;
+// its context is cut into items of 32 tokens (an empty context is one, so every output
+// is written).  The host sees only the tables' width, so how rows go to workgroups
+// comes from the lengths on the device: where the rows are alike each gets workgroups
+// of its own; else the rows' items form one list, cut into equal shares.  The waves
+// of a workgroup take a row's items in turn and join at the row's end in LDS.  A row cut
+// between workgroups leaves partials (sum of p v relative to the piece's max, max, sum of
+// p); the workgroup that completes the row's arrival counter adds the pieces in their
+// order, so repeated calls give the same bits whichever comes last.  Partials are written
 // and read as relaxed agent-scope atomics, which pass by the XCDs' own L2, and each
 // wave waits for its stores before the count (the order of the stream decode
 // kernel's merge).
@@ -24,7 +27,12 @@
 // and turned through LDS, [32 tokens][D] private to the wave, read back
 // transposed.  Weights enter as two bf16 terms, p = hi + lo (16 bits against the
 // output's 8 or 11), whatever the query's type: the matrix cores have the time.
-// Items are loaded one ahead of use.
+// Items are loaded one ahead of use, over a row's end too.
+//
+// Measured (32/8 heads, head_dim 128, bf16): 64 contexts of 128-4096 tokens, 146 MB,
+// 39.1 us (3.7 TB/s); 24 of 4000-32000 (24/8 heads, f16), 506 MB, 102 us (4.95 TB/s,
+// a large copy's rate); one of 700 tokens 8 us, nearly all latency: a launch, lengths, table
+// entries, a part's loads, the join.
 #include "mxfp4_attention.h"
 #include "workspace.h"
 #include "../../include/rllm_kernels.h"
@@ -39,9 +47,14 @@ constexpr int MXD_MAX_PIECES = 64;    // of a row
 // starts more rows gets fewer.  64 contexts of 128-4096 tokens (32/8 heads, head_dim
 // 128): 53.6 us without, 44 with 4, 39.5 with 8, 41 with 12.
 constexpr int MXD_VIRT = 8;
+// A row's pieces are joined by one workgroup, so pieces that its joining would outlast
+// are not cut: a piece holds at least sqrt(items * elements / threads * this) items.
+// One sequence's 4 new tokens on 8000 (32/8 heads, head_dim 128), whose 16 columns make a
+// join four times a token's: 31.8 us without, 21.9 with half of this, 20.3, 21.6 with twice.
+constexpr float MXD_JOIN = 0.1875f;
+constexpr int MXD_JOIN_LOADS = 8;   // pieces of a join in flight: 8.6 us against 9.1 of 16, 1 context of 1024
 
-// waves a SIMD: two, one where a wave needs more than half its registers; and workgroups a CU
-__host__ __device__ constexpr int mxd_per_simd(int64_t d) { return d <= 128 ? 2 : 1; }
+// workgroups a CU
 __host__ __device__ constexpr int mxd_per_cu(int64_t d, int waves) { return 4 * mxd_per_simd(d) / waves; }
 
 struct MxDecodeArgs {
@@ -49,7 +62,9 @@ struct MxDecodeArgs {
     const uint16_t* q;
     const uint8_t *kc, *vc;
     const int32_t *bt, *seq_lens;
-    int32_t num_seqs, hq, hkv, groups;   // groups of query heads a kv head
+    const int32_t* qsl;                  // chunks: their query tokens; else null
+    int32_t num_seqs, num_tokens, hq, hkv;
+    int32_t most_cols;                   // chunks: sequences of more columns are not for this kernel
     int32_t bs, subs;                    // tokens, 16-token parts of a block
     uint64_t subs_mul;                   // ceil(2^32 / subs)
     int32_t maxb;
@@ -74,14 +89,22 @@ struct MxItem {
 };
 
 // A row at hand: row r of sequence s, its first item in the list of all, its items
-// (all of them, and lo .. hi - 1 of this workgroup) and keys.
+// (all of them, and lo .. hi - 1 of this workgroup) and keys; the sequence's n query
+// tokens from q0 on, the first of them at position cached.
 struct MxRow {
-    int s, r, first, items, lo, hi, ctx;
+    int s, r, first, items, lo, hi, ctx, n, q0, cached;
 };
 
-// A piece of a row cut between workgroups: the row, its first workgroup and its pieces.
+// The columns of a row: up to 16 (query token, query head) pairs of a kv head, token
+// by token, from column `col` of the sequence's.
+struct MxCols {
+    int h, col, count, q0;
+};
+
+// A piece of a row cut between workgroups: the row's columns, its first workgroup and its pieces.
 struct Piece {
-    int s, r, first_wg, count;
+    MxCols cols;
+    int first_wg, count;
 };
 
 // two floats past the XCD's own L2, as one access
@@ -95,7 +118,7 @@ __device__ __forceinline__ void load2(const float* p, float& x, float& y) {
     y = __uint_as_float(static_cast<uint32_t>(w >> 32));
 }
 
-template <int QKIND, int NB, int WAVES>
+template <int QKIND, int NB, int WAVES, bool CHUNK>
 __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_kernel(MxDecodeArgs a) {
     constexpr int THREADS = 64 * WAVES;
     constexpr int D = 32 * NB;
@@ -106,12 +129,13 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
     __shared__ float ml_lds[WAVES][MXD_HEADS][2];
     __shared__ float w_lds[MXD_MAX_PIECES][MXD_HEADS];
     __shared__ int last_lds[2];
+    __shared__ uint32_t nan_lds[WAVES][MXD_HEADS];   // chunks: value blocks that are NaN in a column
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int l16 = lane & 15, grp = lane >> 4;
     uint16_t* const v_lds = reinterpret_cast<uint16_t*>(lds) + wave * MXD_ITEM * ROW;
-    const int rows_seq = a.hkv * a.groups;      // rows of a sequence
+    const int G = a.hq / a.hkv;
     const int page_bytes = static_cast<int>(mx4_page_bytes(D, a.bs));
     const int code_bytes = a.bs * (D / 2);      // of a page
     const int width = a.maxb * a.bs;            // tokens a table can hold
@@ -120,88 +144,110 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
         return max((min(len, width) + MXD_ITEM - 1) / MXD_ITEM, 1);
     };
 
+    // groups of 16 columns a kv head of a sequence of n query tokens has
+    auto groups_of = [&](int n) __attribute__((always_inline)) { return (n * G + MXD_HEADS - 1) / MXD_HEADS; };
+    // a sequence's query tokens, and the first of them
+    auto tokens_of = [&](int s, int& q0) __attribute__((always_inline)) {
+        if constexpr (!CHUNK) {
+            q0 = s;
+            return 1;
+        } else {
+            q0 = a.qsl[s];
+            const int n = a.qsl[s + 1] - q0;
+            return n * G <= a.most_cols ? n : 0;
+        }
+    };
+    auto open_row = [&](MxRow& x, int len) __attribute__((always_inline)) {
+        x.items = items_of(len);
+        x.ctx = min(max(len, 0), width);
+        x.cached = max(len, 0) - x.n;
+    };
+
     MxRow row{};
     int virt = 0;     // items a row's start counts for in the list
     int end, share;   // the end of this workgroup's items in the list, and the items of a workgroup
-    if (!a.counters) {
-        // no scratch: a workgroup a row
-        row.s = blockIdx.x / rows_seq;
-        row.r = blockIdx.x % rows_seq;
-        row.items = items_of(a.seq_lens[row.s]);
-        row.ctx = min(max(a.seq_lens[row.s], 0), width);
-        end = share = row.items;
-    } else {
-        // ---- the share: every wave works it out from the lengths.  The lengths of
-        // up to 64 sequences are read once ----
+    {
+        // ---- the share: every wave works it out from the lengths.  Those of up to 64
+        // sequences are read once ----
         const int len0 = a.seq_lens[min(lane, a.num_seqs - 1)];
         auto len_at = [&](int s0) __attribute__((always_inline)) {
             return s0 == 0 ? len0 : a.seq_lens[min(s0 + lane, a.num_seqs - 1)];
         };
-        int total = 0, longest = 1;
+        auto rows_at = [&](int s0) __attribute__((always_inline)) {   // of sequence s0 + lane
+            int q0;
+            return s0 + lane < a.num_seqs ? a.hkv * groups_of(tokens_of(min(s0 + lane, a.num_seqs - 1), q0)) : 0;
+        };
+        int total = 0, longest = 1, all_rows = 0;
         for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-            const int n = s0 + lane < a.num_seqs ? items_of(len_at(s0)) : 0;
-            total += __builtin_amdgcn_readlane(mx4_scan(n), 63);
+            if constexpr (CHUNK) {   // starts that fall or leave the batch: nothing below would hold
+                const int s = min(s0 + lane, a.num_seqs - 1), q0 = a.qsl[s], q1 = a.qsl[s + 1];
+                if (__builtin_amdgcn_ballot_w64(q0 < 0 || q1 < q0 || q1 > a.num_tokens)) return;   // whole workgroup
+            }
+            const int rows = rows_at(s0), n = rows ? items_of(len_at(s0)) : 0;
+            total += __builtin_amdgcn_readlane(mx4_scan(rows * n), 63);
+            all_rows += CHUNK ? __builtin_amdgcn_readlane(mx4_scan(rows), 63) : 0;
             longest = max(longest, mx4_wave_max(n));
         }
-        total *= rows_seq;
-        const uint32_t grid = gridDim.x, all_rows = a.num_seqs * rows_seq;
+        if constexpr (!CHUNK) all_rows = a.num_seqs * a.hkv * groups_of(1);
+        if (all_rows == 0) return;   // no query tokens for this kernel
         // Where each row can have `own` workgroups of its own and the longest row's part is
         // no more than an equal share of the list, starts and joins counted, every row is cut
-        // at multiples of that part and no workgroup touches two rows.  Else the list is
+        // at multiples of that part (or larger ones, see MXD_JOIN) and no workgroup touches two
+        // rows.  Else the list is
         // cut into equal shares, a row's start in it as `virt` items.
-        const int even = static_cast<int>((total + MXD_VIRT * all_rows + grid - 1) / grid);
-        const uint32_t own = grid / all_rows;
-        const int part = own ? max(static_cast<int>((longest + own - 1) / own), max(WAVES, (longest + MXD_MAX_PIECES - 1) / MXD_MAX_PIECES)) : 0;
-        if (own && part <= max(even, WAVES)) {
-            const uint32_t parts = (longest + part - 1) / part, at = blockIdx.x / parts;
-            if (at >= all_rows) return;   // whole workgroup
+        const int grid = gridDim.x;
+        const int even = (total + MXD_VIRT * all_rows + grid - 1) / grid;
+        const int own = static_cast<int>(static_cast<uint32_t>(grid) / static_cast<uint32_t>(all_rows));
+        int part = own ? max((longest + own - 1) / own, max(WAVES, (longest + MXD_MAX_PIECES - 1) / MXD_MAX_PIECES)) : 0;
+        const bool apart = !a.counters || (own && part <= max(even, WAVES));
+        const int joins = min(CHUNK ? MXD_HEADS : G, MXD_HEADS) * D;   // elements of a row
+        const int worth = static_cast<int>(__builtin_sqrtf(static_cast<float>(longest) * joins * (MXD_JOIN / THREADS)));
+        part = max(part, worth);
+        if (!a.counters) part = longest;   // no scratch: a workgroup a row
+        int stride = 0;   // of rows cut apart
+        if (apart) {
             share = __builtin_amdgcn_readfirstlane(part);
-            row.s = __builtin_amdgcn_readfirstlane(static_cast<int>(at / static_cast<uint32_t>(rows_seq)));
-            row.r = __builtin_amdgcn_readfirstlane(static_cast<int>(at)) - row.s * rows_seq;
-            const int len = a.num_seqs <= 64 ? __builtin_amdgcn_readlane(len0, row.s) : a.seq_lens[row.s];
-            row.items = items_of(len);
-            row.ctx = min(max(len, 0), width);
-            virt = __builtin_amdgcn_readfirstlane(static_cast<int>(parts)) * share;   // the next row begins past this share
-            row.first = __builtin_amdgcn_readfirstlane(static_cast<int>(at)) * virt;
-            row.lo = blockIdx.x * share - row.first;
-            end = blockIdx.x * share + share;
+            stride = __builtin_amdgcn_readfirstlane((longest + part - 1) / part) * share;
+            total = all_rows * stride;
         } else {
             virt = __builtin_amdgcn_readfirstlane(min(MXD_VIRT, even / 2));
             total += virt * all_rows;
             // n items span at most ceil(n / share) + 1 pieces
-            const int least = max(WAVES, (longest + virt + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
-            share = __builtin_amdgcn_readfirstlane(max(static_cast<int>((total + grid - 1) / grid), least));
-            const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
-            if (pos64 >= total) return;   // whole workgroup
-            const int pos = static_cast<int>(pos64);
-            end = static_cast<int>(min<int64_t>(pos64 + share, total));
-            int before = 0;   // items of one row of each earlier sequence
-            for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-                const int raw = len_at(s0);
-                const int n = s0 + lane < a.num_seqs ? items_of(raw) + virt : 0;
-                const int incl = mx4_scan(n);
-                const int first = (before + incl - n) * rows_seq;
-                const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && first <= pos && pos - first < n * rows_seq);
-                if (hit) {
-                    const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-                    row.s = s0 + j;
-                    const int len = __builtin_amdgcn_readlane(n, j);
-                    row.items = len - virt;
-                    row.ctx = min(max(__builtin_amdgcn_readlane(raw, j), 0), width);
-                    const int f = __builtin_amdgcn_readlane(first, j);
-                    row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(len));
-                    row.first = f + row.r * len + virt;
-                    break;
-                }
-                before += __builtin_amdgcn_readlane(incl, 63);
-            }
-            row.s = __builtin_amdgcn_readfirstlane(row.s);
-            row.r = __builtin_amdgcn_readfirstlane(row.r);
-            row.first = __builtin_amdgcn_readfirstlane(row.first);
-            row.items = __builtin_amdgcn_readfirstlane(row.items);
-            row.ctx = __builtin_amdgcn_readfirstlane(row.ctx);
-            row.lo = max(pos - row.first, 0);
+            const int least = max(max(WAVES, worth), (longest + virt + MXD_MAX_PIECES - 3) / (MXD_MAX_PIECES - 2));
+            share = __builtin_amdgcn_readfirstlane(max((total + grid - 1) / grid, least));
         }
+        const int64_t pos64 = static_cast<int64_t>(share) * blockIdx.x;
+        if (pos64 >= total) return;   // whole workgroup
+        const int pos = static_cast<int>(pos64);
+        end = static_cast<int>(min<int64_t>(pos64 + share, total));
+        int before = 0;   // of the list in earlier sequences
+        for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+            const int raw = len_at(s0), rows = rows_at(s0);
+            const int len = apart ? stride : items_of(raw) + virt;   // of a row in the list
+            const int incl = mx4_scan(rows * len), first = before + incl - rows * len;
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(first <= pos && pos - first < rows * len);
+            if (hit) {
+                const int j = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+                row.s = s0 + j;
+                const int f = __builtin_amdgcn_readlane(first, j), row_len = __builtin_amdgcn_readlane(len, j);
+                row.r = static_cast<int>(static_cast<uint32_t>(pos - f) / static_cast<uint32_t>(row_len));
+                row.first = f + row.r * row_len + virt;
+                row.n = tokens_of(row.s, row.q0);
+                open_row(row, __builtin_amdgcn_readlane(raw, j));
+                break;
+            }
+            before += __builtin_amdgcn_readlane(incl, 63);
+        }
+        row.s = __builtin_amdgcn_readfirstlane(row.s);
+        row.r = __builtin_amdgcn_readfirstlane(row.r);
+        row.first = __builtin_amdgcn_readfirstlane(row.first);
+        row.items = __builtin_amdgcn_readfirstlane(row.items);
+        row.ctx = __builtin_amdgcn_readfirstlane(row.ctx);
+        row.n = __builtin_amdgcn_readfirstlane(row.n);
+        row.q0 = __builtin_amdgcn_readfirstlane(row.q0);
+        row.cached = __builtin_amdgcn_readfirstlane(row.cached);
+        row.lo = max(pos - row.first, 0);
+        if (apart) virt = stride;   // the next row begins past this share
     }
     row.hi = min(end - row.first, row.items);
 
@@ -212,15 +258,24 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
         y.lo = 0;
         y.hi = 0;
         if (y.first >= end) return y;
-        if (++y.r == rows_seq) {
+        if (++y.r == a.hkv * groups_of(x.n)) {
             y.r = 0;
-            ++y.s;   // within the batch: the list goes on
-            const int len = a.seq_lens[y.s];
-            y.items = items_of(len);
-            y.ctx = min(max(len, 0), width);
+            do ++y.s;   // within the batch: the list goes on
+            while ((y.n = tokens_of(y.s, y.q0)) == 0);
+            open_row(y, a.seq_lens[y.s]);
         }
         y.hi = min(end - y.first, y.items);
         return y;
+    };
+    auto cols_of = [&](const MxRow& x) __attribute__((always_inline)) -> MxCols {
+        const int groups = groups_of(x.n), g = x.r % groups;
+        return MxCols{x.r / groups, g * MXD_HEADS, min(x.n * G - g * MXD_HEADS, MXD_HEADS), x.q0};
+    };
+    // a column's query row
+    auto q_row_of = [&](const MxCols& x, int c) __attribute__((always_inline)) -> int64_t {
+        if constexpr (!CHUNK) return static_cast<int64_t>(x.q0) * a.hq + x.h * G + x.col + c;
+        const int at = x.col + c, tok = static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(G));
+        return (static_cast<int64_t>(x.q0) + tok) * a.hq + x.h * G + (at - tok * G);
     };
 
     // ---- this wave's items of a row are lo + wave + WAVES k.  Lane j holds the table entry
@@ -306,7 +361,7 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
 
     // a row's first workgroup and pieces: one that lies in this share needs no division
     auto piece_of = [&](const MxRow& x) __attribute__((always_inline)) -> Piece {
-        Piece y{x.s, x.r, static_cast<int>(blockIdx.x), 1};
+        Piece y{cols_of(x), static_cast<int>(blockIdx.x), 1};
         if (x.lo > 0) y.first_wg = static_cast<int>(static_cast<uint32_t>(x.first) / static_cast<uint32_t>(share));
         if (x.lo > 0 || x.hi < x.items)
             y.count = static_cast<int>(static_cast<uint32_t>(x.first + x.items - 1) / static_cast<uint32_t>(share)) - y.first_wg + 1;
@@ -314,19 +369,12 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
     };
     Piece head{}, tail{};   // pieces of rows cut at the share's start and end
 
-    // a row's first query row and its number of query heads
-    auto q_row_of = [&](int s, int r, int& heads) __attribute__((always_inline)) -> int64_t {
-        const int g_all = a.hq / a.hkv, hg = r % a.groups;
-        heads = min(g_all - hg * MXD_HEADS, MXD_HEADS);
-        return static_cast<int64_t>(s) * a.hq + r / a.groups * g_all + hg * MXD_HEADS;
-    };
     // the query rows, 4-byte aligned: lane group g holds elements 16 g.. and 64 + 16 g..
     // of each 128-wide step (the order of the 8-bit operand)
     uint4 q_raw[NK][4];
     auto load_q = [&](const MxRow& x) __attribute__((always_inline)) {
-        int heads;
-        const int64_t q_row = q_row_of(x.s, x.r, heads);
-        const uint16_t* src = a.q + (q_row + min(l16, heads - 1)) * D;
+        const MxCols cols = cols_of(x);
+        const uint16_t* src = a.q + q_row_of(cols, min(l16, cols.count - 1)) * D;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
@@ -354,16 +402,24 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                 present[b] = static_cast<uint32_t>(parts.ok >> (2 * b)) & 3u;
             }
     };
-    parts = resolve(load_ids(row, 0), row.r / a.groups);
+    parts = resolve(load_ids(row, 0), cols_of(row).h);
     load_q(row);
     start(row);
 
     while (row.lo < row.hi) {
-        const int h = row.r / a.groups;
-        int heads;   // of this row
-        const int64_t q_row = q_row_of(row.s, row.r, heads);
+        const MxCols cols = cols_of(row);
+        const int h = cols.h, heads = cols.count;
         const MxRow nxt = next_row(row);
-        const int nxt_h = nxt.r / a.groups;
+        const int nxt_h = cols_of(nxt).h;
+        // keys this lane's column sees (a chunk's tokens: up to their own positions), and
+        // those that every column of the row does
+        int seen = row.ctx, seen_all = row.ctx;
+        if constexpr (CHUNK) {
+            const int tok = static_cast<int>(static_cast<uint32_t>(cols.col + min(l16, heads - 1)) / static_cast<uint32_t>(G));
+            seen = min(seen, row.cached + tok + 1);
+            seen_all = min(seen_all, row.cached + static_cast<int>(static_cast<uint32_t>(cols.col) / static_cast<uint32_t>(G)) + 1);
+        }
+        uint32_t nan_blocks = 0;   // chunks: value blocks that are NaN in this lane's column
         const Ids nxt_ids = load_ids(nxt, 0);
 
         // ---- the query rows as E4M3 terms ----
@@ -430,11 +486,11 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                 load_k(p0, p1, x);
             }
             const int t0 = (row.lo + wave + WAVES * k) * MXD_ITEM;
-            const bool full = here == 3u && t0 + MXD_ITEM <= row.ctx;
+            const bool full = here == 3u && t0 + MXD_ITEM <= seen_all;
             if (!full) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const bool ok = ((here >> (e >> 2)) & 1u) && t0 + 16 * (e >> 2) + 4 * grp + (e & 3) < row.ctx;
+                    const bool ok = ((here >> (e >> 2)) & 1u) && t0 + 16 * (e >> 2) + 4 * grp + (e & 3) < seen;
                     sc[e] = ok ? sc[e] : -INFINITY;
                 }
             }
@@ -471,7 +527,17 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                     w = ok ? w : make_uint4(0, 0, 0, 0);
                     e = ok ? e : 127u;
                 }
-                const float f = e > MX4_TOP_SCALE ? INFINITY : mx4_factor(e);   // NaN
+                float f = e > MX4_TOP_SCALE ? INFINITY : mx4_factor(e);   // NaN
+                if constexpr (CHUNK) {
+                    // A NaN block enters with a finite factor and marks the columns that see its
+                    // token: a weight of 0 would not keep NaN out of the others.
+                    uint64_t bad = __builtin_amdgcn_ballot_w64(e > MX4_TOP_SCALE);
+                    f = e > MX4_TOP_SCALE ? 1.f : f;
+                    for (; bad; bad &= bad - 1) {
+                        const int at_lane = 64 * j + __ffsll(static_cast<unsigned long long>(bad)) - 1;
+                        nan_blocks |= t0 + at_lane / NB < seen ? 1u << (at_lane % NB) : 0u;
+                    }
+                }
                 if (NB % 2 == 0 || idx < 2 * MX4_TOKENS * NB) {
                     uint4* dst = reinterpret_cast<uint4*>(v_lds + tok * ROW + 32 * b);
                     const int sw = (b & 3) ^ (2 * ((tok >> 2) & 1));
@@ -522,6 +588,7 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
             if (grp == 0) {
                 ml_lds[wave][l16][0] = m;
                 ml_lds[wave][l16][1] = l;
+                if constexpr (CHUNK) nan_lds[wave][l16] = nan_blocks;
             }
             float* dst = reinterpret_cast<float*>(v_lds) + l16 * D + 4 * grp;
 #pragma unroll
@@ -549,9 +616,15 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                     y1 += f * y[1];
                 }
             }
+            if constexpr (CHUNK) {
+                uint32_t nans = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) nans |= nan_lds[w][hd];
+                if ((nans >> (e % D / MX4_BLOCK)) & 1u) y0 = y1 = __builtin_nanf("");
+            }
             if (piece.count == 1) {
                 const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                *reinterpret_cast<uint32_t*>(a.out + q_row * D + e) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
+                *reinterpret_cast<uint32_t*>(a.out + q_row_of(cols, hd) * D + e % D) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
             } else {
                 store2(a.part_o + slot * (MXD_HEADS * D) + e, y0, y1);
                 if (e == hd * D) store2(a.part_ml + slot * (2 * MXD_HEADS) + 2 * hd, mm, ll);
@@ -581,27 +654,27 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
     for (int side = 0; side < 2; ++side) {
         if (!last_lds[side]) continue;   // uniform
         const Piece x = side ? tail : head;
-        int heads;
-        const int64_t q_row = q_row_of(x.s, x.r, heads);
+        const int heads = x.cols.count;
         if (tid == 0) __hip_atomic_store(a.counters + x.first_wg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // piece p's slot: the row starts in its first workgroup's last piece
         // (slot 2 wg + 1) and goes on in the others' first
         auto slot_of = [&](int p) __attribute__((always_inline)) { return 2 * static_cast<int64_t>(x.first_wg + p) + (p == 0 ? 1 : 0); };
         // the first pieces' outputs travel with the factors
         const int e0 = 2 * tid;
-        float u[8], v[8];
-        auto load8 = [&](int p0, int e) __attribute__((always_inline)) {
+        float u[MXD_JOIN_LOADS], v[MXD_JOIN_LOADS];
+        auto load_some = [&](int p0, int e) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < MXD_JOIN_LOADS; ++k)
                 load2(a.part_o + slot_of(min(p0 + k, x.count - 1)) * (MXD_HEADS * D) + e, u[k], v[k]);
         };
-        if (e0 < heads * D) load8(0, e0);
+        if (e0 < heads * D) load_some(0, e0);
         // a wave a head, a lane a piece: the pieces' factors and the row's sum
         for (int hd = wave; hd < heads; hd += WAVES) {
             float mp = -INFINITY, lp = 0.f;
             if (lane < x.count) load2(a.part_ml + slot_of(lane) * (2 * MXD_HEADS) + 2 * hd, mp, lp);
             const float top = wave_max(mp);
-            const float f = lp == 0.f ? 0.f : __builtin_amdgcn_exp2f(mp - top);
+            // a piece that saw a key keeps a factor, however small: NaN values go on
+            const float f = lp == 0.f ? 0.f : fmaxf(__builtin_amdgcn_exp2f(mp - top), MX4_LEAST);
             const float L = wave_sum(lp == 0.f ? 0.f : f * lp);
             if (lane < x.count) w_lds[lane][hd] = f;
             if (lane == 0) ml_lds[0][hd][0] = L == 0.f ? 0.f : 1.f / L;
@@ -610,10 +683,10 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
         for (int e = e0; e < heads * D; e += 2 * THREADS) {
             const int hd = e / D;
             float y0 = 0.f, y1 = 0.f;
-            for (int p0 = 0; p0 < x.count; p0 += 8) {
-                if (p0 > 0 || e > e0) load8(p0, e);
+            for (int p0 = 0; p0 < x.count; p0 += MXD_JOIN_LOADS) {
+                if (p0 > 0 || e > e0) load_some(p0, e);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < MXD_JOIN_LOADS; ++k) {
                     const float f = p0 + k < x.count ? w_lds[p0 + k][hd] : 0.f;
                     if (f != 0.f) {
                         y0 += f * u[k];
@@ -622,7 +695,7 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                 }
             }
             const float inv = ml_lds[0][hd][0];
-            *reinterpret_cast<uint32_t*>(a.out + q_row * D + e) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
+            *reinterpret_cast<uint32_t*>(a.out + q_row_of(x.cols, hd) * D + e % D) = mx4_pack16<QKIND>(y0 * inv, y1 * inv);
         }
         __syncthreads();   // before the other row's factors
     }
@@ -646,6 +719,14 @@ int64_t mxd_scratch_bytes(int64_t wgs, int64_t d) {
 constexpr int64_t MXD_SHORT = 2048;   // tokens
 
 // Workgroups: what the device holds, fewer where the tables hold less than one item a wave.
+int64_t mxd_at_most(int64_t rows, int64_t d, int64_t bs, int64_t maxb, int cus, int waves) {
+    const int64_t items = (maxb * bs + MXD_ITEM - 1) / MXD_ITEM;
+    const int64_t most = rows * (items > waves ? (items + waves - 1) / waves : 1);
+    int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d, waves);
+    if (held > MXD_MAX_WGS) held = MXD_MAX_WGS;
+    return most < held ? most : held;
+}
+
 int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t* wgs,
                        int* waves) {
     int dev = 0, cus = 0;
@@ -653,11 +734,7 @@ int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t groups = (hq / hkv + MXD_HEADS - 1) / MXD_HEADS, rows = num_seqs * hkv * groups;
     *waves = rows >= static_cast<int64_t>(cus) * mxd_per_cu(d, 2) && maxb * bs <= MXD_SHORT ? 2 : 4;
-    const int64_t items = (maxb * bs + MXD_ITEM - 1) / MXD_ITEM;
-    const int64_t most = rows * (items > *waves ? (items + *waves - 1) / *waves : 1);
-    int64_t held = static_cast<int64_t>(cus) * mxd_per_cu(d, *waves);
-    if (held > MXD_MAX_WGS) held = MXD_MAX_WGS;
-    *wgs = most < held ? most : held;
+    *wgs = mxd_at_most(rows, d, bs, maxb, cus, *waves);
     return 0;
 }
 
@@ -670,11 +747,11 @@ int32_t mxd_check(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t 
     return 0;
 }
 
-template <int QKIND, int WAVES>
+template <int QKIND, int WAVES, bool CHUNK>
 int32_t mxd_launch(const MxDecodeArgs& a, int64_t d, int64_t wgs, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(wgs)), block(64 * WAVES);
     switch (d / 32) {
-#define MXD_CASE(NB) case NB: hipLaunchKernelGGL((mx4_decode_kernel<QKIND, NB, WAVES>), grid, block, 0, st, a); break;
+#define MXD_CASE(NB) case NB: hipLaunchKernelGGL((mx4_decode_kernel<QKIND, NB, WAVES, CHUNK>), grid, block, 0, st, a); break;
         MXD_CASE(1) MXD_CASE(2) MXD_CASE(3) MXD_CASE(4) MXD_CASE(5) MXD_CASE(6) MXD_CASE(7) MXD_CASE(8)
 #undef MXD_CASE
         default: return static_cast<int32_t>(hipErrorInvalidValue);
@@ -682,7 +759,67 @@ int32_t mxd_launch(const MxDecodeArgs& a, int64_t d, int64_t wgs, hipStream_t st
     return launch_status();
 }
 
+MxDecodeArgs mxd_args(void* out, const void* q, const uint8_t* kc, const uint8_t* vc, const int32_t* bt,
+                      const int32_t* seq_lens, int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs,
+                      int64_t maxb, int64_t nb, float scale, void* ws, int64_t wgs) {
+    MxDecodeArgs a{};
+    a.out = static_cast<uint16_t*>(out);
+    a.q = static_cast<const uint16_t*>(q);
+    a.kc = kc;
+    a.vc = vc;
+    a.bt = bt;
+    a.seq_lens = seq_lens;
+    a.num_seqs = static_cast<int32_t>(num_seqs);
+    a.hq = static_cast<int32_t>(hq);
+    a.hkv = static_cast<int32_t>(hkv);
+    a.bs = static_cast<int32_t>(bs);
+    a.subs = static_cast<int32_t>(bs / MX4_TOKENS);
+    a.subs_mul = ((uint64_t(1) << 32) + a.subs - 1) / a.subs;   // exact quotients below 2^23
+    a.maxb = static_cast<int32_t>(maxb);
+    a.nb = static_cast<int32_t>(nb);
+    a.c = scale * MX4_LOG2E;
+    if (ws) {
+        a.counters = static_cast<uint32_t*>(ws);
+        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + MXD_COUNTER_BYTES);
+        a.part_ml = a.part_o + 2 * wgs * MXD_HEADS * d;
+    }
+    return a;
+}
+
 }  // namespace
+
+int64_t mx4_short_rows(int64_t num_seqs, int64_t num_tokens, int64_t hq, int64_t hkv, int64_t bs, int64_t maxb,
+                       int64_t most_cols) {
+    // ceil(c / 16) <= (c - 1) / 16 + 1 for the c > 0 columns of a sequence
+    const int64_t used = num_seqs < num_tokens ? num_seqs : num_tokens;
+    int64_t rows = ((num_tokens * (hq / hkv) - used) / MXD_HEADS + used) * hkv;
+    const int64_t most = used * hkv * ((most_cols + MXD_HEADS - 1) / MXD_HEADS);
+    if (rows > most) rows = most;
+    // the items of all rows are counted in 32 bits
+    return rows * ((maxb * bs + MXD_ITEM - 1) / MXD_ITEM + 1 + MXD_VIRT) <= INT32_MAX ? rows : -1;
+}
+
+int32_t mx4_short_chunks(void* out, const void* q, const uint8_t* kc, const uint8_t* vc, const int32_t* bt,
+                         const int32_t* seq_lens, const int32_t* qsl, int64_t num_seqs, int64_t num_tokens, int64_t hq,
+                         int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t nb, float scale, int32_t q_dtype,
+                         int64_t most_cols, uintptr_t stream) {
+    int dev = 0, cus = 0;
+    RLLM_TRY(hipGetDevice(&dev));
+    RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    const int64_t rows = mx4_short_rows(num_seqs, num_tokens, hq, hkv, bs, maxb, most_cols);
+    RLLM_CHECK_ARG(rows > 0);
+    const int64_t wgs_at_most = mxd_at_most(rows, d, bs, maxb, cus, 4);
+    void* ws = nullptr;
+    RLLM_TRY(static_cast<hipError_t>(g_workspaces.get(stream, WS_MX4_DECODE, mxd_scratch_bytes(wgs_at_most, d), true, &ws)));
+    const int64_t wgs = ws ? wgs_at_most : rows;   // captured before any eager call of this size: a workgroup a row
+    MxDecodeArgs a = mxd_args(out, q, kc, vc, bt, seq_lens, num_seqs, hq, hkv, d, bs, maxb, nb, scale, ws, wgs);
+    a.qsl = qsl;
+    a.num_tokens = static_cast<int32_t>(num_tokens);
+    a.most_cols = static_cast<int32_t>(most_cols);
+    return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 4, true>(a, d, wgs, as_stream(stream))
+                                      : mxd_launch<KIND_F16, 4, true>(a, d, wgs, as_stream(stream));
+}
+
 }  // namespace rllm
 
 using namespace rllm;
@@ -731,34 +868,14 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
             RLLM_CHECK_ARG(wgs <= INT32_MAX);
         }
     }
-    MxDecodeArgs a{};
-    a.out = static_cast<uint16_t*>(output);
-    a.q = static_cast<const uint16_t*>(query);
-    a.kc = key_cache;
-    a.vc = value_cache;
-    a.bt = block_tables;
-    a.seq_lens = seq_lens;
-    a.num_seqs = static_cast<int32_t>(num_seqs);
-    a.hq = static_cast<int32_t>(num_q_heads);
-    a.hkv = static_cast<int32_t>(num_kv_heads);
-    a.groups = static_cast<int32_t>((num_q_heads / num_kv_heads + MXD_HEADS - 1) / MXD_HEADS);
-    a.bs = static_cast<int32_t>(block_size);
-    a.subs = static_cast<int32_t>(block_size / MX4_TOKENS);
-    a.subs_mul = ((uint64_t(1) << 32) + a.subs - 1) / a.subs;   // exact quotients below 2^23
-    a.maxb = static_cast<int32_t>(max_num_blocks_per_seq);
-    a.nb = static_cast<int32_t>(num_blocks);
-    a.c = scale * MX4_LOG2E;
-    if (ws) {
-        a.counters = static_cast<uint32_t*>(ws);
-        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + MXD_COUNTER_BYTES);
-        a.part_ml = a.part_o + 2 * wgs * MXD_HEADS * head_dim;
-    }
+    const MxDecodeArgs a = mxd_args(output, query, key_cache, value_cache, block_tables, seq_lens, num_seqs, num_q_heads,
+                                    num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks, scale, ws, wgs);
     hipStream_t st = as_stream(stream);
     if (waves == 2)
-        return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 2>(a, head_dim, wgs, st)
-                                          : mxd_launch<KIND_F16, 2>(a, head_dim, wgs, st);
-    return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 4>(a, head_dim, wgs, st)
-                                      : mxd_launch<KIND_F16, 4>(a, head_dim, wgs, st);
+        return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 2, false>(a, head_dim, wgs, st)
+                                          : mxd_launch<KIND_F16, 2, false>(a, head_dim, wgs, st);
+    return q_dtype == RLLM_DTYPE_BF16 ? mxd_launch<KIND_BF16, 4, false>(a, head_dim, wgs, st)
+                                      : mxd_launch<KIND_F16, 4, false>(a, head_dim, wgs, st);
 }
 
 }  // extern "C"

@@ -7,15 +7,24 @@
 //
 // Work.  The rows of a (sequence, kv head) are its (token, query head of the
 // group) pairs, token by token; a workgroup takes 32 rows a wave.  Keys go by in
-// tiles of 64 tokens, staged in LDS by all waves: K's code rows as they are
-// ([32-element block][token][16 bytes], one scale byte each), V converted exactly to
-// bf16 ([token][D]).  A wave's products: S^T = K Q^T on the block-scaled 32x32x64
+// tiles of 64 tokens, staged in LDS: K's code rows as they are ([32-element
+// block][token][16 bytes], one scale byte each), V converted exactly to bf16
+// ([token][D]).  A wave's products: S^T = K Q^T on the block-scaled 32x32x64
 // product (A = K from LDS, B = the query terms in registers), so lane l holds the
 // scores of row l % 32; the softmax stays in the lane and its partner l ^ 32; the
 // weights, rounded to bf16, are the B operand of O^T = V^T P^T as they stand, with V
 // read back from LDS transposed.  f16 queries take two terms a weight (16 bits
 // against the output's 11); bf16 ones one, like the 16-bit caches' kernel: an error
 // of at most half a bf16 step a weight, the size of the output's own rounding.
+//
+// The waves are two groups, one a turn behind the other: while one group's wave on a
+// SIMD keeps the matrix core, the other's does its softmax and its copy (group 0 brings
+// V, group 1 K).  With all waves in step, staging together, 2 chunks of 1500-2048 tokens on
+// 14000 took 1038 us, in turns 909 (820 after the later steps).
+//
+// Measured (32/8 heads, head_dim 128, bf16): 8 sequences of 512 new tokens on 2048, 155
+// GF, 151 us (1025 TF/s); 2 of 1500-2048 on 14000, 963 GF, 820 us (1174 TF/s), where a
+// large bf16 product runs at 1242 on the same card.
 #include "mxfp4_attention.h"
 #include "workspace.h"
 #include "../../include/rllm_kernels.h"
@@ -28,6 +37,22 @@ constexpr int MXP_SUBS = MXP_TILE / MX4_TOKENS;
 // Rounds of workgroups up to which the query tiles go by falling key counts: with
 // more, the last round is a small part.
 constexpr int MXP_SORTED_ROUNDS = 4;
+
+// Sequences of few new tokens leave most of a workgroup's 256 rows empty, and stream their
+// context at the pace of a single wave's turns: the decode kernel takes them, a column a
+// row, 16 columns a pass over the context.
+//  - In a batch that may hold both (more than one sequence, no key split, not too many
+//    columns a sequence on average: past MXP_SOME_SHORT the short ones are a small part of
+//    the time, and the second launch costs 3 us) each sequence goes where its own columns
+//    say, up to MXP_SHORT_COLS (twice that past head_dim 128, where this kernel has one wave a
+//    SIMD).  32/8 heads, head_dim 128, us of this kernel / of both: 64 sequences of 4 tokens
+//    on 2000 107 / 38.7, 32 of 8 55.5 / 37.9; 63 of 1 and one of 512 on 2000 155 / 107; 32 of
+//    16 (64 columns) 57 / 60.4 (head_dim 256, 16/4 heads: 189 / 138); 15 of 1 and one of 512 on
+//    8000, which can no longer overlap, 219 / 253.
+//  - Where tables are at most MXP_ALL_SHORT tokens wide and the rows of 16 columns no more
+//    than the workgroups the device holds, the call is all latency and the decode kernel cuts
+//    it finer: 120 fresh tokens 14.9 / 9.5 us, on 500 25.4 / 20.6, on 1000 24.2 / 23.1, on 2000 26.6 / 28.1.
+constexpr int64_t MXP_SHORT_COLS = 32, MXP_SOME_SHORT = 1024, MXP_ALL_SHORT = 1024;
 
 // 8 waves, two a SIMD, up to head_dim 128; past it a wave needs the registers of two
 template <int NB> constexpr int mxp_waves() { return NB <= 4 ? 8 : 4; }
@@ -44,6 +69,7 @@ struct MxPrefillArgs {
     float c;                // scale * log2(e)
     int32_t splits, base_wgs;
     int32_t longest_first;  // query tiles by falling key counts
+    int32_t short_cols;     // sequences of up to this many rows are not for this kernel
     float* part_o;          // [num_tokens * hq][splits][D], relative to the part's max
     float* part_ml;         // [num_tokens * hq][splits][2]
 };
@@ -127,6 +153,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
         if (s0 + lane < a.num_seqs) {
             q0_l = min(max(a.qsl[s0 + lane], 0), a.num_tokens);
             n_l = min(max(a.qsl[s0 + lane + 1], q0_l), a.num_tokens) - q0_l;
+            n_l = n_l * G <= a.short_cols ? 0 : n_l;
         }
         const int nt_l = (n_l * G + ROWS - 1) / ROWS;
         if (a.longest_first) {   // at most 64 sequences
@@ -556,7 +583,7 @@ __global__ __launch_bounds__(256) void mx4_prefill_merge_kernel(MxPrefillArgs a,
         lp = x[1];
     }
     const float top = wave_max(mp);
-    const float f = lp == 0.f ? 0.f : __builtin_amdgcn_exp2f(mp - top);
+    const float f = lp == 0.f ? 0.f : fmaxf(__builtin_amdgcn_exp2f(mp - top), MX4_LEAST);   // NaN values go on
     const float L = wave_sum(lp == 0.f ? 0.f : f * lp);
     const int d0 = 4 * lane;
     if (d0 >= d) return;
@@ -630,11 +657,33 @@ extern "C" int32_t rllm_paged_attention_prefill_mxfp4(
     a.c = scale * MX4_LOG2E;
     a.base_wgs = static_cast<int32_t>(wgs);
     a.splits = 1;
-    // few query tiles over long contexts: several workgroups a tile, each on a part of the keys
     int dev = 0, cus = 0;
     RLLM_TRY(hipGetDevice(&dev));
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-    const int64_t tiles = (max_num_blocks_per_seq * block_size + MXP_TILE - 1) / MXP_TILE;
+    const int64_t width = max_num_blocks_per_seq * block_size;
+    const int64_t every = num_tokens * group;   // columns
+    auto short_rows = [&](int64_t most) {
+        return mx4_short_rows(num_seqs, num_tokens, num_q_heads, num_kv_heads, block_size, max_num_blocks_per_seq, most);
+    };
+    auto short_chunks = [&](int64_t most) {
+        return mx4_short_chunks(output, query, key_cache, value_cache, block_tables, seq_lens, query_start_loc, num_seqs,
+                                num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq,
+                                num_blocks, scale, q_dtype, most, stream);
+    };
+    if (width <= MXP_ALL_SHORT) {
+        const int64_t rows = short_rows(every);
+        if (rows > 0 && rows <= static_cast<int64_t>(cus) * mxd_per_simd(head_dim)) return short_chunks(every);
+    }
+    if (num_seqs > 1 && every <= MXP_SOME_SHORT * num_seqs && 2 * wgs > cus) {
+        const int64_t most = head_dim <= 128 ? MXP_SHORT_COLS : 2 * MXP_SHORT_COLS;
+        if (short_rows(most) > 0) {
+            const int32_t rc = short_chunks(most);
+            if (rc) return rc;
+            a.short_cols = static_cast<int32_t>(most);
+        }
+    }
+    // few query tiles over long contexts: several workgroups a tile, each on a part of the keys
+    const int64_t tiles = (width + MXP_TILE - 1) / MXP_TILE;
     a.longest_first = num_seqs > 1 && num_seqs <= 64 && wgs > cus && wgs <= MXP_SORTED_ROUNDS * cus;
     int64_t splits = cus / wgs;
     if (splits > tiles / 4) splits = tiles / 4;
