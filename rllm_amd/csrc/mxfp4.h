@@ -35,6 +35,8 @@ inline bool mx4_shape_ok(int64_t hkv, int64_t d, int64_t bs, int64_t nb) {
            bs % MX4_TOKENS == 0 && bs <= 4096 && nb >= 0 && nb <= (int64_t(1) << 31) - 1;
 }
 
+constexpr int64_t MX4_MAX_THREADS = (int64_t(1) << 32) - 1;   // of a launch
+
 // the tables and heads of the two attention operators
 inline bool mx4_attention_ok(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t bs, int64_t maxb) {
     return hq > 0 && hq <= 1024 && hq % hkv == 0 && num_seqs <= (int64_t(1) << 20) && maxb >= 0 &&
@@ -110,6 +112,15 @@ __device__ __forceinline__ uint32_t mx4_scale_byte(float amax, bool finite) {
 __device__ __forceinline__ uint32_t mx4_quad_max(uint32_t v) {
     v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), DPP_QUAD_XOR1, 0xF, 0xF, false)));
     return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), DPP_QUAD_XOR2, 0xF, 0xF, false)));
+}
+
+// largest magnitude of 8 16-bit floats, as their 15-bit pattern (patterns rise
+// with the magnitude, infinities and NaNs above every finite value)
+__device__ __forceinline__ uint32_t mx4_amax8(const uint4& w) {
+    const mx_u16x2 a = __builtin_bit_cast(mx_u16x2, w.x & 0x7fff7fffu), b = __builtin_bit_cast(mx_u16x2, w.y & 0x7fff7fffu);
+    const mx_u16x2 c = __builtin_bit_cast(mx_u16x2, w.z & 0x7fff7fffu), d = __builtin_bit_cast(mx_u16x2, w.w & 0x7fff7fffu);
+    const mx_u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(a, b), __builtin_elementwise_max(c, d));
+    return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
 }
 
 }  // namespace rllm

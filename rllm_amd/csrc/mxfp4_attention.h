@@ -97,14 +97,6 @@ __device__ __forceinline__ void mx4_split4(uint32_t p0, uint32_t p1, float facto
     }
 }
 
-// largest 15-bit pattern of 8 16-bit floats (patterns rise with the magnitude,
-// infinities and NaNs above every finite value)
-__device__ __forceinline__ uint32_t mx4_amax8(const uint4& w) {
-    const mx_u16x2 a = __builtin_bit_cast(mx_u16x2, w.x & 0x7fff7fffu), b = __builtin_bit_cast(mx_u16x2, w.y & 0x7fff7fffu);
-    const mx_u16x2 c = __builtin_bit_cast(mx_u16x2, w.z & 0x7fff7fffu), d = __builtin_bit_cast(mx_u16x2, w.w & 0x7fff7fffu);
-    const mx_u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(a, b), __builtin_elementwise_max(c, d));
-    return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
-}
 __device__ __forceinline__ uint32_t mx4_umax_32(uint32_t v) {
     const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));

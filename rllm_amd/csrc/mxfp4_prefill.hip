@@ -631,13 +631,13 @@ extern "C" int32_t rllm_paged_attention_prefill_mxfp4(
     RLLM_CHECK_ARG(mx4_attention_ok(num_seqs, num_q_heads, num_kv_heads, block_size, max_num_blocks_per_seq));
     RLLM_CHECK_ARG(num_tokens <= (int64_t(1) << 26) && num_tokens * (num_q_heads / num_kv_heads) <= (int64_t(1) << 30));
     RLLM_CHECK_ARG(q_dtype == RLLM_DTYPE_F16 || q_dtype == RLLM_DTYPE_BF16);
-    RLLM_CHECK_ARG(std::isfinite(scale));
+    RLLM_CHECK_ARG(std::isfinite(scale * MX4_LOG2E));
     RLLM_CHECK_ARG(mx4_aligned16(key_cache) && mx4_aligned16(value_cache) && mx4_aligned16(query));
     RLLM_CHECK_ARG((reinterpret_cast<uintptr_t>(output) & 7) == 0);
     const int64_t group = num_q_heads / num_kv_heads, rows_wg = head_dim <= 128 ? 256 : 128;
     // ceil(r / rows_wg) <= (r - 1) / rows_wg + 1 for every r >= 0; workgroups past the last tile find none
     const int64_t wgs = ((num_tokens * group - num_seqs) / rows_wg + num_seqs) * num_kv_heads;
-    RLLM_CHECK_ARG(wgs <= INT32_MAX);
+    RLLM_CHECK_ARG(wgs * 512 <= MX4_MAX_THREADS);
     MxPrefillArgs a{};
     a.out = static_cast<uint16_t*>(output);
     a.q = static_cast<const uint16_t*>(query);

@@ -70,6 +70,14 @@ def test_prefill_refuses():
     assert prefill(b=0, o=0) == 0 and prefill(t=0) == 0
 
 
+def test_launches_past_the_devices_limit_are_refused():
+    n = (1 << 31) - 1                                # 2^32 threads and more
+    assert write(n=n, hkv=1024) == 1 and read(n=n, hkv=1024) == 1 and rope(n=n, hkv=1024) == 1
+    assert prefill(b=1 << 20, t=1 << 26, hq=1024, hkv=1024, maxb=1) == 1
+    for f in (decode, prefill):                      # finite, but not in units of log2
+        assert f(scale=3e38) == 1
+
+
 def test_sizes():
     L = rllm_amd.lib()
     assert L.rllm_mxfp4_page_bytes(128, 16) == 16 * (64 + 4) == M.page_bytes(128, 16)
