@@ -138,3 +138,23 @@ def test_nan_of_a_part_with_next_to_no_weight(dev, new):
     want[:, 4:, 64:96] = True
     out = ops.paged_prefill_mxfp4(*dev_args(*c, dev), 0.09) if new else ops.paged_decode_mxfp4(*decode_args(*c, dev), 0.09)
     assert np.array_equal(torch.isnan(out).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("new,ctx,wide", [([40, 3], [200, 64], 0), ([90, 40], [200, 64], 40), ([4], [230], 40)])
+def test_long_cache_past_32_bits(dev, new, ctx, wide):
+    """The contexts' blocks lie past 2^32 bytes; tables of their own width and far wider ones."""
+    rng = np.random.default_rng(17)
+    nb, hkv, d, bs = 70000, 8, 256, 32
+    kt, vt = (ops.mxfp4_cache(nb, hkv, d, bs, dev) for _ in range(2))
+    kc, vc = M.Cache.random(rng, 12, hkv, d, bs), M.Cache.random(rng, 12, hkv, d, bs)
+    kt[nb - 12:] = torch.from_numpy(kc.pages()).to(dev)
+    vt[nb - 12:] = torch.from_numpy(vc.pages()).to(dev)
+    bt = np.full((len(new), 8 + wide), -1, np.int32)
+    for s in range(len(new)):
+        bt[s, :8] = rng.permutation(12)[:8]
+    q = torch.from_numpy(rng.standard_normal((sum(new), 16, d))).to(torch.bfloat16).to(dev)
+    lens, qsl = np.array(ctx, np.int32), np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    far = np.where(bt >= 0, bt + nb - 12, -1).astype(np.int32)
+    out = ops.paged_prefill_mxfp4(q, kt, vt, *(torch.from_numpy(x).to(dev) for x in (far, lens, qsl)), 0.06)
+    ref, mag, big = reference(q, kc, vc, bt, lens, qsl, 0.06)
+    M.check_attention(out.float().cpu().numpy(), ref, mag, big, "bf16", WEIGHT["bf16"], "past 32 bits")
