@@ -89,9 +89,11 @@ __device__ __forceinline__ int mxp_longest(int n, int ctx, int nt, int G, int ra
     constexpr int SH = __builtin_ctz(ROWS);
     ctx = min(max(ctx, 0), 1 << 27);
     auto above = [&](int steps) __attribute__((always_inline)) {
-        // tile i's last token is (ROWS (i + 1) - 1) / G, and attends it and ctx - n more
+        // tile i's last token is (ROWS (i + 1) - 1) / G, and attends it and ctx - n more;
+        // below 0 steps every tile counts, those without a key (ctx < n) too
+        if (steps < 0) return nt;
         const int x = min(max(steps * MXP_TILE - (ctx - n), 0), n);
-        return nt > 0 && (ctx > steps * MXP_TILE || steps < 0) ? nt - min(nt - 1, (x * G) >> SH) : 0;
+        return nt > 0 && ctx > steps * MXP_TILE ? nt - min(nt - 1, (x * G) >> SH) : 0;
     };
     auto all_above = [&](int steps) __attribute__((always_inline)) {
         return __builtin_amdgcn_readlane(mx4_scan(above(steps)), 63);
