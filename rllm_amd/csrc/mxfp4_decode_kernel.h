@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
     };
 
     MxRow row{};
-    int virt = 0;     // items a row's start counts for in the list
+    int virt = 0;     // items a row's start counts for in the list; -1: rows are cut apart
     int end, share;   // the end of this workgroup's items in the list, and the items of a workgroup
     {
         // ---- the share: every wave works it out from the lengths.  Those of up to 64
@@ -248,16 +248,17 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
         row.q0 = __builtin_amdgcn_readfirstlane(row.q0);
         row.cached = __builtin_amdgcn_readfirstlane(row.cached);
         row.lo = max(pos - row.first, 0);
-        if (apart) virt = stride;   // the next row begins past this share
+        if (apart) virt = -1;   // no other row in this share
     }
     row.hi = min(end - row.first, row.items);
 
     // the row after this one, empty (lo == hi) past the share
     auto next_row = [&](const MxRow& x) __attribute__((always_inline)) -> MxRow {
         MxRow y = x;
-        y.first = x.first + x.items + virt;
         y.lo = 0;
         y.hi = 0;
+        if (virt < 0) return y;   // rows cut apart: their strides' sum may be just below 2^31
+        y.first = x.first + x.items + virt;
         if (y.first >= end) return y;
         if (++y.r == a.hkv * groups_of(x.n)) {
             y.r = 0;
