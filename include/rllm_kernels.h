@@ -598,9 +598,12 @@ int32_t rllm_rope_cache_write_mxfp4(void *q_out, const void *q, const void *k, c
  * workspace: at least rllm_paged_attention_decode_mxfp4_workspace_size(...) bytes,
  * 16-byte aligned, zero-filled before its first such call (each completed call
  * leaves it ready for the next, of any size it is large enough for); calls that
- * share it must not overlap in time.
- * NULL: a library-owned buffer per (device, stream); a capture on a stream that
- * has none of the size yet runs a workgroup a (sequence, kv head) and needs none.
+ * share it must not overlap in time.  The size for a batch and a table width (blocks
+ * times block size) serves every call of the same heads and head_dim with no more
+ * sequences and no wider tables.
+ * NULL: a library-owned buffer per (device, stream), sized by the same rule; a capture
+ * on a stream that has none of the size yet runs a workgroup a (sequence, kv head)
+ * and needs none.
  * Graphs captured on one stream share its buffer with each other and with eager
  * calls there: run them in order, or give each its own workspace. */
 int32_t rllm_paged_attention_decode_mxfp4(void *output, const void *query, const uint8_t *key_cache,

@@ -13,14 +13,19 @@ namespace {
 // 512 12.5 / 17.0.
 constexpr int64_t MXD_SHORT = 2048;   // tokens
 
+// *wgs, *waves: of this call; *most: workgroups of any call of these heads with no more
+// sequences and no wider tables, for which scratch is sized.  Where rows are many, narrow
+// tables take more (of two waves) than wide ones.
 int32_t mxd_workgroups(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t maxb, int64_t* wgs,
-                       int* waves) {
+                       int* waves, int64_t* most) {
     int dev = 0, cus = 0;
     RLLM_TRY(hipGetDevice(&dev));
     RLLM_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t groups = (hq / hkv + MXD_HEADS - 1) / MXD_HEADS, rows = num_seqs * hkv * groups;
-    *waves = rows >= static_cast<int64_t>(cus) * mxd_per_cu(d, 2) && maxb * bs <= MXD_SHORT ? 2 : 4;
+    const bool many = rows >= static_cast<int64_t>(cus) * mxd_per_cu(d, 2);
+    *waves = many && maxb * bs <= MXD_SHORT ? 2 : 4;
     *wgs = mxd_at_most(rows, d, bs, maxb, cus, *waves);
+    *most = mxd_at_most(rows, d, bs, maxb, cus, many ? 2 : 4);
     return 0;
 }
 
@@ -45,10 +50,11 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
                                                          int64_t max_num_blocks_per_seq) {
     if (num_seqs <= 0) return 0;
     if (mxd_check(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, 0)) return -1;
-    int64_t wgs = 0;
+    int64_t wgs = 0, most = 0;
     int waves = 0;
-    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves)) return -1;
-    return mxd_scratch_bytes(wgs, head_dim);
+    if (mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves, &most))
+        return -1;
+    return mxd_scratch_bytes(most, head_dim);
 }
 
 int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const uint8_t* key_cache,
@@ -67,16 +73,15 @@ int32_t rllm_paged_attention_decode_mxfp4(void* output, const void* query, const
     RLLM_CHECK_ARG(std::isfinite(scale * MX4_LOG2E));
     RLLM_CHECK_ARG(mx4_aligned16(key_cache) && mx4_aligned16(value_cache));
     RLLM_CHECK_ARG(((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(output)) & 3) == 0);
-    int64_t wgs = 0;
+    int64_t wgs = 0, most = 0;
     int waves = 0;
-    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves);
+    const int32_t rc = mxd_workgroups(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, &wgs, &waves, &most);
     if (rc) return rc;
-    const int64_t need = mxd_scratch_bytes(wgs, head_dim);
     void* ws = workspace;
     if (ws) {
-        RLLM_CHECK_ARG(mx4_aligned16(ws) && workspace_bytes >= need);
+        RLLM_CHECK_ARG(mx4_aligned16(ws) && workspace_bytes >= mxd_scratch_bytes(wgs, head_dim));
     } else {
-        RLLM_TRY(static_cast<hipError_t>(g_workspaces.get(stream, WS_MX4_DECODE, need, true, &ws)));
+        RLLM_TRY(static_cast<hipError_t>(g_workspaces.get(stream, WS_MX4_DECODE, mxd_scratch_bytes(most, head_dim), true, &ws)));
         if (!ws) {   // captured before any eager call of this size: a workgroup a row
             wgs = num_seqs * num_kv_heads * ((num_q_heads / num_kv_heads + MXD_HEADS - 1) / MXD_HEADS);
             RLLM_CHECK_ARG(wgs * 64 * waves <= MX4_MAX_THREADS);
