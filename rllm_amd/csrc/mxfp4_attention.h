@@ -39,6 +39,8 @@ __device__ __forceinline__ void mx4_sub_e4m3(float (&x)[4], uint32_t w, float fa
     x[3] -= b[1];
 }
 
+// What the weights' base is taken ahead of the running max, in log2
+constexpr float MX4_AHEAD = 8.f;
 // the least factor of a part of a row that saw a key (f32's smallest normal)
 constexpr float MX4_LEAST = 1.17549435e-38f;
 

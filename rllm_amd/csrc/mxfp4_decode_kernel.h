@@ -13,7 +13,7 @@
 // comes from the lengths on the device: where the rows are alike each gets workgroups
 // of its own; else the rows' items form one list, cut into equal shares.  The waves
 // of a workgroup take a row's items in turn and join at the row's end in LDS.  A row cut
-// between workgroups leaves partials (sum of p v relative to the piece's max, max, sum of
+// between workgroups leaves partials (sum of p v relative to the piece's m, m, sum of
 // p); the workgroup that completes the row's arrival counter adds the pieces in their
 // order, so repeated calls give the same bits whichever comes last.  Partials are written
 // and read as relaxed agent-scope atomics, which pass by the XCDs' own L2, and each
@@ -496,12 +496,13 @@ __global__ __launch_bounds__(64 * WAVES, mxd_per_simd(32 * NB)) void mx4_decode_
                     sc[e] = ok ? sc[e] : -INFINITY;
                 }
             }
-            // ---- weights against a running max that moves only when a score
-            // passes it by 2^8: no weight passes 2^8, and the outputs are rarely
-            // rescaled ----
+            // ---- weights against m, 2^8 times the running max when it last moved, which
+            // it does only when a score passes m: the outputs are rarely rescaled, and no
+            // weight passes 1, so that sums of large values overflow no sooner than the
+            // softmax's own ----
             const float top = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-            if (__builtin_amdgcn_ballot_w64(top > m + 8.f || m == -INFINITY)) {
-                const float m_new = fmaxf(m, mx4_max_16(top));
+            if (__builtin_amdgcn_ballot_w64(top > m || m == -INFINITY)) {
+                const float m_new = fmaxf(m, mx4_max_16(top) + MX4_AHEAD);
                 const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
                 l *= alpha;
 #pragma unroll

@@ -70,7 +70,7 @@ struct MxPrefillArgs {
     int32_t splits, base_wgs;
     int32_t longest_first;  // query tiles by falling key counts
     int32_t short_cols;     // sequences of up to this many rows are not for this kernel
-    float* part_o;          // [num_tokens * hq][splits][D], relative to the part's max
+    float* part_o;          // [num_tokens * hq][splits][D], relative to 2^8 times the part's max
     float* part_ml;         // [num_tokens * hq][splits][2]
 };
 
@@ -439,8 +439,9 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
             for (int b = 0; b < NB; ++b)
                 nan_blocks |= t * MXP_TILE + key <= pos ? static_cast<uint32_t>(tiles.bad[buf][b][key]) << b : 0u;
     };
-    // ---- scores of tile t -> weights against the max as it stands, which moves only when
-    // a lane's weights sum past 2^8: the tile's own max is not looked for before ----
+    // ---- scores of tile t -> weights against 2^8 times the max as it stands, which moves
+    // only when a lane's weights sum past 1: the tile's own max is not looked for before, and
+    // sums of large values overflow no sooner than the softmax's own ----
     auto mask = [&](int t) __attribute__((always_inline)) {
         const int t0 = t * MXP_TILE;
         const uint32_t present = ring >> (4 * ((t - t_lo) & 7)) & ((1u << MXP_SUBS) - 1);
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
         m = m_new;
     };
     auto weights = [&]() __attribute__((always_inline)) -> float {   // their sum
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        const float mc = m == -INFINITY ? 0.f : __builtin_fmaf(m, c, MX4_AHEAD);
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
@@ -509,7 +510,7 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
                 if (wave_live) {
                     mask(t);
                     const float sum = weights();
-                    rare = __builtin_amdgcn_ballot_w64(!(sum <= 256.f) || m == -INFINITY) || bad_before == t - 1;
+                    rare = __builtin_amdgcn_ballot_w64(!(sum <= 1.f) || m == -INFINITY) || bad_before == t - 1;
                     if (rare) break;
                     l += sum;
                 }
