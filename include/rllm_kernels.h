@@ -625,8 +625,9 @@ int64_t rllm_paged_attention_decode_mxfp4_workspace_size(int64_t num_seqs, int64
  * output 8-byte aligned.  bf16 queries: the weights are rounded to bf16 before they
  * meet the values, as for 16-bit caches (to 16 bits where a sequence has few new
  * tokens); f16: to 16 bits.  Rows of output that query_start_loc leaves out stay as
- * they are; its entries must not fall or pass num_tokens (sequences of one that does
- * may be left unwritten).  Calls of few new tokens use library-owned buffers per
+ * they are; its entries must not fall or pass num_tokens (a call with one that does
+ * may leave any of its outputs unwritten).  Query tokens that see no key, those before
+ * position 0 of a seq_len below its new tokens among them, get zeros.  Calls of few new tokens use library-owned buffers per
  * (device, stream), the decode call's among them, on its terms for captured graphs; a
  * capture on a stream that has none of the size yet runs without. */
 int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,

@@ -20,11 +20,17 @@
 // The waves are two groups, one a turn behind the other: while one group's wave on a
 // SIMD keeps the matrix core, the other's does its softmax and its copy (group 0 brings
 // V, group 1 K).  With all waves in step, staging together, 2 chunks of 1500-2048 tokens on
-// 14000 took 1038 us, in turns 909 (820 after the later steps).
+// 14000 took 1038 us, in turns 909 (800 after the later steps).  That holds up to head_dim
+// 128.  Past it a SIMD has registers for one wave, the groups are on different SIMDs, and
+// a SIMD's matrix core idles while its wave is in its softmax.
 //
 // Measured (32/8 heads, head_dim 128, bf16): 8 sequences of 512 new tokens on 2048, 155
-// GF, 151 us (1025 TF/s); 2 of 1500-2048 on 14000, 963 GF, 820 us (1174 TF/s), where a
-// large bf16 product runs at 1242 on the same card.
+// GF, 150 us (1029 TF/s); 2 of 1500-2048 on 14000, 963 GF, 800 us (1204 TF/s), where a
+// large bf16 product runs at 1242 on the same card.  Replayed from a graph, us of bf16 /
+// f16, whose three 8-bit query terms and two 16-bit weight terms for two and one are 1.75
+// times the matrix time: the first 174 / 229, the second 817 / 1186; the first at head_dim 64 131 / 162, with 16/4
+// heads at 192 193 / 232, at 224 - / 290, at 256 233 / 398.  f16 spills registers to memory at
+// head_dim 64 (36 bytes a lane), 224 (68) and 256 (236), bf16 nowhere.
 #include "mxfp4_attention.h"
 #include "workspace.h"
 #include "../../include/rllm_kernels.h"
@@ -46,15 +52,21 @@ constexpr int MXP_SORTED_ROUNDS = 4;
 //    the time, and the second launch costs 3 us) each sequence goes where its own columns
 //    say, up to MXP_SHORT_COLS (twice that past head_dim 128, where this kernel has one wave a
 //    SIMD).  32/8 heads, head_dim 128, us of this kernel / of both: 64 sequences of 4 tokens
-//    on 2000 107 / 38.7, 32 of 8 55.5 / 37.9; 63 of 1 and one of 512 on 2000 155 / 107; 32 of
-//    16 (64 columns) 57 / 60.4 (head_dim 256, 16/4 heads: 189 / 138); 15 of 1 and one of 512 on
-//    8000, which can no longer overlap, 219 / 253.
+//    on 2000 107 / 38.7, 32 of 8 55.5 / 37.9, 256 of 4 on 500 144 / 69.4; 63 of 1 and one of 512
+//    on 2000 155 / 107; 32 of 4 on 4000 (64/4 heads, head_dim 256) 190 / 138.  What it costs: the
+//    first launch where few or none are short, as only the device knows the lengths (64 of 64
+//    on 500 69.5 / 72.6, 64 of 16 on 500 45.6 / 48.4, 32 of 16 on 2000 57.0 / 60.4, 8 of 512 on
+//    2048 168.6 / 171.4, 64 of 1-400 on 2000 572 / 580); and parts that no longer overlap where
+//    neither fills the card (15 of 1 and one of 512 on 8000 219 / 253).
 //  - Where tables are at most MXP_ALL_SHORT tokens wide and the rows of 16 columns no more
 //    than the workgroups the device holds, the call is all latency and the decode kernel cuts
-//    it finer: 120 fresh tokens 14.9 / 9.5 us, on 500 25.4 / 20.6, on 1000 24.2 / 23.1, on 2000 26.6 / 28.1.
+//    it finer: 120 fresh tokens 14.9 / 9.5 us, on 500 25.4 / 20.6, on 1000 24.2 / 23.1, on 2000
+//    26.6 / 28.1.  Slower: 8 of 4 on 1000 16.2 / 18.1, 8 of 6 16.6 / 19.3, 8 of 8 16.8 / 19.6.  The
+//    host knows the tables' width alone: 120 fresh tokens under tables of 4096 take 22 us.
 constexpr int64_t MXP_SHORT_COLS = 32, MXP_SOME_SHORT = 1024, MXP_ALL_SHORT = 1024;
 
-// 8 waves, two a SIMD, up to head_dim 128; past it a wave needs the registers of two
+// 8 waves, two a SIMD (one of each group), up to head_dim 128; past it a wave needs the
+// registers of two
 template <int NB> constexpr int mxp_waves() { return NB <= 4 ? 8 : 4; }
 
 struct MxPrefillArgs {
@@ -489,8 +501,8 @@ __global__ __launch_bounds__(64 * mxp_waves<NB>(), mxp_waves<NB>() / 4) void mx4
 
     // ---- the turns.  In turn 2t group 0 issues tile t's products (and tile t-1's
     // V products), in turn 2t + 1 its softmax and the copy of V(t); group 1 is one turn
-    // behind, with the copy of K(t + 2).  On every SIMD a wave of one group then keeps the
-    // matrix core while the other's works on the vector units.  K(t) is read in turns 2t
+    // behind, with the copy of K(t + 2).  Where a SIMD holds a wave of each (head_dim up to
+    // 128), one keeps the matrix core while the other works on the vector units.  K(t) is read in turns 2t
     // and 2t + 1, V(t) in 2t + 2 and 2t + 3; K(t + 2) is written over K(t) in turn 2t + 2, V(t)
     // over V(t - 2) in turn 2t + 1. ----
     if (t_lo < t_hi) {
