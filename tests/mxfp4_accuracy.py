@@ -23,8 +23,6 @@ term s a hundred times or more: norms 6 to 100 times what the bound gives."""
 import numpy as np
 import torch
 
-import mxfp4_ref as M
-
 DT = {"bf16": torch.bfloat16, "f16": torch.float16}
 BITS = {"bf16": 7, "f16": 10}
 ONE_TERM, TWO_TERMS = 2.0 ** -8 / np.sqrt(3), 2.0 ** -16 / 3
