@@ -640,6 +640,106 @@ int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,
                                            int64_t num_blocks, float scale, int32_t q_dtype,
                                            uintptr_t stream);
 
+/* ======================================================================
+ * Attention over selected cache blocks
+ * ==================================================================== */
+
+/* New (additive).  Long contexts: a query reads the bounds of its sequence's blocks,
+ * selects some by them, and attends those alone.  Works on the 16-bit and FP8 caches
+ * [num_blocks, num_kv_heads, head_dim, block_size] and tables of the other entry
+ * points, layer by layer, with one more array a layer:
+ *   k_bounds  [num_blocks, num_kv_heads, 2, head_dim] of the cache's type: the smallest
+ *             (0) and the largest (1) key of each channel over the rows of the block
+ *             that hold keys.  A block is num_kv_heads * 2 * head_dim elements in one
+ *             run, so rllm_cache_copy_blocks, rllm_cache_swap_out / _in and
+ *             rllm_cache_block_copy move bounds with the blocks they belong to.
+ * Rows: query_start_loc NULL: one a sequence, its last token (num_rows = num_seqs; a
+ * decode step).  Else as for the prefill entry points: sequence s has rows
+ * query_start_loc[s] .. [s + 1] - 1, its last tokens in order; row i of n sees keys
+ * 0 .. seq_len - n + i.  Rows that no sequence has are left as they were, in every
+ * output; the entries must not fall or pass num_rows.
+ * Shapes: head_dim a multiple of 32 up to 256, block_size 16, 32, 64 or 128, at most
+ * 1024 heads, block_size * max_num_blocks_per_seq below 2^31, all arrays of elements 16-byte
+ * aligned; anything else returns hipErrorInvalidValue.  dtype / q_dtype is
+ * RLLM_DTYPE_F16 or RLLM_DTYPE_BF16, kv_dtype the same or an FP8 one.  Table entries
+ * outside [0, num_blocks) are unused: nothing is written for them, they are in
+ * no list, and lists that name them attend nothing there. */
+
+/* Bounds of the blocks that sequences' keys 0 .. seq_lens[s] - 1 reach, from a cache that
+ * other entry points filled.  first_positions (may be NULL): blocks that end
+ * at or before first_positions[s] keep the bounds they have. */
+int32_t rllm_key_bounds(void *k_bounds, const void *key_cache, const int32_t *block_tables,
+                        const int32_t *seq_lens, const int32_t *first_positions, int64_t num_seqs,
+                        int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                        int64_t max_num_blocks_per_seq, int64_t num_blocks, int32_t kv_dtype,
+                        uintptr_t stream);
+
+/* Appends new tokens: q and k rotated by halves at their positions (f32, each product
+ * and the sum rounded; q_out, which may be q, rounded to dtype once, the key to the
+ * cache's type once), the rotated key and the value written at the places the
+ * table gives, and the bounds of the blocks written brought up to date.  Row i of n
+ * new tokens has position seq_len - n + i; seq_lens count the new tokens.  A block whose
+ * first row is written starts its bounds anew; another goes on from those it has, which must
+ * be its earlier rows'.  Rows at a negative position (padding: seq_len 0) or
+ * past the table are not written; their q is rotated at position 0, or as the
+ * position says, clamped to max_position - 1 as every rotation is.  A block that new
+ * tokens reach must belong to one sequence alone.  num_q_heads 0: no q.
+ * cos / sin as rllm_rope_tables fills them; FP8 as rllm_cache_write_fp8_ex.
+ * (rllm_rope_cache_write rounds every step to dtype; results differ by rounding.) */
+int32_t rllm_rope_cache_append(void *q_out, const void *q, const void *k, const void *v,
+                               void *key_cache, void *value_cache, void *k_bounds,
+                               const int32_t *block_tables, const int32_t *seq_lens,
+                               const int32_t *query_start_loc, const float *cos_cache,
+                               const float *sin_cache, int64_t num_seqs, int64_t num_tokens,
+                               int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t block_size, int64_t max_num_blocks_per_seq, int64_t num_blocks,
+                               int64_t max_position, int32_t dtype, int32_t kv_dtype, float k_scale,
+                               float v_scale, int32_t fp8_rounding, uintptr_t stream);
+
+/* Selects blocks: selected int32 [num_rows, num_kv_heads, num_selected] gets the
+ * numbers, within the sequence (0 = the block of positions 0 .. block_size - 1), of the
+ * blocks that each row and kv head attends, rising, then -1.  Of the nv blocks that the
+ * row sees: all where nv <= num_selected; else the first num_first, the last num_last
+ * (at least 1: the row's own), and for the places left those of the largest
+ *   max over the group's q heads of sum_d max(q_d * bounds[0]_d, q_d * bounds[1]_d),
+ * an upper bound of q . k over the block's keys; of equal ones the lowest.  The lists
+ * are those of the scores in 64 bits.  A score that is NaN ranks above all.
+ * FP8 bounds need no scale (a positive factor keeps the order).
+ * workspace: rllm_select_blocks_workspace_size(...) bytes, 16-byte aligned, of any
+ * content; one sized for a number of rows and a table width serves every call of as many
+ * kv heads with no more rows and no wider table.  Calls that share it must not overlap in
+ * time.  NULL: a library-owned buffer per (device, stream); a call that would have to grow
+ * it while the stream is being captured returns hipErrorStreamCaptureUnsupported,
+ * and graphs captured on one stream share it. */
+#define RLLM_SELECT_MAX_BLOCKS 4096   /* most blocks of a list */
+int32_t rllm_select_blocks(int32_t *selected, const void *query, const void *k_bounds,
+                           const int32_t *block_tables, const int32_t *seq_lens,
+                           const int32_t *query_start_loc, int64_t num_seqs, int64_t num_rows,
+                           int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                           int64_t block_size, int64_t max_num_blocks_per_seq, int64_t num_blocks,
+                           int64_t num_selected, int64_t num_first, int64_t num_last, int32_t q_dtype,
+                           int32_t kv_dtype, void *workspace, int64_t workspace_bytes,
+                           uintptr_t stream);
+int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads,
+                                          int64_t max_num_blocks_per_seq);
+
+/* Attention of each row over the keys it sees in its listed blocks (selected as
+ * above; any list whose entries rise and end in -1s will do: an entry that is
+ * negative, not above the one before it, or past what the row sees attends nothing).  Rows with
+ * nothing to attend get zeros.  scale, k_scale and v_scale as rllm_paged_attention_decode_ex.
+ * Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
+ * and keys past the row are not looked at; a key or value that is attended and not finite makes the
+ * outputs it reaches not finite. */
+int32_t rllm_paged_attention_sparse(void *output, const void *query, const void *key_cache,
+                                    const void *value_cache, const int32_t *block_tables,
+                                    const int32_t *seq_lens, const int32_t *query_start_loc,
+                                    const int32_t *selected, int64_t num_seqs, int64_t num_rows,
+                                    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                    int64_t block_size, int64_t max_num_blocks_per_seq,
+                                    int64_t num_blocks, int64_t num_selected, float scale,
+                                    int32_t q_dtype, int32_t kv_dtype, float k_scale, float v_scale,
+                                    uintptr_t stream);
+
 /* Replace rllm_vector_add_f32(_sync) and rllm_block_copy(_sync),
  * smoke.cu:21-66; bound at cuda.rs:17-35.  out = a + b (f32); nbytes
  * contiguous bytes src -> dst. */

@@ -96,6 +96,14 @@ SIGNATURES = {
     "rllm_paged_attention_decode_mxfp4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64],
     "rllm_paged_attention_prefill_mxfp4": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                            _F, _I32, _U],
+    "rllm_key_bounds": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _U],
+    "rllm_rope_cache_append": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+                               _I64, _I64, _I64, _I32, _I32, _F, _F, _I32, _U],
+    "rllm_select_blocks": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                           _I32, _I32, _P, _I64, _U],
+    "rllm_select_blocks_workspace_size": [_I64, _I64, _I64],
+    "rllm_paged_attention_sparse": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                    _I64, _F, _I32, _I32, _F, _F, _U],
     "rllm_vector_add_f32": [_P, _P, _P, _I64, _U],
     "rllm_vector_add_f32_sync": [_P, _P, _P, _I64],
     "rllm_block_copy": [_P, _P, _I64, _U],
@@ -112,7 +120,7 @@ SIGNATURES = {
     "rllm_gpu_free_host": [_P],
 }
 _RESTYPE = {"rllm_paged_attention_decode_workspace_size": _I64, "rllm_mxfp4_page_bytes": _I64,
-            "rllm_paged_attention_decode_mxfp4_workspace_size": _I64}
+            "rllm_paged_attention_decode_mxfp4_workspace_size": _I64, "rllm_select_blocks_workspace_size": _I64}
 
 
 def lib() -> ctypes.CDLL:

@@ -1,0 +1,66 @@
+// Shared pieces of the operators over selected cache blocks (sparse_bounds.hip,
+// sparse_select.hip, sparse_attention.hip): shape rules, where a query row stands
+// in its sequence, and the order of stored elements.
+//
+// The bounds of a block are the smallest and the largest key of each channel over
+// the block's rows that hold keys, k_bounds [num_blocks, num_kv_heads, 2, head_dim]
+// in the cache's own element type (a minimum of stored keys is a stored key, so
+// nothing is rounded).
+#pragma once
+
+#include "common.h"
+#include "../../include/rllm_kernels.h"
+
+#include <cmath>
+
+namespace rllm {
+
+// shapes every operator here takes
+static inline bool sparse_shape(int64_t hkv, int64_t d, int64_t bs) {
+    return hkv > 0 && hkv <= 1024 && d > 0 && d <= 256 && d % 32 == 0 && (bs == 16 || bs == 32 || bs == 64 || bs == 128);
+}
+static inline bool sparse_heads(int64_t hq, int64_t hkv) { return hq > 0 && hq <= 1024 && hq % hkv == 0; }
+static inline bool sparse_types(int32_t q_dtype, int32_t kv_dtype) {
+    return (q_dtype == RLLM_DTYPE_F16 || q_dtype == RLLM_DTYPE_BF16) &&
+           (kv_dtype == q_dtype || kv_dtype == RLLM_DTYPE_FP8_E4M3 || kv_dtype == RLLM_DTYPE_FP8_E5M2);
+}
+static inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+constexpr int64_t SPARSE_MAX_ROWS = int64_t(1) << 24;    // rows of a call, and sequences
+static inline bool sparse_table(int64_t maxb, int64_t bs) { return maxb >= 0 && maxb <= INT32_MAX / bs; }   // positions are 32-bit
+
+namespace {
+
+template <int KIND> constexpr bool sparse_is_fp8() { return KIND == KIND_FP8_E4M3 || KIND == KIND_FP8_E5M2; }
+
+// A query row (or new token): its sequence, the place among the sequence's rows
+// of the call, their number, and the row's position; seq -1 for a row that no
+// sequence has.
+struct SparseRow {
+    int32_t seq, i, n, pos;
+};
+__device__ __forceinline__ SparseRow sparse_row(int32_t t, const int32_t* qsl, const int32_t* seq_lens, int32_t num_seqs) {
+    if (!qsl) return {t, 0, 1, seq_lens[t] - 1};
+    int32_t lo = 0, hi = num_seqs;       // the first sequence that ends past t
+    while (lo < hi) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (qsl[mid + 1] <= t) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo >= num_seqs) return {-1, 0, 0, -1};
+    const int32_t q0 = qsl[lo], n = qsl[lo + 1] - q0;
+    if (t < q0) return {-1, 0, 0, -1};
+    return {lo, t - q0, n, seq_lens[lo] - n + (t - q0)};
+}
+
+// Stored elements as 16-bit integers that rise with the value (an FP8 byte in the
+// upper half): the sign's magnitude is turned round.  Its own inverse.  A positive
+// NaN lies above +inf, a negative one below -inf, so one of the two bounds keeps it.
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ i16x2 ordered2(uint32_t w) {
+    const i16x2 x = __builtin_bit_cast(i16x2, w);
+    return x ^ ((x >> 15) & i16x2{0x7fff, 0x7fff});
+}
+__device__ __forceinline__ int16_t ordered1(int16_t x) { return static_cast<int16_t>(x ^ ((x >> 15) & 0x7fff)); }
+
+}  // namespace
+}  // namespace rllm

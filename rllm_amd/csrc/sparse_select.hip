@@ -1,0 +1,545 @@
+// Selection of the cache blocks that a query attends, for gfx950.
+//
+//   score(b) = max over the heads of the group of sum_d max(q_d lo_bd, q_d hi_bd)
+//
+// is an upper bound of q . k over the keys of block b.  With q- = min(q, 0) and q+ =
+// max(q, 0) the sum is q- . lo + q+ . hi, a matrix product over 2 head_dim whose
+// right side lies in memory as it is needed.
+//
+// The lists are those of the scores in 64 bits.  The matrix cores give each score in
+// f32 (products of 16-bit values are exact there, sums are not) and a bound E of
+// its error; with T the K-th largest f32 score, every block above T + 2E is in, every
+// one below T - 2E is out, and only those between are scored again in f64.  Equal
+// ones go to the lowest block.
+#include "sparse_blocks.h"
+#include "generic_mfma.h"
+#include "workspace.h"
+
+namespace rllm {
+namespace {
+
+struct SelectArgs {
+    int32_t* sel;
+    const uint16_t* q;
+    const void* kb;
+    const int32_t *bt, *seq_lens, *qsl;
+    uint32_t* keys;     // [rows of the launch, hkv, pitch]: scores in their order, 0 = not to be chosen
+    uint8_t* state;     // the same, where they do not fit in LDS
+    float* kmax;        // [rows of the launch, hkv, chunks]: largest |bound| of a chunk
+    int32_t num_seqs, row0, rows, hq, hkv, d, bs_log2, maxb, k, first, last, chunk, chunks;
+    int64_t num_blocks, pitch;
+};
+
+// blocks of its sequence that a row sees
+__device__ __forceinline__ int visible_blocks(const SelectArgs& a, const SparseRow& r) {
+    return r.pos < 0 ? 0 : min((r.pos >> a.bs_log2) + 1, a.maxb);
+}
+
+// f32 as integers in the order of its values, never 0; NaN above all
+__device__ __forceinline__ uint32_t order32(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unorder32(uint32_t k) {
+    return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t order64(double x) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x + 0.0));   // -0 is 0
+    return x != x ? ~uint64_t(0) : u >> 63 ? ~u : u | (uint64_t(1) << 63);
+}
+
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
+
+// A workgroup per (row, kv head, chunk of its blocks), a wave 16 blocks at a time:
+// v_mfma_16x16x32, rows = heads, columns = blocks, k = channels of lo, then of hi.
+// Each lane loads 8 channels of its column's block, the operand as it stands.
+// Bound by HBM: the bounds are read once a row.
+template <int QKIND, int KVKIND, int NK>
+__global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
+    using M = GenMfma<QKIND>;
+    using raw_t = GenRaw<KVKIND>;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    constexpr int ES = gen_is_fp8<KVKIND>() ? 1 : 2, D = 32 * NK;
+    __shared__ uint32_t s_max[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, kq = lane >> 4;
+    const int unit = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int h = unit % a.hkv, t = a.row0 + unit / a.hkv;
+    const SparseRow row = sparse_row(t, a.qsl, a.seq_lens, a.num_seqs);
+    const int nv = visible_blocks(a, row);
+    if (row.seq < 0 || nv <= a.k) return;
+    const int c0 = max(chunk * a.chunk, a.first), c1 = min((chunk + 1) * a.chunk, nv - a.last);
+    if (c0 >= c1) return;
+    const int G = a.hq / a.hkv, hgs = (G + 15) / 16;
+    uint32_t top = 0;                                   // largest magnitudes, two 16-bit halves
+    const int32_t* const bt = a.bt + static_cast<int64_t>(row.seq) * a.maxb;
+    uint32_t* const keys = a.keys + unit * a.pitch;
+    uint4 qn[NK], qp[NK];
+    auto load_q = [&](int hg) __attribute__((always_inline)) {
+        const bool live = 16 * hg + col < G;
+        const uint16_t* src = a.q + (static_cast<int64_t>(t) * a.hq + h * G + 16 * hg + col) * D;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const uint4 x = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * kq) : make_uint4(0, 0, 0, 0);
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+            uint32_t n[4], p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t neg = (u[j] >> 15 & 0x00010001u) * 0xffffu;
+                n[j] = u[j] & neg;
+                p[j] = u[j] & ~neg;
+            }
+            qn[i] = make_uint4(n[0], n[1], n[2], n[3]);
+            qp[i] = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+    };
+    load_q(0);
+    for (int b0 = chunk * a.chunk + 16 * wave; b0 < c1; b0 += 64) {
+        const int j = b0 + col;
+        int32_t b = -1;
+        if (j >= c0 && j < c1) {
+            b = bt[j];
+            if (b >= a.num_blocks) b = -1;
+        }
+        const uint8_t* src = b >= 0 ? static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES)
+                                    : reinterpret_cast<const uint8_t*>(g_gen_zero);
+        const int st = b >= 0 ? ES : 0;
+        uint4 x[2 * NK];
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i)
+            x[i] = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(src + (32 * i + 8 * kq) * st));
+        u16x2 m = __builtin_bit_cast(u16x2, top);
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i) {
+            const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+        }
+        top = __builtin_bit_cast(uint32_t, m);
+        uint32_t best = 0;
+        for (int hg = 0; hg < hgs; ++hg) {
+            if (hgs > 1) load_q(hg);
+            gm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NK; ++i) acc = M::mma16(qn[i], x[i], acc);
+#pragma unroll
+            for (int i = 0; i < NK; ++i) acc = M::mma16(qp[i], x[NK + i], acc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (16 * hg + 4 * kq + i < G) best = umax(best, order32(acc[i]));
+        }
+        best = umax(best, __shfl_xor(best, 16));
+        best = umax(best, __shfl_xor(best, 32));
+        if (kq == 0 && j >= c0 && j < c1) keys[j] = b >= 0 ? best : 0;
+    }
+    uint32_t t16 = umax(top & 0xffffu, top >> 16);
+    for (int x = 1; x < 64; x <<= 1) t16 = umax(t16, __shfl_xor(t16, x));
+    if (lane == 0) s_max[wave] = t16;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
+        a.kmax[static_cast<int64_t>(unit) * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
+    }
+}
+
+enum : uint8_t { OUT = 0, MID = 1, IN = 2 };
+
+// sums over the workgroup; every thread calls
+struct Team {
+    uint32_t* s;          // [2][waves]
+    int waves, wave, turn;
+    __device__ __forceinline__ int sum(int wave_value) {
+        if (waves == 1) return wave_value;
+        uint32_t* const b = s + (turn ^= 1) * waves;
+        if ((threadIdx.x & 63) == 0) b[wave] = wave_value;
+        __syncthreads();
+        int n = 0;
+        for (int w = 0; w < waves; ++w) n += b[w];
+        return n;
+    }
+    // the sum, and that of the waves before this one
+    __device__ __forceinline__ int scan(int wave_value, int& before) {
+        before = 0;
+        if (waves == 1) return wave_value;
+        uint32_t* const b = s + (turn ^= 1) * waves;
+        if ((threadIdx.x & 63) == 0) b[wave] = wave_value;
+        __syncthreads();
+        int n = 0;
+        for (int w = 0; w < waves; ++w) {
+            if (w == wave) before = n;
+            n += b[w];
+        }
+        return n;
+    }
+    __device__ __forceinline__ uint32_t max(uint32_t wave_value) {
+        if (waves == 1) return wave_value;
+        uint32_t* const b = s + (turn ^= 1) * waves;
+        if ((threadIdx.x & 63) == 0) b[wave] = wave_value;
+        __syncthreads();
+        uint32_t n = 0;
+        for (int w = 0; w < waves; ++w) n = umax(n, b[w]);
+        return n;
+    }
+};
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    for (int x = 1; x < 64; x <<= 1) v = umax(v, __shfl_xor(v, x));
+    return v;
+}
+__device__ __forceinline__ int wave_count(bool p) { return __popcll(__builtin_amdgcn_ballot_w64(p)); }
+
+// The K-th largest key among those in the middle (there are K of them at least), by
+// its bits from the top; the bits that all of them share are not searched.
+template <int NT>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* keys, const uint8_t* state, int n, int K, Team& team) {
+    uint32_t hi = 0, low = 0;
+    for (int i = threadIdx.x; i < n; i += NT)
+        if (state[i] == MID) {
+            hi = umax(hi, keys[i]);
+            low = umax(low, ~keys[i]);
+        }
+    hi = team.max(wave_umax(hi));
+    const uint32_t lo = ~team.max(wave_umax(low));
+    if (hi == lo) return hi;
+    const int b0 = 31 - __builtin_clz(hi ^ lo);
+    uint32_t p = b0 == 31 ? 0 : hi >> (b0 + 1) << (b0 + 1);
+    for (int b = b0; b >= 0; --b) {
+        const uint32_t test = p | 1u << b;
+        int c = 0;
+        for (int i0 = 0; i0 < n; i0 += NT) {
+            const int i = i0 + threadIdx.x;
+            c += wave_count(i < n && state[i] == MID && keys[i] >= test);
+        }
+        if (team.sum(c) >= K) p = test;
+    }
+    return p;
+}
+
+// Settles the middle by its keys: those above the K-th largest are in, those below
+// out, equal ones stay if there are more of them than places.  Returns the places left for them.
+template <int NT>
+__device__ __forceinline__ int settle(const uint32_t* keys, uint8_t* state, int n, int K, Team& team) {
+    const uint32_t th = kth_largest<NT>(keys, state, n, K, team);
+    int c = 0;
+    for (int i0 = 0; i0 < n; i0 += NT) {
+        const int i = i0 + threadIdx.x;
+        const bool mid = i < n && state[i] == MID;
+        const bool in = mid && keys[i] > th;
+        if (in) state[i] = IN;
+        else if (mid && keys[i] < th) state[i] = OUT;
+        c += wave_count(in);
+    }
+    return K - team.sum(c);
+}
+
+// score in 64 bits, the same in every lane of the wave
+template <int QKIND, int KVKIND>
+__device__ double exact_score(const SelectArgs& a, int t, int h, int64_t block) {
+    using tag = typename GenMfma<QKIND>::tag;
+    const int lane = threadIdx.x & 63, D = a.d, G = a.hq / a.hkv;
+    const int64_t at = (block * a.hkv + h) * 2 * D;
+    float lo[4], hi[4];
+    auto bound = [&](int64_t i) __attribute__((always_inline)) -> float {
+        if constexpr (gen_is_fp8<KVKIND>()) {
+            const uint32_t w = static_cast<const uint8_t*>(a.kb)[i];
+            const uint32_t x = KVKIND == KIND_FP8_E4M3 ? e4m3x2_to_bf16x2(w, false) : e5m2x2_to_bf16x2(w, false);
+            return bf16_lo(x);
+        } else {
+            return to_f32<tag>(static_cast<const uint16_t*>(a.kb)[i]);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        lo[i] = d < D ? bound(at + d) : 0.f;
+        hi[i] = d < D ? bound(at + D + d) : 0.f;
+    }
+    double best = -INFINITY;
+    bool nan = false;
+    for (int g = 0; g < G; ++g) {
+        const uint16_t* qrow = a.q + (static_cast<int64_t>(t) * a.hq + h * G + g) * D;
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = lane + 64 * i;
+            if (d >= D) continue;
+            const double q = to_f32<tag>(qrow[d]);
+            const double x = q * lo[i], y = q * hi[i];
+            s += x != x || y != y ? __builtin_nan("") : x > y ? x : y;
+        }
+        for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
+        nan |= s != s;
+        best = s > best ? s : best;
+    }
+    return nan ? __builtin_nan("") : best;
+}
+
+constexpr int SELECT_LDS = 8192;     // candidates whose keys and states fit in LDS
+
+// A workgroup per (row, kv head).
+template <int QKIND, int KVKIND, int NT>
+__global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
+    using tag = typename GenMfma<QKIND>::tag;
+    constexpr int NW = NT / 64;
+    __shared__ uint32_t s_keys[SELECT_LDS];
+    __shared__ uint8_t s_state[SELECT_LDS];
+    __shared__ uint32_t s_team[2 * NW];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x, h = unit % a.hkv, t = a.row0 + unit / a.hkv;
+    const SparseRow row = sparse_row(t, a.qsl, a.seq_lens, a.num_seqs);
+    if (row.seq < 0) return;
+    Team team = {s_team, NW, wave, 0};
+    const int nv = visible_blocks(a, row);
+    const int32_t* const bt = a.bt + static_cast<int64_t>(row.seq) * a.maxb;
+    int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
+    auto usable = [&](int j) __attribute__((always_inline)) {
+        const int32_t b = bt[j];
+        return b >= 0 && b < a.num_blocks;
+    };
+    const bool all = nv <= a.k;
+    const int base = a.first, n = all ? 0 : nv - a.last - a.first;     // candidates base .. base + n - 1
+
+    auto body = [&](uint32_t* keys, uint8_t* state) __attribute__((always_inline)) {
+        int K = 0, ties = 0;
+        if (!all) {
+            const uint32_t* const g = a.keys + unit * a.pitch + base;
+            int c = 0, f = 0;
+            for (int i0 = 0; i0 < a.first + a.last; i0 += NT) {
+                const int i = i0 + threadIdx.x;
+                f += wave_count(i < a.first + a.last && usable(i < a.first ? i : nv - a.last + (i - a.first)));
+            }
+            bool odd = false;
+            for (int i0 = 0; i0 < n; i0 += NT) {
+                const int i = i0 + threadIdx.x;
+                uint32_t key = 0;
+                if (i < n) {
+                    key = g[i];
+                    if (keys != g) keys[i] = key;
+                    state[i] = key ? MID : OUT;
+                }
+                const float x = unorder32(key);
+                odd |= key && !gen_finite(x);
+                c += wave_count(key != 0);
+            }
+            K = a.k - team.sum(f);
+            const int eligible = team.sum(c);
+            if (eligible <= K) {
+                ties = K;          // the whole middle goes in
+            } else if (K > 0) {
+                const bool any_odd = team.max(__builtin_amdgcn_ballot_w64(odd) != 0) != 0;
+                bool again = any_odd;
+                if (!any_odd) {
+                    // E = (2 D + 32) 2^-23 max_h |q_h|_1 max |bound|: every product once, every sum with a rounding
+                    // of its own that may be a whole last bit, and room for this bound's own roundings
+                    const int G = a.hq / a.hkv;
+                    float qs = 0.f;
+                    for (int r = wave; r < G; r += NW) {
+                        const uint16_t* qrow = a.q + (static_cast<int64_t>(t) * a.hq + h * G + r) * a.d;
+                        float s = 0.f;
+                        for (int d = lane; d < a.d; d += 64) s += __builtin_fabsf(to_f32<tag>(qrow[d]));
+                        qs = fmaxf(qs, wave_sum(s));
+                    }
+                    float km = 0.f;
+                    const int ch0 = base / a.chunk, ch1 = (base + n - 1) / a.chunk;
+                    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, a.kmax[static_cast<int64_t>(unit) * a.chunks + i]);
+                    qs = __uint_as_float(team.max(__float_as_uint(qs)));
+                    km = wave_max(km);
+                    const float eps = (2 * a.d + 32) * 0x1p-23f * qs * km + 0x1p-100f;
+                    const float th = unorder32(kth_largest<NT>(keys, state, n, K, team));
+                    const float over = th + 2.f * eps + __builtin_fabsf(th) * 0x1p-22f;
+                    const float under = th - 2.f * eps - __builtin_fabsf(th) * 0x1p-22f;
+                    again = !gen_finite(over) || !gen_finite(under);
+                    if (!again) {
+                        int in = 0, mid = 0;
+                        for (int i0 = 0; i0 < n; i0 += NT) {
+                            const int i = i0 + threadIdx.x;
+                            const bool was = i < n && state[i] == MID;
+                            const float x = was ? unorder32(keys[i]) : 0.f;
+                            const bool is_in = was && x > over, is_mid = was && x >= under && x <= over;
+                            if (was) state[i] = is_in ? IN : is_mid ? MID : OUT;
+                            in += wave_count(is_in);
+                            mid += wave_count(is_mid);
+                        }
+                        K -= team.sum(in);
+                        again = team.sum(mid) > K;
+                    }
+                }
+                ties = K;
+                if (again) {
+                    // the middle once more in 64 bits: upper half, and where that is equal the lower
+                    for (int half = 0; half < 2; ++half) {
+                        __syncthreads();
+                        int mid = 0;
+                        for (int i0 = 64 * wave; i0 < n; i0 += NT) {
+                            uint64_t m = __builtin_amdgcn_ballot_w64(i0 + lane < n && state[i0 + lane] == MID);
+                            mid += __popcll(m);
+                            for (; m; m &= m - 1) {
+                                const int i = i0 + __builtin_ctzll(m);
+                                const uint64_t key = order64(exact_score<QKIND, KVKIND>(a, t, h, bt[base + i]));
+                                if (lane == 0) keys[i] = static_cast<uint32_t>(half ? key : key >> 32);
+                            }
+                        }
+                        if (team.sum(mid) <= ties) break;
+                        __syncthreads();
+                        ties = settle<NT>(keys, state, n, ties, team);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        // the list, in the blocks' order; of the middle the first `ties`
+        int out = 0, mids = 0;
+        const int total = nv;
+        for (int j0 = 0; j0 < total && out < a.k; j0 += NT) {
+            const int j = j0 + threadIdx.x;
+            bool in = false, mid = false;
+            if (j < total) {
+                if (all || j < a.first || j >= nv - a.last) in = usable(j);
+                else {
+                    in = state[j - base] == IN;
+                    mid = state[j - base] == MID;
+                }
+            }
+            int before;
+            const uint64_t below = (uint64_t(1) << lane) - 1;
+            const uint64_t mm = __builtin_amdgcn_ballot_w64(mid);
+            const int found = team.scan(__popcll(mm), before);
+            in |= mid && mids + before + __popcll(mm & below) < ties;
+            mids += found;
+            const uint64_t mi = __builtin_amdgcn_ballot_w64(in);
+            const int taken = team.scan(__popcll(mi), before);
+            const int at = out + before + __popcll(mi & below);
+            if (in && at < a.k) sel[at] = j;
+            out += taken;
+        }
+        for (int i = out + threadIdx.x; i < a.k; i += NT) sel[i] = -1;
+    };
+    if (n <= SELECT_LDS) body(s_keys, s_state);
+    else body(a.keys + unit * a.pitch + base, a.state + unit * a.pitch + base);
+}
+
+template <int QKIND, int KVKIND>
+int32_t launch_select(const SelectArgs& a, hipStream_t st) {
+    const int64_t units = static_cast<int64_t>(a.rows) * a.hkv;
+    const dim3 grid(static_cast<unsigned>(units * a.chunks));
+    if (a.chunks > 0) {
+        switch (a.d / 32) {
+#define RLLM_SCORE(N) \
+    case N: hipLaunchKernelGGL((select_score_kernel<QKIND, KVKIND, N>), grid, dim3(256), 0, st, a); break;
+            RLLM_SCORE(1) RLLM_SCORE(2) RLLM_SCORE(3) RLLM_SCORE(4) RLLM_SCORE(5) RLLM_SCORE(6) RLLM_SCORE(7) RLLM_SCORE(8)
+#undef RLLM_SCORE
+        }
+        const int32_t rc = launch_status();
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
+    return launch_status();
+}
+
+constexpr int64_t SELECT_SLAB = int64_t(1) << 30;    // bytes of scratch of one pair of launches (a row's, where that is more)
+constexpr int64_t SELECT_CHUNK_MIN = 64, SELECT_CHUNK_MAX = 512;
+
+// bytes of scratch of a row: never fewer for a wider table
+int64_t select_row_bytes(int64_t hkv, int64_t maxb, int64_t& pitch) {
+    pitch = (maxb + SELECT_CHUNK_MAX - 1) / SELECT_CHUNK_MAX * SELECT_CHUNK_MAX;
+    return hkv * (pitch * 4 + pitch / SELECT_CHUNK_MIN * 4 + (maxb > SELECT_LDS ? pitch : 0));
+}
+int64_t select_bytes(int64_t num_rows, int64_t row_bytes) {
+    const int64_t slab = row_bytes > SELECT_SLAB ? row_bytes : SELECT_SLAB;
+    return num_rows * row_bytes < slab ? num_rows * row_bytes : slab;
+}
+
+}  // namespace
+}  // namespace rllm
+
+using namespace rllm;
+
+extern "C" {
+
+int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads, int64_t max_num_blocks_per_seq) {
+    if (num_rows < 0 || num_rows > SPARSE_MAX_ROWS || num_kv_heads < 1 || num_kv_heads > 1024 ||
+        !sparse_table(max_num_blocks_per_seq, 16))
+        return -1;
+    int64_t pitch;
+    return select_bytes(num_rows, select_row_bytes(num_kv_heads, max_num_blocks_per_seq, pitch));
+}
+
+int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_bounds, const int32_t* block_tables,
+                           const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs, int64_t num_rows,
+                           int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                           int64_t max_num_blocks_per_seq, int64_t num_blocks, int64_t num_selected, int64_t num_first,
+                           int64_t num_last, int32_t q_dtype, int32_t kv_dtype, void* workspace, int64_t workspace_bytes,
+                           uintptr_t stream) {
+    if (num_seqs <= 0 || num_rows <= 0) return 0;
+    RLLM_CHECK_ARG(sparse_shape(num_kv_heads, head_dim, block_size) && sparse_heads(num_q_heads, num_kv_heads));
+    RLLM_CHECK_ARG(sparse_types(q_dtype, kv_dtype));
+    RLLM_CHECK_ARG(num_seqs <= SPARSE_MAX_ROWS && num_rows <= SPARSE_MAX_ROWS && num_blocks >= 0);
+    RLLM_CHECK_ARG(sparse_table(max_num_blocks_per_seq, block_size));
+    RLLM_CHECK_ARG(query_start_loc || num_rows == num_seqs);
+    RLLM_CHECK_ARG(num_selected >= 1 && num_selected <= RLLM_SELECT_MAX_BLOCKS);
+    RLLM_CHECK_ARG(num_first >= 0 && num_last >= 1 && num_first <= num_selected && num_last <= num_selected - num_first);
+    RLLM_CHECK_ARG(selected && query && k_bounds && seq_lens && (block_tables || max_num_blocks_per_seq == 0));
+    RLLM_CHECK_ARG(aligned_to(query, 16) && aligned_to(k_bounds, 16));
+    int64_t pitch = 0, need = 0, slab = num_rows, chunk = SELECT_CHUNK_MIN, chunks = 0;
+    if (max_num_blocks_per_seq > num_selected) {       // else every list is the whole sequence
+        const int64_t row_bytes = select_row_bytes(num_kv_heads, max_num_blocks_per_seq, pitch);
+        need = select_bytes(num_rows, row_bytes);
+        slab = need / row_bytes;
+        // enough workgroups to fill the card, and not many more
+        while (chunk < SELECT_CHUNK_MAX && slab * num_kv_heads * ((max_num_blocks_per_seq + chunk - 1) / chunk) > 4096) chunk *= 2;
+        chunks = (max_num_blocks_per_seq + chunk - 1) / chunk;
+        if (slab > INT32_MAX / (num_kv_heads * chunks)) slab = INT32_MAX / (num_kv_heads * chunks);
+    }
+    WorkspaceHold hold;
+    void* ws = workspace;
+    if (workspace) {
+        RLLM_CHECK_ARG(workspace_bytes >= need && aligned_to(workspace, 16));
+    } else if (need > 0) {
+        const int32_t rc = g_workspaces.get(stream, WS_SELECT, need, false, &ws, &hold);
+        if (rc) return rc;
+        if (!ws) return static_cast<int32_t>(hipErrorStreamCaptureUnsupported);
+    }
+    SelectArgs a = {};
+    a.sel = selected;
+    a.q = static_cast<const uint16_t*>(query);
+    a.kb = k_bounds;
+    a.bt = block_tables;
+    a.seq_lens = seq_lens;
+    a.qsl = query_start_loc;
+    a.keys = static_cast<uint32_t*>(ws);
+    a.num_seqs = static_cast<int32_t>(num_seqs);
+    a.hq = static_cast<int32_t>(num_q_heads);
+    a.hkv = static_cast<int32_t>(num_kv_heads);
+    a.d = static_cast<int32_t>(head_dim);
+    a.bs_log2 = __builtin_ctz(static_cast<unsigned>(block_size));
+    a.maxb = static_cast<int32_t>(max_num_blocks_per_seq);
+    a.k = static_cast<int32_t>(num_selected);
+    a.first = static_cast<int32_t>(num_first);
+    a.last = static_cast<int32_t>(num_last);
+    a.chunk = static_cast<int32_t>(chunk);
+    a.chunks = static_cast<int32_t>(chunks);
+    a.num_blocks = num_blocks;
+    a.pitch = pitch;
+    const hipStream_t st = as_stream(stream);
+    for (int64_t r = 0; r < num_rows; r += slab) {
+        a.row0 = static_cast<int32_t>(r);
+        a.rows = static_cast<int32_t>(num_rows - r < slab ? num_rows - r : slab);
+        const int64_t units = slab * num_kv_heads;     // the scratch's layout is that of a whole slab
+        a.kmax = reinterpret_cast<float*>(a.keys + units * pitch);
+        a.state = reinterpret_cast<uint8_t*>(a.kmax + units * (pitch / SELECT_CHUNK_MIN));
+        int32_t rc;
+        if (q_dtype == RLLM_DTYPE_BF16)
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_BF16, KIND_FP8_E4M3>(a, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_BF16, KIND_FP8_E5M2>(a, st)
+                                                   : launch_select<KIND_BF16, KIND_BF16>(a, st);
+        else
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_F16, KIND_FP8_E4M3>(a, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_F16, KIND_FP8_E5M2>(a, st)
+                                                   : launch_select<KIND_F16, KIND_F16>(a, st);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -537,6 +537,202 @@ def paged_prefill_mxfp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     return out
 
 
+def new_key_bounds(k_cache: torch.Tensor) -> torch.Tensor:
+    """Zeroed key bounds [num_blocks, Hkv, 2, D] for a key cache [num_blocks, Hkv, D, bs], in its type."""
+    if k_cache.dim() != 4:
+        raise ValueError("a key cache [num_blocks, Hkv, D, bs] required")
+    nb, hkv, d, _ = k_cache.shape
+    return torch.zeros((nb, hkv, 2, d), dtype=k_cache.dtype, device=k_cache.device)
+
+
+def _check_rows(rows: int, block_tables, seq_lens, query_start_loc, device: int) -> int:
+    """Checks of what places rows in sequences; returns the number of sequences."""
+    if block_tables.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
+        raise TypeError("block_tables and seq_lens must be int32")
+    table = block_tables.shape
+    if len(table) != 2 or seq_lens.shape != table[:1]:
+        raise ValueError("block_tables [num_seqs, max_blocks] and seq_lens [num_seqs] required")
+    if query_start_loc is None:
+        if rows != table[0]:
+            raise ValueError("without query_start_loc there is one row a sequence")
+    elif query_start_loc.dtype is not torch.int32 or query_start_loc.shape != (table[0] + 1,) \
+            or query_start_loc.get_device() != device or not query_start_loc.is_contiguous():
+        raise ValueError("query_start_loc must be contiguous int32 [num_seqs + 1] on the device of the rows")
+    return table[0]
+
+
+def _validate_rows(rows: int, block_tables, seq_lens, query_start_loc, num_blocks: int, block_size: int) -> None:
+    validate_tables(block_tables, seq_lens, num_blocks, block_size)
+    if query_start_loc is not None:
+        qsl = query_start_loc.detach().cpu()
+        if int(qsl[0]) < 0 or int(qsl[-1]) > rows or bool((qsl[1:] < qsl[:-1]).any()):
+            raise ValueError("query_start_loc must rise, within the rows")
+
+
+def _sparse_shape(d: int, bs: int) -> None:
+    if d % 32 or not 0 < d <= 256 or bs not in (16, 32, 64, 128):
+        raise ValueError("head_dim must be a multiple of 32 up to 256, block_size 16, 32, 64 or 128")
+
+
+def _check_bounds(k_bounds: torch.Tensor, nb: int, hkv: int, d: int, dtype: torch.dtype) -> None:
+    if k_bounds.shape != (nb, hkv, 2, d) or k_bounds.dtype is not dtype:
+        raise ValueError("k_bounds must be [num_blocks, Hkv, 2, D] of the cache's type")
+
+
+def key_bounds(k_cache: torch.Tensor, k_bounds: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, *,
+               first_positions: Optional[torch.Tensor] = None, kv_dtype: Optional[int] = None, validate: bool = True,
+               stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Brings up to date the bounds of the blocks that the sequences' keys reach (of those that end
+    past first_positions, int32 [num_seqs], if given), through rllm_key_bounds; returns k_bounds."""
+    if k_cache.dim() != 4:
+        raise ValueError("a key cache [num_blocks, Hkv, D, bs] required")
+    nb, hkv, d, bs = k_cache.shape
+    kv = _kv_code(k_cache, kv_dtype)
+    _sparse_shape(d, bs)
+    _check_bounds(k_bounds, nb, hkv, d, k_cache.dtype)
+    b = _check_rows(seq_lens.shape[0], block_tables, seq_lens, None, k_cache.get_device())
+    _all_dense(k_cache, k_bounds, block_tables, seq_lens)
+    if first_positions is not None:
+        if first_positions.dtype is not torch.int32 or first_positions.shape != (b,):
+            raise ValueError("first_positions must be int32 [num_seqs]")
+        _all_dense(k_cache, first_positions)
+    if validate:
+        validate_tables(block_tables, seq_lens, nb, bs)
+    call("rllm_key_bounds", _ptr(k_bounds), _ptr(k_cache), _ptr(block_tables), _ptr(seq_lens), _ptr(first_positions),
+         b, hkv, d, bs, block_tables.shape[1], nb, kv, _stream(stream))
+    return k_bounds
+
+
+def rope_and_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, k_bounds: torch.Tensor, block_tables: torch.Tensor,
+                    seq_lens: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                    query_start_loc: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                    kv_dtype: Optional[int] = None, k_scale: float = 1.0, v_scale: float = 1.0,
+                    fp8_rounding: int = FP8_ROUND_TOWARD_ZERO, validate: bool = True,
+                    stream: Optional[torch.cuda.Stream] = None) -> Optional[torch.Tensor]:
+    """Rotates q and k by halves at their positions, writes the sequences' new keys and values where the block
+    tables say, and keeps the bounds of the blocks written, through rllm_rope_cache_append.  seq_lens count the
+    new tokens; without query_start_loc each sequence has one.  Returns the rotated q (``q_out``, which
+    may be ``q`` itself), or None when q is None."""
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4:
+        raise ValueError("k/v [num_tokens, Hkv, D] of one shape and caches [nb, Hkv, D, bs] required")
+    n, hkv, d = k.shape
+    nb, hkv2, d2, bs = k_cache.shape
+    if (hkv, d) != (hkv2, d2) or k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+        raise ValueError("token rows do not match the cache layout")
+    dt = _TORCH_16.get(k.dtype)
+    if dt is None or v.dtype is not k.dtype:
+        raise TypeError("k/v must be float16 or bfloat16")
+    kv = _kv_code(k_cache, kv_dtype)
+    if kv in (DTYPE_F16, DTYPE_BF16) and kv != dt:
+        raise TypeError("16-bit cache dtype must equal the input dtype")
+    _sparse_shape(d, bs)
+    _check_bounds(k_bounds, nb, hkv, d, k_cache.dtype)
+    b = _check_rows(n, block_tables, seq_lens, query_start_loc, k.get_device())
+    if cos.dtype is not torch.float32 or sin.shape != cos.shape or sin.dtype is not cos.dtype \
+            or cos.dim() != 2 or cos.shape[1] != d // 2:
+        raise ValueError("cos/sin must be float32 [max_position, head_dim // 2]")
+    hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype is not k.dtype:
+            raise ValueError("q must be [num_tokens, Hq, D] of the k dtype")
+        hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        elif q_out.shape != q.shape or q_out.dtype is not q.dtype:
+            raise ValueError("q_out must match q")
+        _all_dense(k, v, k_cache, v_cache, k_bounds, block_tables, seq_lens, cos, sin, q, q_out)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    else:
+        _all_dense(k, v, k_cache, v_cache, k_bounds, block_tables, seq_lens, cos, sin)
+    if validate:
+        _validate_rows(n, block_tables, seq_lens, query_start_loc, nb, bs)
+    call("rllm_rope_cache_append", _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_bounds),
+         _ptr(block_tables), _ptr(seq_lens), _ptr(query_start_loc), _ptr(cos), _ptr(sin), b, n, hq, hkv, d, bs,
+         block_tables.shape[1], nb, cos.shape[0], dt, kv, k_scale, v_scale, fp8_rounding, _stream(stream))
+    return q_out
+
+
+def select_blocks(q: torch.Tensor, k_bounds: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                  block_size: int, num_selected: int, *, num_first: int = 1, num_last: int = 1,
+                  query_start_loc: Optional[torch.Tensor] = None, kv_dtype: Optional[int] = None,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                  validate: bool = True, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """The blocks that each query row and kv head attends, int32 [num_rows, Hkv, num_selected] (rising,
+    then -1): the first num_first, the last num_last and those of the largest upper bound of q . k, through
+    rllm_select_blocks.  Without query_start_loc each sequence has one row, its last token."""
+    if q.dim() != 3 or k_bounds.dim() != 4:
+        raise ValueError("q [*, Hq, D] and k_bounds [nb, Hkv, 2, D] required")
+    rows, hq, d = q.shape
+    nb, hkv = k_bounds.shape[:2]
+    dt = _TORCH_16.get(q.dtype)
+    if dt is None:
+        raise TypeError("q must be float16 or bfloat16")
+    kv = _kv_code(k_bounds, kv_dtype)
+    if kv in (DTYPE_F16, DTYPE_BF16) and kv != dt:
+        raise TypeError("16-bit bounds must have the dtype of q")
+    _sparse_shape(d, block_size)
+    _check_bounds(k_bounds, nb, hkv, d, k_bounds.dtype)
+    b = _check_rows(rows, block_tables, seq_lens, query_start_loc, q.get_device())
+    if out is None:
+        out = torch.empty((rows, hkv, num_selected), dtype=torch.int32, device=q.device)
+        _all_dense(q, k_bounds, block_tables, seq_lens)
+    elif out.shape != (rows, hkv, num_selected) or out.dtype is not torch.int32:
+        raise ValueError("out must be int32 [num_rows, Hkv, num_selected]")
+    else:
+        _all_dense(q, k_bounds, block_tables, seq_lens, out)
+    ws_bytes = 0
+    if workspace is not None:
+        _all_dense(q, workspace)
+        ws_bytes = workspace.numel() * workspace.element_size()
+    if validate:
+        _validate_rows(rows, block_tables, seq_lens, query_start_loc, nb, block_size)
+    call("rllm_select_blocks", _ptr(out), _ptr(q), _ptr(k_bounds), _ptr(block_tables), _ptr(seq_lens),
+         _ptr(query_start_loc), b, rows, hq, hkv, d, block_size, block_tables.shape[1], nb, num_selected, num_first,
+         num_last, dt, kv, _ptr(workspace), ws_bytes, _stream(stream))
+    return out
+
+
+def paged_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                 seq_lens: torch.Tensor, selected: torch.Tensor, scale: float, *,
+                 query_start_loc: Optional[torch.Tensor] = None, kv_dtype: Optional[int] = None, k_scale: float = 1.0,
+                 v_scale: float = 1.0, out: Optional[torch.Tensor] = None, validate: bool = True,
+                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Attention of each query row over the keys it sees in the blocks that selected [num_rows, Hkv, n]
+    lists for it (as select_blocks returns them), through rllm_paged_attention_sparse."""
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("q [*, Hq, D] and caches [nb, Hkv, D, bs] of equal shape and type required")
+    rows, hq, d = q.shape
+    nb, hkv, d2, bs = k_cache.shape
+    dt = _TORCH_16.get(q.dtype)
+    if dt is None:
+        raise TypeError("q must be float16 or bfloat16")
+    if d != d2:
+        raise ValueError("head_dim of q and caches differ")
+    kv = _kv_code(k_cache, kv_dtype)
+    if kv in (DTYPE_F16, DTYPE_BF16) and kv != dt:
+        raise TypeError("a 16-bit cache must have the dtype of q")
+    _sparse_shape(d, bs)
+    b = _check_rows(rows, block_tables, seq_lens, query_start_loc, q.get_device())
+    if selected.dtype is not torch.int32 or selected.dim() != 3 or selected.shape[:2] != (rows, hkv):
+        raise ValueError("selected must be int32 [num_rows, Hkv, n]")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype is not q.dtype:
+        raise ValueError("out must be a contiguous tensor like q")
+    _all_dense(q, k_cache, v_cache, block_tables, seq_lens, selected, out)
+    if validate:
+        _validate_rows(rows, block_tables, seq_lens, query_start_loc, nb, bs)
+        s = selected.detach().cpu()
+        if bool(((s[..., 1:] >= 0) & (s[..., 1:] <= s[..., :-1])).any()):
+            raise ValueError("the blocks of a list must rise")
+    call("rllm_paged_attention_sparse", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+         _ptr(seq_lens), _ptr(query_start_loc), _ptr(selected), b, rows, hq, hkv, d, bs, block_tables.shape[1], nb,
+         selected.shape[2], scale, dt, kv, k_scale, v_scale, _stream(stream))
+    return out
+
+
 def layer_table(caches, device) -> torch.Tensor:
     """DEVICE uint64 array of the per-layer cache base addresses, the form
     rllm_cache_copy_blocks / rllm_cache_swap_{out,in} take.  Build it once per
