@@ -724,8 +724,8 @@ int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads
                                           int64_t max_num_blocks_per_seq);
 
 /* Attention of each row over the keys it sees in its listed blocks (selected as
- * above; any list whose entries rise and end in -1s will do: an entry that is
- * negative, not above the one before it, or past what the row sees attends nothing).  Rows with
+ * above, or any other lists: one ends at its first entry that is negative or not above the
+ * one before it, and an entry past what the row sees attends nothing).  Rows with
  * nothing to attend get zeros.  scale, k_scale and v_scale as rllm_paged_attention_decode_ex.
  * Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
  * and keys past the row are not looked at; a key or value that is attended and not finite makes the

@@ -52,6 +52,33 @@ __device__ __forceinline__ SparseRow sparse_row(int32_t t, const int32_t* qsl, c
     return {lo, t - q0, n, seq_lens[lo] - n + (t - q0)};
 }
 
+struct SparseTile {
+    int32_t seq, row, i, n;
+};
+// Tile x of the sequences' rows, each sequence's cut into tiles of its own: its sequence
+// (-1: there are fewer), first row, place among the sequence's rows, and their number.
+__device__ __forceinline__ SparseTile sparse_tile(int x, int tile, const int32_t* qsl, int num_seqs) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < num_seqs; s0 += 64) {
+        const int s = s0 + lane;
+        const int q0 = s < num_seqs ? qsl[s] : 0, n = s < num_seqs ? max(qsl[s + 1] - q0, 0) : 0;
+        const int tiles = (n + tile - 1) / tile;
+        int sum = tiles;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(sum, d);
+            if (lane >= d) sum += y;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(sum > x);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const int i = (x - __builtin_amdgcn_readlane(sum - tiles, l)) * tile;
+            return {s0 + l, __builtin_amdgcn_readlane(q0, l) + i, i, __builtin_amdgcn_readlane(n, l)};
+        }
+        x -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return {-1, 0, 0, 0};
+}
+
 // Stored elements as 16-bit integers that rise with the value (an FP8 byte in the
 // upper half): the sign's magnitude is turned round.  Its own inverse.  A positive
 // NaN lies above +inf, a negative one below -inf, so one of the two bounds keeps it.

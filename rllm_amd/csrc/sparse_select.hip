@@ -27,6 +27,7 @@ struct SelectArgs {
     uint8_t* state;     // the same, where they do not fit in LDS
     float* kmax;        // [rows of the launch, hkv, chunks]: largest |bound| of a chunk
     int32_t num_seqs, row0, rows, hq, hkv, d, bs_log2, maxb, k, first, last, chunk, chunks;
+    int32_t group_log2; // heads of a group, as a power of two, where rows go in tiles
     int64_t num_blocks, pitch;
 };
 
@@ -37,7 +38,7 @@ __device__ __forceinline__ int visible_blocks(const SelectArgs& a, const SparseR
 
 // f32 as integers in the order of its values, never 0; NaN above all
 __device__ __forceinline__ uint32_t order32(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(x + 0.0f);            // -0 is 0
     return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unorder32(uint32_t k) {
@@ -50,6 +51,21 @@ __device__ __forceinline__ uint64_t order64(double x) {
 
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
+
+// q- and q+ of 8 elements (NaN in one of them)
+__device__ __forceinline__ void split_signs(const uint4& x, uint4& neg, uint4& pos) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    uint32_t n[4], p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t m = (u[j] >> 15 & 0x00010001u) * 0xffffu;
+        n[j] = u[j] & m;
+        p[j] = u[j] & ~m;
+    }
+    neg = make_uint4(n[0], n[1], n[2], n[3]);
+    pos = make_uint4(p[0], p[1], p[2], p[3]);
+}
+constexpr int select_m_tiles(int d) { return d > 128 ? 2 : 4; }   // 16-row tiles of a chunk's workgroup
 
 // A workgroup per (row, kv head, chunk of its blocks), a wave 16 blocks at a time:
 // v_mfma_16x16x32, rows = heads, columns = blocks, k = channels of lo, then of hi.
@@ -82,16 +98,7 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             const uint4 x = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * kq) : make_uint4(0, 0, 0, 0);
-            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-            uint32_t n[4], p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t neg = (u[j] >> 15 & 0x00010001u) * 0xffffu;
-                n[j] = u[j] & neg;
-                p[j] = u[j] & ~neg;
-            }
-            qn[i] = make_uint4(n[0], n[1], n[2], n[3]);
-            qp[i] = make_uint4(p[0], p[1], p[2], p[3]);
+            split_signs(x, qn[i], qp[i]);
         }
     };
     load_q(0);
@@ -141,6 +148,110 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
         t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
         a.kmax[static_cast<int64_t>(unit) * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
     }
+}
+
+// Rows of a chunk: a tile of them, 64 (row, head) pairs (32 past head_dim 128) of one
+// sequence and kv head, holds its queries in registers and takes the blocks as above;
+// a block's bounds serve every row of the tile.
+template <int QKIND, int KVKIND, int NK>
+__global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a) {
+    using M = GenMfma<QKIND>;
+    using raw_t = GenRaw<KVKIND>;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    constexpr int ES = gen_is_fp8<KVKIND>() ? 1 : 2, D = 32 * NK, MT = select_m_tiles(D);
+    __shared__ uint32_t s_max[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, kq = lane >> 4;
+    const int h = blockIdx.x % a.hkv, chunk = blockIdx.x / a.hkv % a.chunks;
+    const int G = a.hq / a.hkv, gl = a.group_log2, tile = 16 * MT >> gl;
+    const SparseTile x = sparse_tile(blockIdx.x / a.hkv / a.chunks, tile, a.qsl, a.num_seqs);
+    if (x.seq < 0 || x.row < 0) return;
+    const int nt = min(min(tile, x.n - x.i), a.row0 + a.rows - x.row);        // rows of the tile within the launch
+    if (nt <= 0 || x.row + nt <= a.row0) return;
+    const int pos = a.seq_lens[x.seq] - x.n + x.i;
+    const SparseRow last = {x.seq, 0, 0, pos + nt - 1};
+    const int nv = visible_blocks(a, last);
+    if (nv <= a.k) return;
+    const int c0 = max(chunk * a.chunk, a.first), c1 = min((chunk + 1) * a.chunk, nv - a.last);
+    if (c0 >= c1) return;
+    const int32_t* const bt = a.bt + static_cast<int64_t>(x.seq) * a.maxb;
+    uint4 qn[MT][NK], qp[MT][NK];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int r = 16 * m + col, tok = r >> gl, g = r & ((1 << gl) - 1);
+        const bool live = tok < nt && g < G;
+        const uint16_t* src = a.q + (static_cast<int64_t>(x.row + tok) * a.hq + h * G + g) * D;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const uint4 y = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * kq) : make_uint4(0, 0, 0, 0);
+            split_signs(y, qn[m][i], qp[m][i]);
+        }
+    }
+    u16x2 top = {0, 0};
+    for (int b0 = chunk * a.chunk + 16 * wave; b0 < c1; b0 += 64) {
+        const int j = b0 + col;
+        int32_t b = -1;
+        if (j >= c0 && j < c1) {
+            b = bt[j];
+            if (b >= a.num_blocks) b = -1;
+        }
+        const uint8_t* src = b >= 0 ? static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES)
+                                    : reinterpret_cast<const uint8_t*>(g_gen_zero);
+        const int st = b >= 0 ? ES : 0;
+        uint4 y[2 * NK];
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i)
+            y[i] = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(src + (32 * i + 8 * kq) * st));
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i) {
+            const uint32_t u[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+        }
+        gm_f32x4 acc[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m] = M::mma16(qn[m][i], y[i], acc[m]);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m] = M::mma16(qp[m][i], y[NK + i], acc[m]);
+        const bool in = j >= c0 && j < c1;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            uint32_t key[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) key[i] = ((4 * kq + i) & ((1 << gl) - 1)) < G ? order32(acc[m][i]) : 0;
+            // rows 4 kq + i of the tile's m-th 16: the heads of a row one after the other
+            auto put = [&](int tok, uint32_t k) __attribute__((always_inline)) {
+                const int t = x.row + tok;
+                if (in && tok < nt && t >= a.row0) a.keys[(static_cast<int64_t>(t - a.row0) * a.hkv + h) * a.pitch + j] = b >= 0 ? k : 0;
+            };
+            if (gl == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put(16 * m + 4 * kq + i, key[i]);
+            } else if (gl == 1) {
+                put(8 * m + 2 * kq, umax(key[0], key[1]));
+                put(8 * m + 2 * kq + 1, umax(key[2], key[3]));
+            } else {
+                uint32_t k = umax(umax(key[0], key[1]), umax(key[2], key[3]));
+                if (gl >= 3) k = umax(k, __shfl_xor(k, 16));
+                if (gl >= 4) k = umax(k, __shfl_xor(k, 32));
+                if ((kq & ((1 << (gl - 2)) - 1)) == 0) put((16 * m + 4 * kq) >> gl, k);
+            }
+        }
+    }
+    uint32_t t16 = umax(top[0], top[1]);
+    for (int d = 1; d < 64; d <<= 1) t16 = umax(t16, __shfl_xor(t16, d));
+    if (lane == 0) s_max[wave] = t16;
+    __syncthreads();
+    t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
+    const int t = x.row + static_cast<int>(threadIdx.x);
+    if (static_cast<int>(threadIdx.x) < nt && t >= a.row0)
+        a.kmax[(static_cast<int64_t>(t - a.row0) * a.hkv + h) * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
 }
 
 enum : uint8_t { OUT = 0, MID = 1, IN = 2 };
@@ -274,36 +385,68 @@ __device__ double exact_score(const SelectArgs& a, int t, int h, int64_t block) 
     return nan ? __builtin_nan("") : best;
 }
 
-constexpr int SELECT_LDS = 8192;     // candidates whose keys and states fit in LDS
-
-// A workgroup per (row, kv head).
-template <int QKIND, int KVKIND, int NT>
-__global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
-    using tag = typename GenMfma<QKIND>::tag;
-    constexpr int NW = NT / 64;
-    __shared__ uint32_t s_keys[SELECT_LDS];
-    __shared__ uint8_t s_state[SELECT_LDS];
-    __shared__ uint32_t s_team[2 * NW];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int unit = blockIdx.x, h = unit % a.hkv, t = a.row0 + unit / a.hkv;
-    const SparseRow row = sparse_row(t, a.qsl, a.seq_lens, a.num_seqs);
-    if (row.seq < 0) return;
-    Team team = {s_team, NW, wave, 0};
-    const int nv = visible_blocks(a, row);
-    const int32_t* const bt = a.bt + static_cast<int64_t>(row.seq) * a.maxb;
-    int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
-    auto usable = [&](int j) __attribute__((always_inline)) {
+// What the lists of a row and kv head are made from.
+struct Pick {
+    const SelectArgs& a;
+    const int32_t* bt;
+    int32_t* sel;
+    int unit, h, t, nv;
+    int base, n;            // candidates: blocks base .. base + n - 1
+    __device__ __forceinline__ bool usable(int j) const {
         const int32_t b = bt[j];
         return b >= 0 && b < a.num_blocks;
-    };
-    const bool all = nv <= a.k;
-    const int base = a.first, n = all ? 0 : nv - a.last - a.first;     // candidates base .. base + n - 1
+    }
+};
 
-    auto body = [&](uint32_t* keys, uint8_t* state) __attribute__((always_inline)) {
+// f32 scores that are certainly above, or below, the K-th largest in 64 bits; th: the
+// K-th largest f32 score.  False where the bound is not finite.
+template <int QKIND, int NT>
+__device__ __forceinline__ bool select_window(const Pick& p, float th, Team& team, float& over, float& under) {
+    using tag = typename GenMfma<QKIND>::tag;
+    const SelectArgs& a = p.a;
+    const int lane = threadIdx.x & 63, G = a.hq / a.hkv;
+    // E = (D + 32) 2^-23 max_h |q_h|_1 max |bound|: D products that are not 0, each with a sum whose rounding may
+    // be a whole last bit, and room for this bound's own roundings
+    float qs = 0.f;
+    for (int r = team.wave; r < G; r += NT / 64) {
+        const uint16_t* qrow = a.q + (static_cast<int64_t>(p.t) * a.hq + p.h * G + r) * a.d;
+        float s = 0.f;
+        for (int d = 2 * lane; d < a.d; d += 128) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(qrow + d);
+            s += __builtin_fabsf(to_f32<tag>(static_cast<uint16_t>(w))) + __builtin_fabsf(to_f32<tag>(static_cast<uint16_t>(w >> 16)));
+        }
+        qs = fmaxf(qs, wave_sum(s));
+    }
+    float km = 0.f;
+    const int ch0 = p.base / a.chunk, ch1 = (p.base + p.n - 1) / a.chunk;
+    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, a.kmax[static_cast<int64_t>(p.unit) * a.chunks + i]);
+    qs = __uint_as_float(team.max(__float_as_uint(qs)));
+    km = wave_max(km);
+    const float all = qs * km;                               // 0: every score is exactly 0
+    const float eps = all == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * all + 0x1p-100f;
+    const float slack = 2.f * eps + (eps > 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
+    over = th + slack;
+    under = th - slack;
+    return gen_finite(over) && gen_finite(under);
+}
+
+// The list of a row of any number of candidates, whatever their scores: keys and states in memory.
+template <int QKIND, int KVKIND, int NT>
+__device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h, int t, int seq, int nv, uint32_t* s_team) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Team team = {s_team, NT / 64, wave, 0};
+    const int32_t* const bt = a.bt + static_cast<int64_t>(seq) * a.maxb;
+    int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
+    const bool all = nv <= a.k;
+    const int base = a.first, n = all ? 0 : nv - a.last - a.first;
+    const Pick p = {a, bt, sel, unit, h, t, nv, base, n};
+    auto usable = [&](int j) __attribute__((always_inline)) { return p.usable(j); };
+    uint32_t* const keys = a.keys + unit * a.pitch + base;
+    uint8_t* const state = a.state + unit * a.pitch + base;
+    __syncthreads();
         int K = 0, ties = 0;
         if (!all) {
-            const uint32_t* const g = a.keys + unit * a.pitch + base;
             int c = 0, f = 0;
             for (int i0 = 0; i0 < a.first + a.last; i0 += NT) {
                 const int i = i0 + threadIdx.x;
@@ -314,8 +457,7 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
                 const int i = i0 + threadIdx.x;
                 uint32_t key = 0;
                 if (i < n) {
-                    key = g[i];
-                    if (keys != g) keys[i] = key;
+                    key = keys[i];
                     state[i] = key ? MID : OUT;
                 }
                 const float x = unorder32(key);
@@ -330,26 +472,9 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
                 const bool any_odd = team.max(__builtin_amdgcn_ballot_w64(odd) != 0) != 0;
                 bool again = any_odd;
                 if (!any_odd) {
-                    // E = (2 D + 32) 2^-23 max_h |q_h|_1 max |bound|: every product once, every sum with a rounding
-                    // of its own that may be a whole last bit, and room for this bound's own roundings
-                    const int G = a.hq / a.hkv;
-                    float qs = 0.f;
-                    for (int r = wave; r < G; r += NW) {
-                        const uint16_t* qrow = a.q + (static_cast<int64_t>(t) * a.hq + h * G + r) * a.d;
-                        float s = 0.f;
-                        for (int d = lane; d < a.d; d += 64) s += __builtin_fabsf(to_f32<tag>(qrow[d]));
-                        qs = fmaxf(qs, wave_sum(s));
-                    }
-                    float km = 0.f;
-                    const int ch0 = base / a.chunk, ch1 = (base + n - 1) / a.chunk;
-                    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, a.kmax[static_cast<int64_t>(unit) * a.chunks + i]);
-                    qs = __uint_as_float(team.max(__float_as_uint(qs)));
-                    km = wave_max(km);
-                    const float eps = (2 * a.d + 32) * 0x1p-23f * qs * km + 0x1p-100f;
+                    float over, under;
                     const float th = unorder32(kth_largest<NT>(keys, state, n, K, team));
-                    const float over = th + 2.f * eps + __builtin_fabsf(th) * 0x1p-22f;
-                    const float under = th - 2.f * eps - __builtin_fabsf(th) * 0x1p-22f;
-                    again = !gen_finite(over) || !gen_finite(under);
+                    again = !select_window<QKIND, NT>(p, th, team, over, under);
                     if (!again) {
                         int in = 0, mid = 0;
                         for (int i0 = 0; i0 < n; i0 += NT) {
@@ -414,26 +539,253 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
             out += taken;
         }
         for (int i = out + threadIdx.x; i < a.k; i += NT) sel[i] = -1;
+}
+
+// Scores of up to four candidates at once, 16 lanes each: the lane's own, in all 16.
+template <int QKIND, int KVKIND>
+__device__ __forceinline__ double exact_score16(const Pick& p, int j) {
+    using tag = typename GenMfma<QKIND>::tag;
+    using raw_t = GenRaw<KVKIND>;
+    constexpr int ES = gen_is_fp8<KVKIND>() ? 1 : 2;
+    const SelectArgs& a = p.a;
+    const int l = threadIdx.x & 15, D = a.d, G = a.hq / a.hkv;
+    const uint8_t* const at = static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(p.bt[j]) * a.hkv + p.h) * 2 * D * ES;
+    double best = -INFINITY;
+    bool nan = false;
+    for (int g = 0; g < G; ++g) {
+        const uint16_t* qrow = a.q + (static_cast<int64_t>(p.t) * a.hq + p.h * G + g) * D;
+        double s = 0.0;
+        for (int d0 = 8 * l; d0 < D; d0 += 128) {
+            const uint4 q = *reinterpret_cast<const uint4*>(qrow + d0);
+            const uint4 lo = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(at + d0 * ES));
+            const uint4 hi = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(at + (D + d0) * ES));
+            const uint32_t qu[4] = {q.x, q.y, q.z, q.w}, lu[4] = {lo.x, lo.y, lo.z, lo.w}, hu[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int w = i >> 1, sh = (i & 1) * 16;
+                const double qd = to_f32<tag>(static_cast<uint16_t>(qu[w] >> sh));
+                const double x = qd * to_f32<tag>(static_cast<uint16_t>(lu[w] >> sh));
+                const double y = qd * to_f32<tag>(static_cast<uint16_t>(hu[w] >> sh));
+                s += x > y ? x : y;                          // finite: the window was
+            }
+        }
+        for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x);
+        nan |= s != s;
+        best = s > best ? s : best;
+    }
+    return nan ? __builtin_nan("") : best;
+}
+
+// A workgroup per (row, kv head), each thread KPT candidates in registers: wave w the
+// w-th part of them, so that a list comes out in order.  Latency counts here: bits
+// that all keys share are not searched, and the search ends where K keys remain.
+template <int QKIND, int KVKIND, int NT, int KPT>
+__global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
+    constexpr int NW = NT / 64, REFINE = 64;
+    __shared__ uint32_t s_team[2 * NW];
+    __shared__ uint64_t s_exact[REFINE];
+    __shared__ int s_cand[REFINE];
+    __shared__ uint8_t s_take[REFINE];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x, h = unit % a.hkv, t = a.row0 + unit / a.hkv;
+    const SparseRow row = sparse_row(t, a.qsl, a.seq_lens, a.num_seqs);
+    if (row.seq < 0) return;
+    const int nv = visible_blocks(a, row);
+    const int n = nv - a.last - a.first;
+    auto quickly = [&]() __attribute__((always_inline)) -> bool {
+        Team team = {s_team, NW, wave, 0};
+        const Pick p = {a, a.bt + static_cast<int64_t>(row.seq) * a.maxb, a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k,
+                        unit, h, t, nv, a.first, n};
+        const uint64_t below = (uint64_t(1) << lane) - 1;
+
+        const uint32_t* const keys = a.keys + unit * a.pitch + p.base;
+        const int kpw = (n + NT - 1) / NT, i0 = wave * kpw * 64 + lane;      // keys of a lane, its first candidate
+        uint32_t key[KPT], hi = 0, low = 0;
+        int eligible = 0;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) key[j] = j < kpw && i0 + 64 * j < n ? keys[i0 + 64 * j] : 0;
+        auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < KPT; ++j)
+                if (j < kpw) f(j);
+        };
+        // the forced blocks, by every wave for itself
+        int nf = 0, nl = 0;
+        for (int x = 0; x < a.first; x += 64) nf += wave_count(x + lane < a.first && p.usable(x + lane));
+        for (int x = 0; x < a.last; x += 64) nl += wave_count(x + lane < a.last && p.usable(nv - a.last + x + lane));
+        each([&](int j) __attribute__((always_inline)) {
+            eligible += wave_count(key[j] != 0);
+            hi = umax(hi, key[j]);
+            if (key[j]) {
+                low = umax(low, ~key[j]);
+                odd |= !gen_finite(unorder32(key[j]));
+            }
+        });
+        eligible = team.sum(eligible);
+        int K = a.k - nf - nl;
+        uint32_t over_key = 0xffffffffu, under_key = 0xffffffffu;            // above: in; from under on: in the middle
+        int places = 0;                                                      // for the middle
+        bool refine = false, slow = false;
+        if (eligible <= K) {
+            over_key = 0;
+        } else if (K > 0) {
+            hi = team.max(wave_umax(hi));
+            const uint32_t lo = ~team.max(wave_umax(low));
+            slow = team.max(__builtin_amdgcn_ballot_w64(odd) != 0) != 0;
+            uint32_t th = hi;
+            if (!slow && hi != lo) {
+                const int b0 = 31 - __builtin_clz(hi ^ lo);
+                uint32_t pre = b0 == 31 ? 0 : hi >> (b0 + 1) << (b0 + 1);
+                bool exact = false;
+                for (int b = b0; b >= 0 && !exact; --b) {
+                    const uint32_t test = pre | 1u << b;
+                    int c = 0;
+                    each([&](int j) __attribute__((always_inline)) {
+                        c += wave_count(key[j] >= test);
+                    });
+                    c = team.sum(c);
+                    if (c >= K) pre = test;
+                    exact = c == K;
+                }
+                th = pre;
+                if (exact) {                                                 // the least of the K
+                    uint32_t least = 0;
+#pragma unroll
+                    for (int j = 0; j < KPT; ++j)
+                        if (key[j] >= pre) least = umax(least, ~key[j]);
+                    th = ~team.max(wave_umax(least));
+                }
+            }
+            float over = 0.f, under = 0.f;
+            if (!slow) slow = !select_window<QKIND, NT>(p, unorder32(th), team, over, under);
+            if (!slow) {
+                over_key = order32(over);
+                under_key = order32(under);
+                int in = 0, mid = 0;
+                each([&](int j) __attribute__((always_inline)) {
+                    in += wave_count(key[j] > over_key);
+                    mid += wave_count(key[j] >= under_key);
+                });
+                in = team.sum(in);
+                mid = team.sum(mid) - in;
+                places = K - in;
+                refine = mid > places && over_key != under_key;
+                slow = refine && mid > REFINE;
+                if (refine && !slow) {
+                    int mine = 0, before;
+                    each([&](int j) __attribute__((always_inline)) {
+                        mine += wave_count(key[j] >= under_key && key[j] <= over_key);
+                    });
+                    team.scan(mine, before);
+                    each([&](int j) __attribute__((always_inline)) {
+                        const bool is = key[j] >= under_key && key[j] <= over_key;
+                        const uint64_t m = __builtin_amdgcn_ballot_w64(is);
+                        if (is) s_cand[before + __popcll(m & below)] = i0 + 64 * j;
+                        before += __popcll(m);
+                    });
+                    __syncthreads();
+                    for (int e = threadIdx.x >> 4; e < mid; e += NT / 16) {
+                        const uint64_t k64 = order64(exact_score16<QKIND, KVKIND>(p, p.base + s_cand[e]));
+                        if ((lane & 15) == 0) s_exact[e] = k64;
+                    }
+                    __syncthreads();
+                    if (static_cast<int>(threadIdx.x) < mid) {               // candidates stand in their order: ties to the lower
+                        const uint64_t me = s_exact[threadIdx.x];
+                        int rank = 0;
+                        for (int e = 0; e < mid; ++e) rank += s_exact[e] > me || (s_exact[e] == me && e < static_cast<int>(threadIdx.x));
+                        s_take[threadIdx.x] = rank < places;
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+        if (slow) return false;
+
+        // the list: the first blocks, the candidates in order, the last blocks, -1
+        int mine = 0, taken = 0, mids, outs;
+        if (eligible > K) {
+            int m = 0;
+            each([&](int j) __attribute__((always_inline)) {
+                m += wave_count(key[j] >= under_key && key[j] <= over_key);
+            });
+            team.scan(m, mids);
+        } else {
+            mids = 0;
+        }
+        const int mids0 = mids;
+        auto chosen = [&](int j) __attribute__((always_inline)) -> bool {    // and moves `mids` on
+            const bool is = key[j] >= under_key && key[j] <= over_key;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(is);
+            const int at = mids + __popcll(m & below);
+            mids += __popcll(m);
+            return key[j] > over_key || (is && (refine ? s_take[at] != 0 : at < places));
+        };
+        each([&](int j) __attribute__((always_inline)) {
+            mine += wave_count(chosen(j));
+        });
+        taken = team.scan(mine, outs);
+        mids = mids0;
+        outs += nf;
+        each([&](int j) __attribute__((always_inline)) {
+            const bool in = chosen(j);
+            const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+            if (in) p.sel[outs + __popcll(m & below)] = p.base + i0 + 64 * j;
+            outs += __popcll(m);
+        });
+        if (wave == 0) {
+            int at = 0;
+            auto forced = [&](int j0, int count) __attribute__((always_inline)) {
+                for (int x = 0; x < count; x += 64) {
+                    const bool in = x + lane < count && p.usable(j0 + x + lane);
+                    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+                    if (in) p.sel[at + __popcll(m & below)] = j0 + x + lane;
+                    at += __popcll(m);
+                }
+            };
+            forced(0, a.first);
+            at += taken;
+            forced(nv - a.last, a.last);
+            for (int i = at + lane; i < a.k; i += 64) p.sel[i] = -1;
+        }
+        return true;
     };
-    if (n <= SELECT_LDS) body(s_keys, s_state);
-    else body(a.keys + unit * a.pitch + base, a.state + unit * a.pitch + base);
+    if (nv > a.k && n <= NT * KPT && quickly()) return;
+    pick_slowly<QKIND, KVKIND, NT>(a, unit, h, t, row.seq, nv, s_team);
 }
 
 template <int QKIND, int KVKIND>
-int32_t launch_select(const SelectArgs& a, hipStream_t st) {
+int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
     const int64_t units = static_cast<int64_t>(a.rows) * a.hkv;
-    const dim3 grid(static_cast<unsigned>(units * a.chunks));
     if (a.chunks > 0) {
-        switch (a.d / 32) {
+        if (tiles) {
+            const int tile = 16 * select_m_tiles(a.d) >> a.group_log2;
+            const int64_t count = (static_cast<int64_t>(a.row0) + a.rows + tile - 1) / tile + a.num_seqs;
+            const dim3 grid(static_cast<unsigned>(count * a.hkv * a.chunks));
+            switch (a.d / 32) {
+#define RLLM_SCORE(N) \
+    case N: hipLaunchKernelGGL((select_score_tile_kernel<QKIND, KVKIND, N>), grid, dim3(256), 0, st, a); break;
+                RLLM_SCORE(1) RLLM_SCORE(2) RLLM_SCORE(3) RLLM_SCORE(4) RLLM_SCORE(5) RLLM_SCORE(6) RLLM_SCORE(7) RLLM_SCORE(8)
+#undef RLLM_SCORE
+            }
+        } else {
+            const dim3 grid(static_cast<unsigned>(units * a.chunks));
+            switch (a.d / 32) {
 #define RLLM_SCORE(N) \
     case N: hipLaunchKernelGGL((select_score_kernel<QKIND, KVKIND, N>), grid, dim3(256), 0, st, a); break;
-            RLLM_SCORE(1) RLLM_SCORE(2) RLLM_SCORE(3) RLLM_SCORE(4) RLLM_SCORE(5) RLLM_SCORE(6) RLLM_SCORE(7) RLLM_SCORE(8)
+                RLLM_SCORE(1) RLLM_SCORE(2) RLLM_SCORE(3) RLLM_SCORE(4) RLLM_SCORE(5) RLLM_SCORE(6) RLLM_SCORE(7) RLLM_SCORE(8)
 #undef RLLM_SCORE
+            }
         }
         const int32_t rc = launch_status();
         if (rc) return rc;
     }
-    hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
+    // a wave a row where rows are many and short enough, else four
+    if (units >= 2048 && a.maxb <= 64 * 32)
+        hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 64, 32>), dim3(static_cast<unsigned>(units)), dim3(64), 0, st, a);
+    else
+        hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256, 32>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
     return launch_status();
 }
 
@@ -443,7 +795,7 @@ constexpr int64_t SELECT_CHUNK_MIN = 64, SELECT_CHUNK_MAX = 512;
 // bytes of scratch of a row: never fewer for a wider table
 int64_t select_row_bytes(int64_t hkv, int64_t maxb, int64_t& pitch) {
     pitch = (maxb + SELECT_CHUNK_MAX - 1) / SELECT_CHUNK_MAX * SELECT_CHUNK_MAX;
-    return hkv * (pitch * 4 + pitch / SELECT_CHUNK_MIN * 4 + (maxb > SELECT_LDS ? pitch : 0));
+    return hkv * (pitch * 4 + pitch / SELECT_CHUNK_MIN * 4 + pitch);
 }
 int64_t select_bytes(int64_t num_rows, int64_t row_bytes) {
     const int64_t slab = row_bytes > SELECT_SLAB ? row_bytes : SELECT_SLAB;
@@ -521,6 +873,10 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     a.chunks = static_cast<int32_t>(chunks);
     a.num_blocks = num_blocks;
     a.pitch = pitch;
+    const int64_t group = num_q_heads / num_kv_heads;
+    while ((1 << a.group_log2) < group) ++a.group_log2;
+    const bool tiles = query_start_loc && group <= 16 && num_rows >= 2 * num_seqs;
+    if (tiles) RLLM_CHECK_ARG((num_rows + num_seqs) * num_kv_heads * chunks <= INT32_MAX);
     const hipStream_t st = as_stream(stream);
     for (int64_t r = 0; r < num_rows; r += slab) {
         a.row0 = static_cast<int32_t>(r);
@@ -530,13 +886,13 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
         a.state = reinterpret_cast<uint8_t*>(a.kmax + units * (pitch / SELECT_CHUNK_MIN));
         int32_t rc;
         if (q_dtype == RLLM_DTYPE_BF16)
-            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_BF16, KIND_FP8_E4M3>(a, st)
-                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_BF16, KIND_FP8_E5M2>(a, st)
-                                                   : launch_select<KIND_BF16, KIND_BF16>(a, st);
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_BF16, KIND_FP8_E4M3>(a, tiles, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_BF16, KIND_FP8_E5M2>(a, tiles, st)
+                                                   : launch_select<KIND_BF16, KIND_BF16>(a, tiles, st);
         else
-            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_F16, KIND_FP8_E4M3>(a, st)
-                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_F16, KIND_FP8_E5M2>(a, st)
-                                                   : launch_select<KIND_F16, KIND_F16>(a, st);
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_F16, KIND_FP8_E4M3>(a, tiles, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_F16, KIND_FP8_E5M2>(a, tiles, st)
+                                                   : launch_select<KIND_F16, KIND_F16>(a, tiles, st);
         if (rc) return rc;
     }
     return 0;

@@ -155,7 +155,9 @@ def attend(q, kc, vc, bt, lens, qsl, sel, scale, k_scale=1.0, v_scale=1.0):
         for h in range(hkv):
             keys, before = [], -1
             for j in sel[t, h].tolist():
-                if j > before and usable(bt, s, j, nb) and j * bs <= pos:
+                if j <= before:
+                    break
+                if usable(bt, s, j, nb) and j * bs <= pos:
                     keys += [(int(bt[s, j]), o) for o in range(min(bs, pos + 1 - j * bs))]
                 before = j
             hs = slice(h * g, (h + 1) * g)

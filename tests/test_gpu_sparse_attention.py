@@ -74,6 +74,60 @@ def test_chunk_rows(dev, kind, kv, hq, hkv, d, bs):
     check(dev, q, kc, vc, kind, kv, bt, lens, lists(rng, bt, lens, qsl, n, hkv, bs, 12), bs, d ** -0.5, qsl)
 
 
+def chunk(rng, lens, new, hq, hkv, d, bs, kind, kv):
+    bt, nb = S.tables(rng, lens, bs)
+    qsl = (2 + np.concatenate([[0], np.cumsum(new)])).tolist()
+    n = sum(new) + 5
+    return bt, pool(rng, nb, hkv, d, bs, kv), qsl, n, queries(rng, n, hq, d, kind)
+
+
+@pytest.mark.parametrize("kind,kv,hq,hkv,d,bs,n", [
+    ("bf16", "bf16", 32, 8, 128, 16, 150), ("f16", "e4m3", 24, 8, 128, 32, 150), ("bf16", "e5m2", 16, 16, 32, 16, 280),
+    ("f16", "f16", 16, 8, 64, 64, 300), ("bf16", "bf16", 28, 4, 96, 128, 150), ("f16", "f16", 16, 2, 256, 16, 270),
+    ("f16", "e5m2", 32, 8, 224, 16, 140), ("bf16", "e4m3", 32, 8, 96, 16, 140)])
+def test_tiles_of_rows(dev, kind, kv, hq, hkv, d, bs, n):
+    """Chunks whose rows share a workgroup: lists that overlap in part, that end where each row does, and empty ones; runs that end
+    inside a tile, a sequence without rows, more rows than keys."""
+    rng = np.random.default_rng(d + n)
+    new = [n // 2 + 1, 0, 1, n // 3, 7, n - n // 2 - n // 3 - 9]
+    lens = [9 * bs + 3 + new[0], 40, 1, 200 + new[3], 4, new[5]]
+    bt, (kc, vc), qsl, rows, q = chunk(rng, lens, new, hq, hkv, d, bs, kind, kv)
+    assert rows >= 2 * len(lens)
+    sel = lists(rng, bt, lens, qsl, rows, hkv, bs, 7)
+    check(dev, q, kc, vc, kind, kv, bt, lens, sel, bs, d ** -0.5, qsl)
+    bt[0, 2], bt[3, 1], bt[5, 0] = -1, kc.shape[0], -7          # unused entries among the listed
+    check(dev, q, kc, vc, kind, kv, bt, lens, sel, bs, 0.0, qsl)
+    sel[:] = torch.from_numpy(rng.integers(-2, 12, tuple(sel.shape)).astype(np.int32))   # lists that do not rise
+    check(dev, q, kc, vc, kind, kv, bt, lens, sel, bs, -d ** -0.5, qsl)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_rows_of_a_tile_do_not_see_each_other_s_blocks(dev, kv):
+    rng = np.random.default_rng(91)
+    lens, new = [400], [160]
+    bt, (kc, vc), qsl, n, q = chunk(rng, lens, new, 32, 8, 64, 16, "bf16", kv)
+    sel = lists(rng, bt, lens, qsl, n, 8, 16, 9)
+    sel = torch.where(sel == 5, 6, sel)                         # now and then 6 twice: the second attends nothing
+    kc, vc = S.values(kc, kv), S.values(vc, kv)
+    kc[int(bt[0, 5])] = float("nan")
+    vc[int(bt[0, 5])] = float("nan")
+    vc[int(bt[0, 24]), :, :, 15] = float("nan")                 # the chunk's last key: the other rows stand before it
+    some = sel.clone()
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[rng.permutation(n - 10)[:20]] = True
+    some[hit, :, 0], some[hit, :, 1:] = 5, -1
+    kc, vc = S.store(kc.float(), kv), S.store(vc.float(), kv)
+    ks, vs = SCALES if kv in S.FP8 else (1.0, 1.0)
+    ref, mag, spread = S.attend(q, S.values(kc, kv), S.values(vc, kv), bt, lens, qsl, some, 0.125, ks, vs)
+    ref = torch.where(torch.isnan(ref), float("nan"), ref)
+    kw = dict(k_scale=ks, v_scale=vs, **S.fp8(kv)) if kv in S.FP8 else {}
+    out = ops.paged_sparse(q.to(dev), kc.to(dev), vc.to(dev), bt.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev),
+                           some.to(dev), 0.125, query_start_loc=torch.tensor(qsl, dtype=torch.int32, device=dev), validate=False, **kw)
+    S.check_attend(out, ref, mag, spread, "bf16", 64, 9 * 16, "beside rows with NaN")
+    rows = torch.arange(n)
+    assert out.cpu()[hit & (rows >= 2) & (rows < 162)].isnan().all()
+
+
 def test_what_is_not_attended_is_not_looked_at(dev):
     """NaN and infinities behind the last key, in unlisted blocks, in blocks of unused entries."""
     rng = np.random.default_rng(3)
