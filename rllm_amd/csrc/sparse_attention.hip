@@ -36,12 +36,26 @@ int32_t rllm_paged_attention_sparse(void* output, const void* query, const void*
     RLLM_CHECK_ARG(std::isfinite(scale) && std::isfinite(k_scale) && std::isfinite(v_scale) && std::isfinite(s_scale));
     const int64_t head_groups = (num_q_heads / num_kv_heads + 15) / 16;
     RLLM_CHECK_ARG(num_rows * num_kv_heads * head_groups <= INT32_MAX);
-    SparseArgs a = {static_cast<uint16_t*>(output), static_cast<const uint16_t*>(query),
-                    static_cast<const uint8_t*>(key_cache), static_cast<const uint8_t*>(value_cache), block_tables, seq_lens,
-                    query_start_loc, selected, static_cast<int32_t>(num_seqs), static_cast<int32_t>(num_rows),
-                    static_cast<int32_t>(num_q_heads), static_cast<int32_t>(num_kv_heads),
-                    __builtin_ctz(static_cast<unsigned>(block_size)), static_cast<int32_t>(max_num_blocks_per_seq),
-                    static_cast<int32_t>(num_selected), static_cast<int32_t>(head_groups), 1, 0, num_blocks, s_scale, v_scale};
+    SparseArgs a = {};
+    a.out = static_cast<uint16_t*>(output);
+    a.q = static_cast<const uint16_t*>(query);
+    a.kc = static_cast<const uint8_t*>(key_cache);
+    a.vc = static_cast<const uint8_t*>(value_cache);
+    a.bt = block_tables;
+    a.seq_lens = seq_lens;
+    a.qsl = query_start_loc;
+    a.sel = selected;
+    a.num_seqs = static_cast<int32_t>(num_seqs);
+    a.rows = static_cast<int32_t>(num_rows);
+    a.hq = static_cast<int32_t>(num_q_heads);
+    a.hkv = static_cast<int32_t>(num_kv_heads);
+    a.bs_log2 = __builtin_ctz(static_cast<unsigned>(block_size));
+    a.maxb = static_cast<int32_t>(max_num_blocks_per_seq);
+    a.k = static_cast<int32_t>(num_selected);
+    a.head_groups = static_cast<int32_t>(head_groups);
+    a.num_blocks = num_blocks;
+    a.s_scale = s_scale;
+    a.v_scale = v_scale;
     const hipStream_t st = as_stream(stream);
     if (kv_dtype == RLLM_DTYPE_FP8_E4M3) return launch_sparse_e4m3(a, q_dtype, head_dim, st);
     if (kv_dtype == RLLM_DTYPE_FP8_E5M2) return launch_sparse_e5m2(a, q_dtype, head_dim, st);

@@ -29,10 +29,12 @@
 
 #include "sparse_blocks.h"
 #include "generic_mfma.h"
+#include "workspace.h"
 
 namespace rllm {
 
 constexpr int SA_WIN = 64;      // tokens of a wave's window: 4 groups of 16
+constexpr int SA_MAX_SPLITS = 8;
 constexpr int SA_MAX_LIST = RLLM_SELECT_MAX_BLOCKS;   // entries of a tile's list, 10 bytes of LDS each
 
 struct SparseArgs {
@@ -41,6 +43,9 @@ struct SparseArgs {
     const uint8_t *kc, *vc;
     const int32_t *bt, *seq_lens, *qsl, *sel;
     int32_t num_seqs, rows, hq, hkv, bs_log2, maxb, k, head_groups;
+    int32_t splits;             // workgroups of a unit, joined by the last to end
+    int32_t* count;             // arrivals of a unit, 0 between calls
+    float* part;                // [unit][split][16 columns][head_dim + 2]: sum, max and sum of weights
     int32_t tile, list;         // rows of a workgroup (1, or 16 / heads of a kv head), and the entries its list has room for
     int64_t num_blocks;
     float s_scale, v_scale;     // s_scale: scale * k_scale * log2(e)
@@ -142,7 +147,8 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
     const int r = lane & 15, q4 = lane >> 4;
     const int G = a.hq / a.hkv;
     const int hg = blockIdx.x % a.head_groups;
-    const int unit = blockIdx.x / a.head_groups, h = unit % a.hkv;
+    const int split = blockIdx.x / a.head_groups % a.splits;
+    const int unit = blockIdx.x / a.head_groups / a.splits, h = unit % a.hkv;
     // column r: row r >> gl of the tile, head 16 hg + (r & (2^gl - 1)) of the group
     const int gl = a.tile > 1 ? 31 - __builtin_clz(16 / a.tile) : 4;
     const int col_row = r >> gl, col_head = 16 * hg + (r & ((1 << gl) - 1));
@@ -212,11 +218,8 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
                     if (b >= 0) most = i + 1;
                 }
             }
-            const uint64_t some = __builtin_amdgcn_ballot_w64(most > 0);
-            if (some) {
-                const int top = __builtin_amdgcn_readlane(most, 63 - __builtin_clzll(some));   // i rises with the lane
-                if (lane == 0) atomicMax(&s_used, top);
-            }
+            most = static_cast<int>(wave_umax(static_cast<uint32_t>(most)));
+            if (lane == 0 && most) atomicMax(&s_used, most);
         } else {
             // the union: a word of bits for every block of the sequence, where the windows will be
             uint16_t* const s_bits = reinterpret_cast<uint16_t*>(lds);
@@ -358,7 +361,8 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) o[dt] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
-    int w0 = SA_WIN * wave;
+    const int stride = SA_WIN * waves * a.splits;               // from a wave's window to its next
+    int w0 = SA_WIN * (split * waves + wave);
     int blocks, nums, masks;
     entries(w0, blocks, nums, masks);
     if (w0 < end) {
@@ -368,7 +372,7 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
     const uint8_t* const k_src = stage + (4 * q4 + (r >> 2)) * 32 + (((r & 3) * 8) ^ swap16(4 * q4));
     const uint8_t* const v_src = stage + r * 32 + ((q4 * 8) ^ swap16(r));
     while (w0 < end) {
-        const int w1 = w0 + SA_WIN * waves;
+        const int w1 = w0 + stride;
         int next, next_nums, next_masks;
         entries(w1, next, next_nums, next_masks);
         // ---- S^T = K Q^T ----
@@ -507,6 +511,7 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
     for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<gm_f32x4*>(s_o(wave) + r * OST + 16 * dt + 4 * q4) = o[dt];
     __syncthreads();
     constexpr int quads = D >> 2;
+    const int64_t part_unit = static_cast<int64_t>(unit) * a.head_groups + hg;
     bool bad = false;
     for (int it = threadIdx.x; it < 16 * quads; it += threads) {
         const int col = it / quads, d0 = (it - col * quads) * 4;
@@ -523,10 +528,56 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
             L = fmaf(f, lw, L);
             sum += f * *reinterpret_cast<const gm_f32x4*>(s_o(w) + col * OST + d0);
         }
+        if (a.splits > 1) {
+            float* const x = a.part + ((part_unit * a.splits + split) * 16 + col) * (D + 4);
+            *reinterpret_cast<gm_f32x4*>(x + d0) = sum;
+            if (d0 == 0) *reinterpret_cast<gm_f32x4*>(x + D) = gm_f32x4{mx, L, 0.f, 0.f};
+            continue;
+        }
         const gm_f32x4 v = sum * gen_inv(a.v_scale, L);
         bad |= !(gen_finite(v[0]) && gen_finite(v[1]) && gen_finite(v[2]) && gen_finite(v[3]));
         *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(t + cr) * a.hq + h * G + ch) * D + d0) =
             make_uint2(M::pack2(v[0], v[1]), M::pack2(v[2], v[3]));
+    }
+    if (a.splits > 1) {
+        // the last workgroup of the unit joins its parts, in their order
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const int before = __hip_atomic_fetch_add(a.count + part_unit, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            s_used = before == a.splits - 1;
+            if (s_used) __hip_atomic_store(a.count + part_unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!s_used) return;
+        for (int it = threadIdx.x; it < 16 * quads; it += threads) {
+            const int col = it / quads, d0 = (it - col * quads) * 4;
+            if (16 * hg + col >= G) continue;
+            const float* const x = a.part + (part_unit * a.splits * 16 + col) * (D + 4);
+            constexpr int step = 16 * (D + 4);
+            gm_f32x4 v[SA_MAX_SPLITS];
+            gm_f32x2 ml[SA_MAX_SPLITS];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < SA_MAX_SPLITS; ++i) {
+                const int j = min(i, a.splits - 1);
+                v[i] = *reinterpret_cast<const gm_f32x4*>(x + j * step + d0);
+                ml[i] = *reinterpret_cast<const gm_f32x2*>(x + j * step + D);
+                mx = fmaxf(mx, ml[i][0]);
+            }
+            gm_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            float L = 0.f;
+#pragma unroll
+            for (int i = 0; i < SA_MAX_SPLITS; ++i) {
+                if (i >= a.splits || ml[i][1] == 0.f) continue;
+                const float f = exp2f(ml[i][0] - mx);
+                L = fmaf(f, ml[i][1], L);
+                sum += f * v[i];
+            }
+            sum *= gen_inv(a.v_scale, L);
+            *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(t) * a.hq + h * G + 16 * hg + col) * D + d0) =
+                make_uint2(M::pack2(sum[0], sum[1]), M::pack2(sum[2], sum[3]));
+        }
+        return;
     }
     // 0 * Inf from a block that another row of the tile lists would show here: rows by themselves
     if (nt > 1 && __syncthreads_or(bad))
@@ -538,7 +589,7 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
 template <int QKIND, int KVKIND, int RUN>
 int32_t launch_sparse_run(const SparseArgs& a, int64_t d, int waves, hipStream_t st) {
     const int64_t tiles = a.tile > 1 ? (static_cast<int64_t>(a.rows) + a.tile - 1) / a.tile + a.num_seqs : a.rows;
-    const dim3 grid(static_cast<unsigned>(tiles * a.hkv * a.head_groups)), block(64 * waves);
+    const dim3 grid(static_cast<unsigned>(tiles * a.hkv * a.head_groups * a.splits)), block(64 * waves);
     const size_t lds = static_cast<size_t>(waves) * sa_stage_bytes(static_cast<int>(d)) + a.list * 10;
     switch (d / 32) {
 #define RLLM_SPARSE(N) \
@@ -552,8 +603,27 @@ int32_t launch_sparse_run(const SparseArgs& a, int64_t d, int waves, hipStream_t
 template <int QKIND, int KVKIND>
 int32_t launch_sparse(SparseArgs a, int64_t d, hipStream_t st) {
     const int64_t units = static_cast<int64_t>(a.rows) * a.hkv * a.head_groups;
-    int waves = units <= 256 && (static_cast<int64_t>(a.k) << a.bs_log2) > 4 * SA_WIN ? 8 : 4;
-    waves = waves < sa_max_waves(static_cast<int>(d)) ? waves : sa_max_waves(static_cast<int>(d));
+    int waves = 4;
+    // Few units: a CU draws some 13 bytes a clock from memory however much it asks for,
+    // so a unit goes to several (1 row on 64 blocks, 8 kv heads, head_dim 128: one
+    // workgroup of 8 waves 13.5 us).  A capture on a stream without scratch does without.
+    a.splits = 1;
+    const int64_t windows = ((static_cast<int64_t>(a.k) << a.bs_log2) + SA_WIN - 1) / SA_WIN;
+    if (units <= 128 && windows > 2) {
+        int64_t splits = 256 / units < SA_MAX_SPLITS ? 256 / units : SA_MAX_SPLITS;
+        if (splits > (windows + 1) / 2) splits = (windows + 1) / 2;
+        void* ws = nullptr;
+        const int32_t rc = g_workspaces.get(reinterpret_cast<uintptr_t>(st), WS_SPARSE, 1024 + 256 * 16 * (d + 4) * 4, true, &ws);
+        if (rc) return rc;
+        if (ws) {
+            a.splits = static_cast<int32_t>(splits);
+            a.count = static_cast<int32_t*>(ws);
+            a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 1024);
+            waves = windows <= 2 * splits ? 2 : 4;
+        } else {
+            waves = sa_max_waves(static_cast<int>(d));
+        }
+    }
     // tiles: in a chunk of several rows a sequence, where heads leave columns free, tiles
     // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 -> 156 us),
     // the blocks' bits fit where the windows go, and the union of the lists beside it

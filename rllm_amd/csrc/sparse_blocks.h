@@ -89,5 +89,38 @@ __device__ __forceinline__ i16x2 ordered2(uint32_t w) {
 }
 __device__ __forceinline__ int16_t ordered1(int16_t x) { return static_cast<int16_t>(x ^ ((x >> 15) & 0x7fff)); }
 
+// lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ uint32_t quads_umax(uint32_t v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
+    const auto y = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(static_cast<uint32_t>(y[0]), static_cast<uint32_t>(y[1]));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+// of all 64 lanes
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = max(v, dpp_u<DPP_QUAD_XOR1>(v));
+    v = max(v, dpp_u<DPP_QUAD_XOR2>(v));
+    v = max(v, dpp_u<DPP_ROW_HALF_MIRROR>(v));
+    v = max(v, dpp_u<DPP_ROW_MIRROR>(v));
+    return quads_umax(v);
+}
+// the sum of 16 lanes, in each of them
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint64_t w = static_cast<uint64_t>(dpp_u<CTRL>(static_cast<uint32_t>(u >> 32))) << 32 | dpp_u<CTRL>(static_cast<uint32_t>(u));
+    return __longlong_as_double(static_cast<long long>(w));
+}
+__device__ __forceinline__ double row_sum16(double v) {
+    v += dpp_d<DPP_QUAD_XOR1>(v);
+    v += dpp_d<DPP_QUAD_XOR2>(v);
+    v += dpp_d<DPP_ROW_HALF_MIRROR>(v);
+    return v + dpp_d<DPP_ROW_MIRROR>(v);
+}
+
 }  // namespace
 }  // namespace rllm

@@ -25,8 +25,9 @@ struct SelectArgs {
     const int32_t *bt, *seq_lens, *qsl;
     uint32_t* keys;     // [rows of the launch, hkv, pitch]: scores in their order, 0 = not to be chosen
     uint8_t* state;     // the same, where they do not fit in LDS
-    float* kmax;        // [rows of the launch, hkv, chunks]: largest |bound| of a chunk
+    float* kmax;        // [rows of the launch, hkv, chunks]: largest |bound| of a chunk, at a sequence's last row of the launch
     int32_t num_seqs, row0, rows, hq, hkv, d, bs_log2, maxb, k, first, last, chunk, chunks;
+    int32_t tiles;      // whether rows were scored in tiles
     int32_t group_log2; // heads of a group, as a power of two, where rows go in tiles
     int64_t num_blocks, pitch;
 };
@@ -65,105 +66,125 @@ __device__ __forceinline__ void split_signs(const uint4& x, uint4& neg, uint4& p
     neg = make_uint4(n[0], n[1], n[2], n[3]);
     pos = make_uint4(p[0], p[1], p[2], p[3]);
 }
-constexpr int select_m_tiles(int d) { return d > 128 ? 2 : 4; }   // 16-row tiles of a chunk's workgroup
+constexpr int select_m_tiles(int d) { return d > 128 ? 2 : 4; }   // 16-row tiles of a wave, in a chunk
 
-// A workgroup per (row, kv head, chunk of its blocks), a wave 16 blocks at a time:
-// v_mfma_16x16x32, rows = heads, columns = blocks, k = channels of lo, then of hi.
-// Each lane loads 8 channels of its column's block, the operand as it stands.
-// Bound by HBM: the bounds are read once a row.
+// A workgroup per (row, chunk of its blocks), a wave kv heads w, w + 4, ..., 16 blocks at
+// a time: v_mfma_16x16x32, rows = heads, columns = blocks, k = channels of lo, then of
+// hi.  Each lane loads 8 channels of its column's block, the operand as it stands.
+// Bound by HBM: the bounds are read once a row.  The heads of a block lie in a run, so
+// the waves of a workgroup read whole runs between them (64 rows of 250-2000 blocks, 8 kv
+// heads, head_dim 128: 84 us where a workgroup kept to one head).
 template <int QKIND, int KVKIND, int NK>
 __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
     using M = GenMfma<QKIND>;
     using raw_t = GenRaw<KVKIND>;
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     constexpr int ES = gen_is_fp8<KVKIND>() ? 1 : 2, D = 32 * NK;
-    __shared__ uint32_t s_max[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, kq = lane >> 4;
-    const int unit = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int h = unit % a.hkv, t = a.row0 + unit / a.hkv;
+    const int chunk = blockIdx.x % a.chunks, t = a.row0 + blockIdx.x / a.chunks;
     const SparseRow row = sparse_row(t, a.qsl, a.seq_lens, a.num_seqs);
     const int nv = visible_blocks(a, row);
     if (row.seq < 0 || nv <= a.k) return;
     const int c0 = max(chunk * a.chunk, a.first), c1 = min((chunk + 1) * a.chunk, nv - a.last);
     if (c0 >= c1) return;
     const int G = a.hq / a.hkv, hgs = (G + 15) / 16;
-    uint32_t top = 0;                                   // largest magnitudes, two 16-bit halves
     const int32_t* const bt = a.bt + static_cast<int64_t>(row.seq) * a.maxb;
-    uint32_t* const keys = a.keys + unit * a.pitch;
-    uint4 qn[NK], qp[NK];
-    auto load_q = [&](int hg) __attribute__((always_inline)) {
-        const bool live = 16 * hg + col < G;
-        const uint16_t* src = a.q + (static_cast<int64_t>(t) * a.hq + h * G + 16 * hg + col) * D;
+    for (int h = wave; h < a.hkv; h += 4) {
+        const int64_t unit = static_cast<int64_t>(t - a.row0) * a.hkv + h;
+        uint32_t top = 0;                                   // largest magnitudes, two 16-bit halves
+        uint32_t* const keys = a.keys + unit * a.pitch;
+        uint4 qn[NK], qp[NK];
+        auto load_q = [&](int hg) __attribute__((always_inline)) {
+            const bool live = 16 * hg + col < G;
+            const uint16_t* src = a.q + (static_cast<int64_t>(t) * a.hq + h * G + 16 * hg + col) * D;
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const uint4 x = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * kq) : make_uint4(0, 0, 0, 0);
-            split_signs(x, qn[i], qp[i]);
+            for (int i = 0; i < NK; ++i) {
+                const uint4 x = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * kq) : make_uint4(0, 0, 0, 0);
+                split_signs(x, qn[i], qp[i]);
+            }
+        };
+        load_q(0);
+        // the next tile's bounds are on their way while this one's are worked on, and its blocks' ids
+        auto block_at = [&](int b0) __attribute__((always_inline)) -> int32_t {
+            const int j = b0 + col;
+            int32_t b = -1;
+            if (j >= c0 && j < c1) {
+                b = bt[j];
+                if (b >= a.num_blocks) b = -1;
+            }
+            return b;
+        };
+        raw_t raw[2 * NK];
+        auto load = [&](int32_t b) __attribute__((always_inline)) {
+            const uint8_t* src = b >= 0 ? static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES)
+                                        : reinterpret_cast<const uint8_t*>(g_gen_zero);
+            const int st = b >= 0 ? ES : 0;
+#pragma unroll
+            for (int i = 0; i < 2 * NK; ++i) raw[i] = *reinterpret_cast<const raw_t*>(src + (32 * i + 8 * kq) * st);
+        };
+        const int first_tile = chunk * a.chunk;
+        int32_t b = block_at(first_tile), b_next = block_at(first_tile + 16);
+        load(b);
+        for (int b0 = first_tile; b0 < c1; b0 += 16) {
+            const int j = b0 + col;
+            uint4 x[2 * NK];
+#pragma unroll
+            for (int i = 0; i < 2 * NK; ++i) x[i] = gen_to16<QKIND, KVKIND>(raw[i]);
+            const bool here = b >= 0;
+            b = b_next;
+            if (b0 + 16 < c1) {
+                load(b);
+                b_next = block_at(b0 + 32);
+            }
+            u16x2 m = __builtin_bit_cast(u16x2, top);
+#pragma unroll
+            for (int i = 0; i < 2 * NK; ++i) {
+                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+            }
+            top = __builtin_bit_cast(uint32_t, m);
+            uint32_t best = 0;
+            for (int hg = 0; hg < hgs; ++hg) {
+                if (hgs > 1) load_q(hg);
+                gm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NK; ++i) acc = M::mma16(qn[i], x[i], acc);
+#pragma unroll
+                for (int i = 0; i < NK; ++i) acc = M::mma16(qp[i], x[NK + i], acc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * hg + 4 * kq + i < G) best = umax(best, order32(acc[i]));
+            }
+            best = quads_umax(best);
+            if (kq == 0 && j >= c0 && j < c1) keys[j] = here ? best : 0;
         }
-    };
-    load_q(0);
-    for (int b0 = chunk * a.chunk + 16 * wave; b0 < c1; b0 += 64) {
-        const int j = b0 + col;
-        int32_t b = -1;
-        if (j >= c0 && j < c1) {
-            b = bt[j];
-            if (b >= a.num_blocks) b = -1;
-        }
-        const uint8_t* src = b >= 0 ? static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES)
-                                    : reinterpret_cast<const uint8_t*>(g_gen_zero);
-        const int st = b >= 0 ? ES : 0;
-        uint4 x[2 * NK];
-#pragma unroll
-        for (int i = 0; i < 2 * NK; ++i)
-            x[i] = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(src + (32 * i + 8 * kq) * st));
-        u16x2 m = __builtin_bit_cast(u16x2, top);
-#pragma unroll
-        for (int i = 0; i < 2 * NK; ++i) {
-            const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
-        }
-        top = __builtin_bit_cast(uint32_t, m);
-        uint32_t best = 0;
-        for (int hg = 0; hg < hgs; ++hg) {
-            if (hgs > 1) load_q(hg);
-            gm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < NK; ++i) acc = M::mma16(qn[i], x[i], acc);
-#pragma unroll
-            for (int i = 0; i < NK; ++i) acc = M::mma16(qp[i], x[NK + i], acc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (16 * hg + 4 * kq + i < G) best = umax(best, order32(acc[i]));
-        }
-        best = umax(best, __shfl_xor(best, 16));
-        best = umax(best, __shfl_xor(best, 32));
-        if (kq == 0 && j >= c0 && j < c1) keys[j] = b >= 0 ? best : 0;
-    }
-    uint32_t t16 = umax(top & 0xffffu, top >> 16);
-    for (int x = 1; x < 64; x <<= 1) t16 = umax(t16, __shfl_xor(t16, x));
-    if (lane == 0) s_max[wave] = t16;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
-        a.kmax[static_cast<int64_t>(unit) * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
+        const uint32_t t16 = wave_umax(umax(top & 0xffffu, top >> 16));
+        if (lane == 0) a.kmax[unit * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
     }
 }
 
-// Rows of a chunk: a tile of them, 64 (row, head) pairs (32 past head_dim 128) of one
-// sequence and kv head, holds its queries in registers and takes the blocks as above;
-// a block's bounds serve every row of the tile.
+// Rows of a chunk: a workgroup has a tile of them, 256 (row, head) pairs (128 past head_dim
+// 128) of one sequence and kv head, a quarter a wave, their queries in registers.  The
+// bounds of 16 blocks at a time go to LDS in whole runs, the next ones on their way,
+// and serve every row of the tile.  704 rows of 1250-1650
+// blocks, 32/8 heads, head_dim 128: 60 us, 26 of them vector instructions; a
+// workgroup's start (its queries) is as long as its four steps.
 template <int QKIND, int KVKIND, int NK>
 __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a) {
     using M = GenMfma<QKIND>;
     using raw_t = GenRaw<KVKIND>;
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     constexpr int ES = gen_is_fp8<KVKIND>() ? 1 : 2, D = 32 * NK, MT = select_m_tiles(D);
+    constexpr int PIECES = 2 * D * ES / 16, ROW = 2 * D * ES + 16;    // 16-byte pieces of a block's bounds; a block in LDS
+    constexpr int NP = (16 * PIECES + 255) / 256;                      // of a thread
+    __shared__ __align__(16) uint8_t s_bounds[2][16 * ROW];
     __shared__ uint32_t s_max[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, kq = lane >> 4;
     const int h = blockIdx.x % a.hkv, chunk = blockIdx.x / a.hkv % a.chunks;
-    const int G = a.hq / a.hkv, gl = a.group_log2, tile = 16 * MT >> gl;
+    const int G = a.hq / a.hkv, gl = a.group_log2, tile = 64 * MT >> gl;
     const SparseTile x = sparse_tile(blockIdx.x / a.hkv / a.chunks, tile, a.qsl, a.num_seqs);
     if (x.seq < 0 || x.row < 0) return;
     const int nt = min(min(tile, x.n - x.i), a.row0 + a.rows - x.row);        // rows of the tile within the launch
@@ -175,10 +196,11 @@ __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a)
     const int c0 = max(chunk * a.chunk, a.first), c1 = min((chunk + 1) * a.chunk, nv - a.last);
     if (c0 >= c1) return;
     const int32_t* const bt = a.bt + static_cast<int64_t>(x.seq) * a.maxb;
+    const int wave_tok = wave * (16 * MT >> gl);                       // the wave's first row of the tile
     uint4 qn[MT][NK], qp[MT][NK];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        const int r = 16 * m + col, tok = r >> gl, g = r & ((1 << gl) - 1);
+        const int r = 16 * m + col, tok = wave_tok + (r >> gl), g = r & ((1 << gl) - 1);
         const bool live = tok < nt && g < G;
         const uint16_t* src = a.q + (static_cast<int64_t>(x.row + tok) * a.hq + h * G + g) * D;
 #pragma unroll
@@ -187,26 +209,70 @@ __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a)
             split_signs(y, qn[m][i], qp[m][i]);
         }
     }
+    // the last rows of the sequence see every block that the others see: their workgroups
+    // alone take the bounds' magnitudes
+    const bool widest = x.row + nt == min(x.row - x.i + x.n, a.row0 + a.rows);
     u16x2 top = {0, 0};
-    for (int b0 = chunk * a.chunk + 16 * wave; b0 < c1; b0 += 64) {
-        const int j = b0 + col;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 next[NP];
+    auto usable = [&](int j) __attribute__((always_inline)) -> int32_t {
         int32_t b = -1;
         if (j >= c0 && j < c1) {
             b = bt[j];
             if (b >= a.num_blocks) b = -1;
         }
-        const uint8_t* src = b >= 0 ? static_cast<const uint8_t*>(a.kb) + (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES)
-                                    : reinterpret_cast<const uint8_t*>(g_gen_zero);
-        const int st = b >= 0 ? ES : 0;
+        return b;
+    };
+    auto load = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int i = threadIdx.x + 256 * p, blk = i / PIECES;
+            const int32_t b = blk < 16 ? usable(b0 + blk) : -1;
+            next[p] = u32x4{0, 0, 0, 0};
+            if (b >= 0)
+                next[p] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.kb) +
+                                                          (static_cast<int64_t>(b) * a.hkv + h) * (2 * D * ES) + (i - blk * PIECES) * 16);
+        }
+    };
+    auto store = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int i = threadIdx.x + 256 * p, blk = i / PIECES;
+            if (16 * PIECES % 256 == 0 || blk < 16) *reinterpret_cast<u32x4*>(s_bounds[buffer] + blk * ROW + (i - blk * PIECES) * 16) = next[p];
+        }
+    };
+    // where the lane's results go: row wave_tok + ((16 m + 4 kq) >> gl) for groups of 4 heads or more
+    const int64_t row_pitch = a.hkv * a.pitch;
+    uint32_t* const keys0 = a.keys + (static_cast<int64_t>(x.row - a.row0) * a.hkv + h) * a.pitch;
+    uint32_t* keys_m[MT];
+    uint32_t owns = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int tok = wave_tok + ((16 * m + 4 * kq) >> gl);
+        keys_m[m] = keys0 + tok * row_pitch;
+        if (gl >= 2 && tok < nt && x.row + tok >= a.row0 && (kq & ((1 << (gl - 2)) - 1)) == 0) owns |= 1u << m;
+    }
+    const bool full = 1 << gl == G;
+    const int first_tile = chunk * a.chunk;
+    load(first_tile);
+    store(0);
+    int buffer = 0;
+    for (int b0 = first_tile; b0 < c1; b0 += 16, buffer ^= 1) {
+        __syncthreads();                                               // this tile is there, the other's readers are done
+        if (b0 + 16 < c1) load(b0 + 16);
+        const int j = b0 + col;
+        const bool here = usable(j) >= 0;
         uint4 y[2 * NK];
 #pragma unroll
         for (int i = 0; i < 2 * NK; ++i)
-            y[i] = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(src + (32 * i + 8 * kq) * st));
+            y[i] = gen_to16<QKIND, KVKIND>(*reinterpret_cast<const raw_t*>(s_bounds[buffer] + col * ROW + (32 * i + 8 * kq) * ES));
+        if (widest) {
 #pragma unroll
-        for (int i = 0; i < 2 * NK; ++i) {
-            const uint32_t u[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+            for (int i = 0; i < 2 * NK; ++i) {
+                const uint32_t u[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+                for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+            }
         }
         gm_f32x4 acc[MT];
 #pragma unroll
@@ -222,36 +288,50 @@ __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a)
         const bool in = j >= c0 && j < c1;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            uint32_t key[4];
+            // a NaN among values that are added up shows in the sum
+            float v[4], w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) key[i] = ((4 * kq + i) & ((1 << gl) - 1)) < G ? order32(acc[m][i]) : 0;
-            // rows 4 kq + i of the tile's m-th 16: the heads of a row one after the other
-            auto put = [&](int tok, uint32_t k) __attribute__((always_inline)) {
-                const int t = x.row + tok;
-                if (in && tok < nt && t >= a.row0) a.keys[(static_cast<int64_t>(t - a.row0) * a.hkv + h) * a.pitch + j] = b >= 0 ? k : 0;
+            for (int i = 0; i < 4; ++i) v[i] = w[i] = acc[m][i];
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (((4 * kq + i) & ((1 << gl) - 1)) >= G) {
+                        v[i] = -INFINITY;
+                        w[i] = 0.f;
+                    }
+            }
+            if (gl >= 2) {
+                const float z = (w[0] + w[1]) + (w[2] + w[3]);
+                uint32_t key = order32(z != z ? z : fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+                if (gl >= 3) key = umax(key, __shfl_xor(key, 16));
+                if (gl >= 4) key = umax(key, __shfl_xor(key, 32));
+                if (in && (owns >> m & 1)) keys_m[m][j] = here ? key : 0;
+                continue;
+            }
+            // rows 4 kq + i of the tile's m-th 16, of one head or two
+            auto put = [&](int tok, uint32_t key) __attribute__((always_inline)) {
+                if (in && tok < nt && x.row + tok >= a.row0) keys0[tok * row_pitch + j] = here ? key : 0;
             };
             if (gl == 0) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) put(16 * m + 4 * kq + i, key[i]);
-            } else if (gl == 1) {
-                put(8 * m + 2 * kq, umax(key[0], key[1]));
-                put(8 * m + 2 * kq + 1, umax(key[2], key[3]));
+                for (int i = 0; i < 4; ++i) put(wave_tok + 16 * m + 4 * kq + i, order32(v[i]));
             } else {
-                uint32_t k = umax(umax(key[0], key[1]), umax(key[2], key[3]));
-                if (gl >= 3) k = umax(k, __shfl_xor(k, 16));
-                if (gl >= 4) k = umax(k, __shfl_xor(k, 32));
-                if ((kq & ((1 << (gl - 2)) - 1)) == 0) put((16 * m + 4 * kq) >> gl, k);
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float z = w[i] + w[i + 1];
+                    put(wave_tok + 8 * m + 2 * kq + i / 2, order32(z != z ? z : fmaxf(v[i], v[i + 1])));
+                }
             }
         }
+        if (b0 + 16 < c1) store(buffer ^ 1);
     }
-    uint32_t t16 = umax(top[0], top[1]);
-    for (int d = 1; d < 64; d <<= 1) t16 = umax(t16, __shfl_xor(t16, d));
+    uint32_t t16 = wave_umax(umax(top[0], top[1]));
     if (lane == 0) s_max[wave] = t16;
     __syncthreads();
     t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
-    const int t = x.row + static_cast<int>(threadIdx.x);
-    if (static_cast<int>(threadIdx.x) < nt && t >= a.row0)
-        a.kmax[(static_cast<int64_t>(t - a.row0) * a.hkv + h) * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
+    if (widest && threadIdx.x == 0)
+        a.kmax[(static_cast<int64_t>(x.row + nt - 1 - a.row0) * a.hkv + h) * a.chunks + chunk] =
+            to_f32<typename M::tag>(static_cast<uint16_t>(t16));
 }
 
 enum : uint8_t { OUT = 0, MID = 1, IN = 2 };
@@ -293,10 +373,6 @@ struct Team {
         return n;
     }
 };
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-    for (int x = 1; x < 64; x <<= 1) v = umax(v, __shfl_xor(v, x));
-    return v;
-}
 __device__ __forceinline__ int wave_count(bool p) { return __popcll(__builtin_amdgcn_ballot_w64(p)); }
 
 // The K-th largest key among those in the middle (there are K of them at least), by
@@ -391,6 +467,7 @@ struct Pick {
     const int32_t* bt;
     int32_t* sel;
     int unit, h, t, nv;
+    int widest;             // the sequence's last row of the launch
     int base, n;            // candidates: blocks base .. base + n - 1
     __device__ __forceinline__ bool usable(int j) const {
         const int32_t b = bt[j];
@@ -398,10 +475,10 @@ struct Pick {
     }
 };
 
-// f32 scores that are certainly above, or below, the K-th largest in 64 bits; th: the
-// K-th largest f32 score.  False where the bound is not finite.
+// A bound of the f32 scores' error; and the f32 scores that are certainly above, or below,
+// the K-th largest in 64 bits, th being the K-th largest in f32 (false: not finite).
 template <int QKIND, int NT>
-__device__ __forceinline__ bool select_window(const Pick& p, float th, Team& team, float& over, float& under) {
+__device__ __forceinline__ float select_error(const Pick& p, Team& team) {
     using tag = typename GenMfma<QKIND>::tag;
     const SelectArgs& a = p.a;
     const int lane = threadIdx.x & 63, G = a.hq / a.hkv;
@@ -418,12 +495,15 @@ __device__ __forceinline__ bool select_window(const Pick& p, float th, Team& tea
         qs = fmaxf(qs, wave_sum(s));
     }
     float km = 0.f;
+    const float* const kmax = a.kmax + (static_cast<int64_t>(p.widest - a.row0) * a.hkv + p.h) * a.chunks;
     const int ch0 = p.base / a.chunk, ch1 = (p.base + p.n - 1) / a.chunk;
-    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, a.kmax[static_cast<int64_t>(p.unit) * a.chunks + i]);
+    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, kmax[i]);
     qs = __uint_as_float(team.max(__float_as_uint(qs)));
     km = wave_max(km);
     const float all = qs * km;                               // 0: every score is exactly 0
-    const float eps = all == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * all + 0x1p-100f;
+    return all == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * all + 0x1p-100f;
+}
+__device__ __forceinline__ bool select_window(float th, float eps, float& over, float& under) {
     const float slack = 2.f * eps + (eps > 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
     over = th + slack;
     under = th - slack;
@@ -432,7 +512,7 @@ __device__ __forceinline__ bool select_window(const Pick& p, float th, Team& tea
 
 // The list of a row of any number of candidates, whatever their scores: keys and states in memory.
 template <int QKIND, int KVKIND, int NT>
-__device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h, int t, int seq, int nv, uint32_t* s_team) {
+__device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h, int t, int seq, int nv, int widest, uint32_t* s_team) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Team team = {s_team, NT / 64, wave, 0};
@@ -440,7 +520,7 @@ __device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h
     int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
     const bool all = nv <= a.k;
     const int base = a.first, n = all ? 0 : nv - a.last - a.first;
-    const Pick p = {a, bt, sel, unit, h, t, nv, base, n};
+    const Pick p = {a, bt, sel, unit, h, t, nv, widest, base, n};
     auto usable = [&](int j) __attribute__((always_inline)) { return p.usable(j); };
     uint32_t* const keys = a.keys + unit * a.pitch + base;
     uint8_t* const state = a.state + unit * a.pitch + base;
@@ -474,7 +554,7 @@ __device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h
                 if (!any_odd) {
                     float over, under;
                     const float th = unorder32(kth_largest<NT>(keys, state, n, K, team));
-                    again = !select_window<QKIND, NT>(p, th, team, over, under);
+                    again = !select_window(th, select_error<QKIND, NT>(p, team), over, under);
                     if (!again) {
                         int in = 0, mid = 0;
                         for (int i0 = 0; i0 < n; i0 += NT) {
@@ -569,11 +649,23 @@ __device__ __forceinline__ double exact_score16(const Pick& p, int j) {
                 s += x > y ? x : y;                          // finite: the window was
             }
         }
-        for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x);
+        s = row_sum16(s);
         nan |= s != s;
         best = s > best ? s : best;
     }
     return nan ? __builtin_nan("") : best;
+}
+
+// f(0) .. f(n - 1) with constant arguments, n <= MOST: one branch leaves the rest out
+// (a condition each made a taken branch each: 1250 candidates of one row and 8 heads 16.5 us, 13.0 so)
+template <int J, int MOST, class F>
+__device__ __forceinline__ void upto(int n, F& f) {
+    if constexpr (J < MOST) {
+        if (J < n) {
+            f(J);
+            upto<J + 1, MOST>(n, f);
+        }
+    }
 }
 
 // A workgroup per (row, kv head), each thread KPT candidates in registers: wave w the
@@ -593,10 +685,12 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
     if (row.seq < 0) return;
     const int nv = visible_blocks(a, row);
     const int n = nv - a.last - a.first;
+    // where its chunks' largest bounds are: with the last row where rows went in tiles
+    const int widest = a.tiles ? min(t - row.i + row.n, a.row0 + a.rows) - 1 : t;
     auto quickly = [&]() __attribute__((always_inline)) -> bool {
         Team team = {s_team, NW, wave, 0};
         const Pick p = {a, a.bt + static_cast<int64_t>(row.seq) * a.maxb, a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k,
-                        unit, h, t, nv, a.first, n};
+                        unit, h, t, nv, widest, a.first, n};
         const uint64_t below = (uint64_t(1) << lane) - 1;
 
         const uint32_t* const keys = a.keys + unit * a.pitch + p.base;
@@ -606,11 +700,8 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
         bool odd = false;
 #pragma unroll
         for (int j = 0; j < KPT; ++j) key[j] = j < kpw && i0 + 64 * j < n ? keys[i0 + 64 * j] : 0;
-        auto each = [&](auto f) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < KPT; ++j)
-                if (j < kpw) f(j);
-        };
+        const float eps = select_error<QKIND, NT>(p, team);              // its loads go with the keys'
+        auto each = [&](auto f) __attribute__((always_inline)) { upto<0, KPT>(kpw, f); };
         // the forced blocks, by every wave for itself
         int nf = 0, nl = 0;
         for (int x = 0; x < a.first; x += 64) nf += wave_count(x + lane < a.first && p.usable(x + lane));
@@ -659,7 +750,7 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
                 }
             }
             float over = 0.f, under = 0.f;
-            if (!slow) slow = !select_window<QKIND, NT>(p, unorder32(th), team, over, under);
+            if (!slow) slow = !select_window(unorder32(th), eps, over, under);
             if (!slow) {
                 over_key = order32(over);
                 under_key = order32(under);
@@ -752,7 +843,7 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
         return true;
     };
     if (nv > a.k && n <= NT * KPT && quickly()) return;
-    pick_slowly<QKIND, KVKIND, NT>(a, unit, h, t, row.seq, nv, s_team);
+    pick_slowly<QKIND, KVKIND, NT>(a, unit, h, t, row.seq, nv, widest, s_team);
 }
 
 template <int QKIND, int KVKIND>
@@ -760,7 +851,7 @@ int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
     const int64_t units = static_cast<int64_t>(a.rows) * a.hkv;
     if (a.chunks > 0) {
         if (tiles) {
-            const int tile = 16 * select_m_tiles(a.d) >> a.group_log2;
+            const int tile = 64 * select_m_tiles(a.d) >> a.group_log2;
             const int64_t count = (static_cast<int64_t>(a.row0) + a.rows + tile - 1) / tile + a.num_seqs;
             const dim3 grid(static_cast<unsigned>(count * a.hkv * a.chunks));
             switch (a.d / 32) {
@@ -770,7 +861,7 @@ int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
 #undef RLLM_SCORE
             }
         } else {
-            const dim3 grid(static_cast<unsigned>(units * a.chunks));
+            const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.rows) * a.chunks));
             switch (a.d / 32) {
 #define RLLM_SCORE(N) \
     case N: hipLaunchKernelGGL((select_score_kernel<QKIND, KVKIND, N>), grid, dim3(256), 0, st, a); break;
@@ -784,13 +875,15 @@ int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
     // a wave a row where rows are many and short enough, else four
     if (units >= 2048 && a.maxb <= 64 * 32)
         hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 64, 32>), dim3(static_cast<unsigned>(units)), dim3(64), 0, st, a);
+    else if (a.maxb <= 256 * 8)
+        hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256, 8>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256, 32>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
     return launch_status();
 }
 
 constexpr int64_t SELECT_SLAB = int64_t(1) << 30;    // bytes of scratch of one pair of launches (a row's, where that is more)
-constexpr int64_t SELECT_CHUNK_MIN = 64, SELECT_CHUNK_MAX = 512;
+constexpr int64_t SELECT_CHUNK_MIN = 16, SELECT_CHUNK_MAX = 512;
 
 // bytes of scratch of a row: never fewer for a wider table
 int64_t select_row_bytes(int64_t hkv, int64_t maxb, int64_t& pitch) {
@@ -833,15 +926,22 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     RLLM_CHECK_ARG(num_first >= 0 && num_last >= 1 && num_first <= num_selected && num_last <= num_selected - num_first);
     RLLM_CHECK_ARG(selected && query && k_bounds && seq_lens && (block_tables || max_num_blocks_per_seq == 0));
     RLLM_CHECK_ARG(aligned_to(query, 16) && aligned_to(k_bounds, 16));
+    const int64_t group = num_q_heads / num_kv_heads;
+    const bool tiles = query_start_loc && group <= 16 && num_rows >= 2 * num_seqs;
     int64_t pitch = 0, need = 0, slab = num_rows, chunk = SELECT_CHUNK_MIN, chunks = 0;
     if (max_num_blocks_per_seq > num_selected) {       // else every list is the whole sequence
         const int64_t row_bytes = select_row_bytes(num_kv_heads, max_num_blocks_per_seq, pitch);
         need = select_bytes(num_rows, row_bytes);
         slab = need / row_bytes;
-        // enough workgroups to fill the card, and not many more
-        while (chunk < SELECT_CHUNK_MAX && slab * num_kv_heads * ((max_num_blocks_per_seq + chunk - 1) / chunk) > 4096) chunk *= 2;
+        // Row by row, small chunks keep a block's heads together in time and fill the card
+        // with few rows (64 rows of 250-2000 blocks: 16 blocks 72 us, 64 92, 128 109); a tile
+        // of rows loads its queries for each chunk (704 rows: 32 blocks 79 us, 64 60, 128 67).
+        // Not many more workgroups than it takes.
+        chunk = tiles ? 64 : SELECT_CHUNK_MIN;
+        while (chunk < SELECT_CHUNK_MAX && slab * ((max_num_blocks_per_seq + chunk - 1) / chunk) > 32768) chunk *= 2;
         chunks = (max_num_blocks_per_seq + chunk - 1) / chunk;
-        if (slab > INT32_MAX / (num_kv_heads * chunks)) slab = INT32_MAX / (num_kv_heads * chunks);
+        if (slab > INT32_MAX / (num_kv_heads * chunks)) slab = INT32_MAX / (num_kv_heads * chunks);   // workgroups of a launch
+        if (tiles) RLLM_CHECK_ARG((num_rows + num_seqs) * num_kv_heads * chunks <= INT32_MAX);
     }
     WorkspaceHold hold;
     void* ws = workspace;
@@ -873,10 +973,8 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     a.chunks = static_cast<int32_t>(chunks);
     a.num_blocks = num_blocks;
     a.pitch = pitch;
-    const int64_t group = num_q_heads / num_kv_heads;
+    a.tiles = tiles;
     while ((1 << a.group_log2) < group) ++a.group_log2;
-    const bool tiles = query_start_loc && group <= 16 && num_rows >= 2 * num_seqs;
-    if (tiles) RLLM_CHECK_ARG((num_rows + num_seqs) * num_kv_heads * chunks <= INT32_MAX);
     const hipStream_t st = as_stream(stream);
     for (int64_t r = 0; r < num_rows; r += slab) {
         a.row0 = static_cast<int32_t>(r);

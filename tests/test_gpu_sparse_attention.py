@@ -206,6 +206,45 @@ def test_a_key_that_is_not_finite_shows(dev):
     assert not out[1, :, 9].isfinite().any() and out[1, :, 10:].isfinite().all() and out[1, :, :9].isfinite().all()
 
 
+@pytest.mark.parametrize("kind,kv,hq,hkv,d,bs,k", [("bf16", "bf16", 32, 8, 128, 16, 64), ("f16", "e4m3", 20, 1, 64, 32, 40),
+                                                   ("f16", "f16", 2, 2, 256, 128, 9), ("bf16", "e5m2", 6, 2, 96, 16, 300)])
+def test_few_rows_over_several_workgroups(dev, kind, kv, hq, hkv, d, bs, k):
+    """Lists cut between workgroups that the last to end joins: the same bits every time, also where the lists are short; and as
+    a graph, with the stream's scratch and without."""
+    rng = np.random.default_rng(k)
+    lens = [k * bs + 40, 1, 5 * bs + 3, 0]
+    bt, nb = S.tables(rng, lens, bs)
+    kc, vc = pool(rng, nb, hkv, d, bs, kv)
+    q = queries(rng, 4, hq, d, kind)
+    sel = lists(rng, bt, lens, None, 4, hkv, bs, k)
+    out = check(dev, q, kc, vc, kind, kv, bt, lens, sel, bs, d ** -0.5)
+    ref = S.attend(q, S.values(kc, kv), S.values(vc, kv), bt, lens, None, sel, d ** -0.5, *(SCALES if kv in S.FP8 else (1.0, 1.0)))
+    args = [x.to(dev) for x in (q, kc, vc, bt, torch.tensor(lens, dtype=torch.int32), sel)]
+    kw = dict(k_scale=SCALES[0], v_scale=SCALES[1], **S.fp8(kv)) if kv in S.FP8 else {}
+    for _ in range(5):
+        assert torch.equal(ops.paged_sparse(*args, d ** -0.5, **kw), out)
+    with RawStream() as st:
+        torch.cuda.synchronize()
+        got = [torch.zeros_like(out) for _ in range(2)]
+        graphs = []
+        for g in got:                                           # first without scratch, then with
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=st):
+                ops.paged_sparse(*args, d ** -0.5, out=g, validate=False, **kw)
+            torch.cuda.synchronize()
+            ops.paged_sparse(*args, d ** -0.5, validate=False, stream=st, **kw)
+            torch.cuda.synchronize()
+        for _ in range(3):
+            for g, x in zip(graphs, got):
+                x.fill_(float("nan"))
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+                S.check_attend(x, *ref, kind, d, k * bs, "replayed")
+            assert torch.equal(got[1], out)
+            assert torch.equal(ops.paged_sparse(*args, d ** -0.5, **kw), out)
+
+
 def test_whole_lists_match_the_dense_kernels(dev):
     rng = np.random.default_rng(33)
     lens = [500, 3, 999, 160]
@@ -297,6 +336,9 @@ def test_a_run_of_steps(dev, kind, kv):
         ops.paged_sparse(got[0], kc, vc, t, lt, got[1], d ** -0.5, out=got[2], validate=False, **kw)
 
     with RawStream() as st:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            step()                                              # the stream's scratch, as the default stream has it
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=st):

@@ -203,6 +203,30 @@ def test_append_without_q_and_step_by_step(dev):
         assert all(torch.equal(a, b) for a, b in zip(got[0], other))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("kv", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("scale", [1.0, 0.37, 2.0 ** -7])
+def test_every_16_bit_value_into_an_fp8_cache(dev, kind, kv, scale):
+    """All 65536 patterns as values, in both roundings; as keys unrotated (position 0)."""
+    x = torch.from_numpy(np.arange(65536, dtype=np.uint16).view(np.int16)).view(S.HALF[kind]).view(2048, 1, 32)
+    cos, sin = ops.rope_cache_tables(4, 32, 10000.0)
+    for nearest in (True, False):
+        n = 2048
+        bt = torch.arange(n, dtype=torch.int32)[:, None]        # a block for each token, the first of its sequence
+        kc, vc = (torch.full((n, 1, 32, 16), 9, dtype=torch.uint8, device=dev) for _ in range(2))
+        kb = ops.new_key_bounds(kc)
+        ops.rope_and_append(None, x.to(dev), x.to(dev), kc, vc, kb, bt.to(dev), torch.ones(n, dtype=torch.int32, device=dev),
+                            cos.to(dev), sin.to(dev), k_scale=scale, v_scale=scale, validate=False, **S.fp8(kv),
+                            fp8_rounding=FP8_ROUND_NEAREST_EVEN if nearest else FP8_ROUND_TOWARD_ZERO)
+        want = S.encode(x.float(), kv, scale, nearest)[:, 0]
+        assert torch.equal(vc[:, 0, :, 0].cpu(), want)
+        # rotation by 0 leaves a finite pair as it is, but for the sign of zeros
+        fine = torch.isfinite(x.float().view(n, 2, 16)).all(1).repeat(1, 2)
+        got, k = kc[:, 0, :, 0].cpu(), want.clone()
+        k[(k & 0x7F) == 0], got[(got & 0x7F) == 0] = 0, 0
+        assert torch.equal(got[fine], k[fine])
+
+
 def test_append_on_a_stream_and_replayed(dev):
     rng = np.random.default_rng(9)
     cos, sin = ops.rope_cache_tables(300, 64, 10000.0)
