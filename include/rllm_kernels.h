@@ -729,7 +729,9 @@ int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads
  * nothing to attend get zeros.  scale, k_scale and v_scale as rllm_paged_attention_decode_ex.
  * Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
  * and keys past the row are not looked at; a key or value that is attended and not finite makes the
- * outputs it reaches not finite. */
+ * outputs it reaches not finite.  Calls of few rows (rows * num_kv_heads at most 128) use a
+ * library-owned buffer per (device, stream), which graphs captured on one stream share; a capture
+ * on a stream that has none runs without (results within rounding). */
 int32_t rllm_paged_attention_sparse(void *output, const void *query, const void *key_cache,
                                     const void *value_cache, const int32_t *block_tables,
                                     const int32_t *seq_lens, const int32_t *query_start_loc,

@@ -634,12 +634,14 @@ int32_t launch_sparse(SparseArgs a, int64_t d, hipStream_t st) {
         int tile = 16;
         while (tile * G > 16) tile /= 2;
         const int64_t most = static_cast<int64_t>(tile) * a.k < a.maxb ? static_cast<int64_t>(tile) * a.k : a.maxb;
-        if (units >= 256 * tile && a.maxb <= waves * sa_stage_bytes(static_cast<int>(d)) / 2 - 2 && most <= SA_MAX_LIST) {
+        if (units >= 256 * tile && a.splits == 1 && a.maxb <= waves * sa_stage_bytes(static_cast<int>(d)) / 2 - 2 && most <= SA_MAX_LIST) {
             a.tile = tile;
             a.list = static_cast<int32_t>(most > a.k ? most : a.k);
         }
     }
     a.list = (a.list + 3) & ~3;
+    // long lists beside the windows of wide heads: fewer waves where the LDS of a CU ends
+    while (waves * sa_stage_bytes(static_cast<int>(d)) + a.list * 10 > 160 * 1024 - 256) waves /= 2;
     if (a.bs_log2 == 4) return launch_sparse_run<QKIND, KVKIND, 4>(a, d, waves, st);
     if (a.bs_log2 == 5) return launch_sparse_run<QKIND, KVKIND, 5>(a, d, waves, st);
     return launch_sparse_run<QKIND, KVKIND, 6>(a, d, waves, st);

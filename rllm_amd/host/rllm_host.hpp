@@ -542,6 +542,61 @@ inline Result<void> paged_attention_prefill_mxfp4(void* output, const void* quer
 }
 
 // ---------------------------------------------------------------------------
+// attention over selected cache blocks (additive entry points): key bounds
+// [num_blocks, num_kv_heads, 2, head_dim] of the cache's type beside each key cache
+// ---------------------------------------------------------------------------
+// first_positions null: all of each sequence
+inline Result<void> key_bounds(void* k_bounds, const void* key_cache, const int32_t* block_tables, const int32_t* seq_lens,
+                               int64_t num_seqs, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                               int64_t max_num_blocks_per_seq, int64_t num_blocks, DType kv_dtype, uintptr_t stream,
+                               const int32_t* first_positions = nullptr) {
+    return check(rllm_key_bounds(k_bounds, key_cache, block_tables, seq_lens, first_positions, num_seqs, num_kv_heads,
+                                 head_dim, block_size, max_num_blocks_per_seq, num_blocks, abi_dtype(kv_dtype), stream));
+}
+
+// q_out may equal q; query_start_loc null: one new token a sequence
+inline Result<void> rope_cache_append(void* q_out, const void* q, const void* k, const void* v, void* key_cache,
+                                      void* value_cache, void* k_bounds, const int32_t* block_tables,
+                                      const int32_t* seq_lens, const int32_t* query_start_loc, const float* cos_cache,
+                                      const float* sin_cache, int64_t num_seqs, int64_t num_tokens, int64_t num_q_heads,
+                                      int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                      int64_t max_num_blocks_per_seq, int64_t num_blocks, int64_t max_position,
+                                      DType dtype, DType kv_dtype, float k_scale, float v_scale, uintptr_t stream,
+                                      int32_t fp8_rounding = RLLM_FP8_ROUND_TOWARD_ZERO) {
+    return check(rllm_rope_cache_append(q_out, q, k, v, key_cache, value_cache, k_bounds, block_tables, seq_lens,
+                                        query_start_loc, cos_cache, sin_cache, num_seqs, num_tokens, num_q_heads,
+                                        num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks,
+                                        max_position, abi_dtype(dtype), abi_dtype(kv_dtype), k_scale, v_scale,
+                                        fp8_rounding, stream));
+}
+
+// workspace null: library-owned scratch
+inline Result<void> select_blocks(int32_t* selected, const void* query, const void* k_bounds, const int32_t* block_tables,
+                                  const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs,
+                                  int64_t num_rows, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                  int64_t block_size, int64_t max_num_blocks_per_seq, int64_t num_blocks,
+                                  int64_t num_selected, int64_t num_first, int64_t num_last, DType q_dtype, DType kv_dtype,
+                                  uintptr_t stream, void* workspace = nullptr, int64_t workspace_bytes = 0) {
+    return check(rllm_select_blocks(selected, query, k_bounds, block_tables, seq_lens, query_start_loc, num_seqs, num_rows,
+                                    num_q_heads, num_kv_heads, head_dim, block_size, max_num_blocks_per_seq, num_blocks,
+                                    num_selected, num_first, num_last, abi_dtype(q_dtype), abi_dtype(kv_dtype), workspace,
+                                    workspace_bytes, stream));
+}
+
+inline Result<void> paged_attention_sparse(void* output, const void* query, const void* key_cache, const void* value_cache,
+                                           const int32_t* block_tables, const int32_t* seq_lens,
+                                           const int32_t* query_start_loc, const int32_t* selected, int64_t num_seqs,
+                                           int64_t num_rows, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                           int64_t block_size, int64_t max_num_blocks_per_seq, int64_t num_blocks,
+                                           int64_t num_selected, float scale, DType q_dtype, DType kv_dtype, float k_scale,
+                                           float v_scale, uintptr_t stream) {
+    return check(rllm_paged_attention_sparse(output, query, key_cache, value_cache, block_tables, seq_lens,
+                                             query_start_loc, selected, num_seqs, num_rows, num_q_heads, num_kv_heads,
+                                             head_dim, block_size, max_num_blocks_per_seq, num_blocks, num_selected, scale,
+                                             abi_dtype(q_dtype), abi_dtype(kv_dtype), k_scale, v_scale, stream));
+}
+
+// ---------------------------------------------------------------------------
 // block lists: copy-on-write copies and swap records (additive entry points)
 // ---------------------------------------------------------------------------
 inline Result<void> cache_copy_blocks(const uint64_t* key_caches, const uint64_t* value_caches, int64_t num_layers,

@@ -245,6 +245,30 @@ def test_few_rows_over_several_workgroups(dev, kind, kv, hq, hkv, d, bs, k):
             assert torch.equal(ops.paged_sparse(*args, d ** -0.5, **kw), out)
 
 
+@pytest.mark.parametrize("d,hkv,rows", [(256, 1, 2), (128, 1, 2), (256, 4, 40), (128, 4, 40)])
+def test_the_longest_lists(dev, d, hkv, rows):
+    """4096 entries, beside the windows of wide heads; also as a graph on a stream without scratch."""
+    rng = np.random.default_rng(d + hkv)
+    lens = [70000, 30] + [400] * (rows - 2)
+    bt, nb = S.tables(rng, lens, 16)
+    kc, vc = pool(rng, nb, hkv, d, 16, "bf16")
+    q = queries(rng, rows, 2 * hkv, d, "bf16")
+    sel = lists(rng, bt, lens, None, rows, hkv, 16, 4096)
+    sel[0, 0] = torch.arange(4096) + 200
+    sel[0, -1, 4000:] = -1
+    out = check(dev, q, kc, vc, "bf16", "bf16", bt, lens, sel, 16, d ** -0.5)
+    args = [x.to(dev) for x in (q, kc, vc, bt, torch.tensor(lens, dtype=torch.int32), sel)]
+    with RawStream() as st:
+        torch.cuda.synchronize()
+        got = torch.zeros_like(out)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            ops.paged_sparse(*args, d ** -0.5, out=got, validate=False)
+        g.replay()
+        torch.cuda.synchronize()
+    assert ((got - out).float().abs() <= 2.0 ** -7 * out.float().abs() + 1e-6).all()
+
+
 def test_whole_lists_match_the_dense_kernels(dev):
     rng = np.random.default_rng(33)
     lens = [500, 3, 999, 160]

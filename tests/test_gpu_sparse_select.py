@@ -51,7 +51,8 @@ def test_decode_rows(dev, kind, kv, hq, hkv, d, bs):
 
 
 @pytest.mark.parametrize("kind,kv", [("bf16", "bf16"), ("f16", "f16"), ("f16", "e4m3")])
-@pytest.mark.parametrize("hq,hkv,d,bs", [(32, 8, 128, 16), (6, 2, 64, 32), (20, 1, 96, 16), (2, 2, 256, 16), (5, 1, 32, 64)])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(32, 8, 128, 16), (6, 2, 64, 32), (20, 1, 96, 16), (2, 2, 256, 16), (5, 1, 32, 64),
+                                         (4, 2, 160, 32), (16, 1, 224, 16), (9, 1, 192, 16)])
 def test_chunk_rows(dev, kind, kv, hq, hkv, d, bs):
     rng = np.random.default_rng(d * 3 + hq)
     lens, new = [30 * bs + 5, 90 * bs, 17, 11 * bs + 1, 300], [1, 37, 17, 0, 9]
@@ -184,6 +185,30 @@ def test_more_scratch_than_a_slab(dev):
     out = ops.select_blocks(q.to(dev), kb.to(dev), bt, torch.tensor(lens, dtype=torch.int32, device=dev), 16, 8, validate=False)
     ref = S.select(q, S.values(kb, "bf16"), small, lens, None, 16, 8, 1, 1)
     assert torch.equal(out.cpu(), ref)
+
+
+def test_a_chunk_with_more_scratch_than_a_slab(dev):
+    """The same for tiles of rows, cut by the parts' ends."""
+    rng = np.random.default_rng(22)
+    new, width = [901, 1, 1300, 40], 16384
+    lens = [1500, 2000, 1300, 900]
+    small, nb = S.tables(rng, lens, 16)
+    qsl = np.concatenate([[0], np.cumsum(new)]).tolist()
+    n = qsl[-1]
+    kb, q = key_like(rng, nb, 8, 32, "bf16"), queries(rng, n, 16, 32, "bf16")
+    assert n * 8 * width * 4 > ops.lib().rllm_select_blocks_workspace_size(n, 8, width)
+    bt = torch.full((4, width), -1, dtype=torch.int32, device=dev)
+    bt[:, :small.shape[1]] = small.to(dev)
+    out = ops.select_blocks(q.to(dev), kb.to(dev), bt, torch.tensor(lens, dtype=torch.int32, device=dev), 16, 8, validate=False,
+                            query_start_loc=torch.tensor(qsl, dtype=torch.int32, device=dev))
+    wide = out.cpu()
+    narrow = ops.select_blocks(q.to(dev), kb.to(dev), small.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), 16, 8,
+                               query_start_loc=torch.tensor(qsl, dtype=torch.int32, device=dev)).cpu()
+    assert torch.equal(wide, narrow)                            # every row; some of them against the formula
+    for t in list(range(0, n, 97)) + [900, 901, 902, n - 41, n - 1]:
+        s = int(np.searchsorted(qsl, t, side="right")) - 1
+        one = S.select(q[t:t + 1], S.values(kb, "bf16"), small[s:s + 1], [lens[s] - (qsl[s + 1] - 1 - t)], None, 16, 8, 1, 1)
+        assert torch.equal(wide[t:t + 1], one), t
 
 
 def test_workspace_of_the_largest_serves_the_smaller(dev):
