@@ -727,7 +727,7 @@ int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads
  * above, or any other lists: one ends at its first entry that is negative or not above the
  * one before it, and an entry past what the row sees attends nothing).  Rows with
  * nothing to attend get zeros.  scale, k_scale and v_scale as rllm_paged_attention_decode_ex.
- * Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
+ * output must not be query.  Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
  * and keys past the row are not looked at; a key or value that is attended and not finite makes the
  * outputs it reaches not finite.  Calls of few rows (rows * num_kv_heads at most 128) use a
  * library-owned buffer per (device, stream), which graphs captured on one stream share; a capture

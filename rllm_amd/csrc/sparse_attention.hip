@@ -28,6 +28,7 @@ int32_t rllm_paged_attention_sparse(void* output, const void* query, const void*
     RLLM_CHECK_ARG(query_start_loc || num_rows == num_seqs);
     RLLM_CHECK_ARG(num_selected >= 1 && num_selected <= RLLM_SELECT_MAX_BLOCKS);
     RLLM_CHECK_ARG(output && query && key_cache && value_cache && seq_lens && selected);
+    RLLM_CHECK_ARG(output != query);                   // a row may be computed again
     RLLM_CHECK_ARG(block_tables || max_num_blocks_per_seq == 0);
     for (const void* p : {static_cast<const void*>(output), query, key_cache, value_cache}) RLLM_CHECK_ARG(aligned_to(p, 16));
     const bool fp8 = kv_dtype == RLLM_DTYPE_FP8_E4M3 || kv_dtype == RLLM_DTYPE_FP8_E5M2;

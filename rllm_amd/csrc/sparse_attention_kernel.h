@@ -23,7 +23,8 @@
 //                 LDS reads.
 // Loads that gave every lane the 8 x 8 tile it transposes itself read 16 bytes here
 // and there: one lane a clock, 13.5 bytes a clock and CU, whatever was in flight (64
-// rows on 128 blocks, head_dim 128, 103 us; 704 rows of two chunks on 64, 340).
+// rows on 128 blocks, head_dim 128, 103 us, 99 so, 5.4 TB/s; 704 rows of two chunks on 64,
+// 340, 148 so).
 // Weights enter as two 16-bit terms (generic_mfma.h).
 #pragma once
 
@@ -45,7 +46,7 @@ struct SparseArgs {
     int32_t num_seqs, rows, hq, hkv, bs_log2, maxb, k, head_groups;
     int32_t splits;             // workgroups of a unit, joined by the last to end
     int32_t* count;             // arrivals of a unit, 0 between calls
-    float* part;                // [unit][split][16 columns][head_dim + 2]: sum, max and sum of weights
+    float* part;                // [unit][split][16 columns][head_dim + 4]: sum, max, sum of weights, two unused
     int32_t tile, list;         // rows of a workgroup (1, or 16 / heads of a kv head), and the entries its list has room for
     int64_t num_blocks;
     float s_scale, v_scale;     // s_scale: scale * k_scale * log2(e)
@@ -170,7 +171,6 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
     const int lane_half = FP8 ? 0 : (lane_chunk & 1) * 16;
     constexpr int groups_log2 = RUN - 4;                        // 16-token groups of a block within a window
 
-
     // the rows: t .. t + nt - 1 of sequence seq, the first at position pos
     int t, nt, seq, pos;
     if (a.tile > 1) {
@@ -189,109 +189,108 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
         nt = 1;
         pos = x.pos;
     }
-    {
-        const int32_t* const bt = a.bt + static_cast<int64_t>(seq) * a.maxb;
-        const int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
-        const int64_t sel_row = static_cast<int64_t>(a.hkv) * a.k;
-        // a list ends at its first entry that is not above the one before it
-        auto ends = [&](int j, int before) __attribute__((always_inline)) { return j <= before || j < 0; };
-        auto seen = [&](int j, int p) __attribute__((always_inline)) { return j < a.maxb && j <= p >> bs_log2; };
-        auto block_of = [&](int j) __attribute__((always_inline)) -> int {
-            const int b = bt[j];
-            return b >= 0 && b < a.num_blocks ? b : -1;
-        };
-        if (threadIdx.x == 0) s_used = 0;
-        if (threadIdx.x < 16) s_end[threadIdx.x] = a.k;
-        if (nt == 1) {
-            __syncthreads();
-            int most = 0;
-            for (int i0 = 0; i0 < a.k; i0 += threads) {
-                const int i = i0 + threadIdx.x;
-                const int j = i < a.k ? sel[i] : 0x7fffffff, before = i > 0 && i < a.k ? sel[i - 1] : -1;
-                const uint64_t over = __builtin_amdgcn_ballot_w64(ends(j, before));
-                if (over && lane == 0) atomicMin(&s_end[0], i + __builtin_ctzll(over));
-                if (i < a.k) {
-                    const int b = !ends(j, before) && seen(j, pos) ? block_of(j) : -1;
-                    s_list[i] = b;
-                    s_num[i] = j;
-                    s_mask[i] = 1;
-                    if (b >= 0) most = i + 1;
-                }
+    const int32_t* const bt = a.bt + static_cast<int64_t>(seq) * a.maxb;
+    const int32_t* const sel = a.sel + (static_cast<int64_t>(t) * a.hkv + h) * a.k;
+    const int64_t sel_row = static_cast<int64_t>(a.hkv) * a.k;
+    // a list ends at its first entry that is not above the one before it
+    auto ends = [&](int j, int before) __attribute__((always_inline)) { return j <= before || j < 0; };
+    auto seen = [&](int j, int p) __attribute__((always_inline)) { return j < a.maxb && j <= p >> bs_log2; };
+    auto block_of = [&](int j) __attribute__((always_inline)) -> int {
+        const int b = bt[j];
+        return b >= 0 && b < a.num_blocks ? b : -1;
+    };
+    if (threadIdx.x == 0) s_used = 0;
+    if (threadIdx.x < 16) s_end[threadIdx.x] = a.k;
+    if (nt == 1) {
+        __syncthreads();
+        int most = 0;
+        for (int i0 = 0; i0 < a.k; i0 += threads) {
+            const int i = i0 + threadIdx.x;
+            const int j = i < a.k ? sel[i] : 0x7fffffff, before = i > 0 && i < a.k ? sel[i - 1] : -1;
+            const uint64_t over = __builtin_amdgcn_ballot_w64(ends(j, before));
+            if (over && lane == 0) atomicMin(&s_end[0], i + __builtin_ctzll(over));
+            if (i < a.k) {
+                const int b = !ends(j, before) && seen(j, pos) ? block_of(j) : -1;
+                s_list[i] = b;
+                s_num[i] = j;
+                s_mask[i] = 1;
+                if (b >= 0) most = i + 1;
             }
-            most = static_cast<int>(wave_umax(static_cast<uint32_t>(most)));
-            if (lane == 0 && most) atomicMax(&s_used, most);
-        } else {
-            // the union: a word of bits for every block of the sequence, where the windows will be
-            uint16_t* const s_bits = reinterpret_cast<uint16_t*>(lds);
-            const int nv = pos + nt - 1 < 0 ? 0 : min(((pos + nt - 1) >> bs_log2) + 1, a.maxb);
-            const int words = (nv + 1) >> 1;
-            for (int i = threadIdx.x; i < words; i += threads) reinterpret_cast<uint32_t*>(s_bits)[i] = 0;
-            __syncthreads();
-            auto entry = [&](int i, int& x, int& e, int& before) __attribute__((always_inline)) -> int {
-                x = i / a.k;
-                e = i - x * a.k;
-                before = e ? sel[x * sel_row + e - 1] : -1;
-                return sel[x * sel_row + e];
-            };
-            int x, e, before;
-            for (int i = threadIdx.x; i < nt * a.k; i += threads)
-                if (ends(entry(i, x, e, before), before)) atomicMin(&s_end[x], e);
-            __syncthreads();
-            for (int i = threadIdx.x; i < nt * a.k; i += threads) {
-                const int j = entry(i, x, e, before);
-                if (e < s_end[x] && seen(j, pos + x)) atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (j >> 1), 1u << (16 * (j & 1) + x));
-            }
-            __syncthreads();
-            // wave w the w-th part of the blocks
-            const int part = (nv + 64 * waves - 1) / (64 * waves) * 64;
-            const int j0 = wave * part, j1 = min(j0 + part, nv);
-            int n = 0;
-            for (int j = j0; j < j1; j += 64) n += __popcll(__builtin_amdgcn_ballot_w64(j + lane < j1 && s_bits[j + lane]));
-            if (lane == 0) s_count[wave] = n;
-            __syncthreads();
-            int at = 0;
-            for (int w = 0; w < waves; ++w) {
-                if (w == wave) n = at;
-                at += s_count[w];
-            }
-            for (int j = j0; j < j1; j += 64) {
-                const uint32_t bits = j + lane < j1 ? s_bits[j + lane] : 0;
-                const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0);
-                if (bits) {
-                    const int i = n + __popcll(m & ((uint64_t(1) << lane) - 1));
-                    s_list[i] = block_of(j + lane);
-                    s_num[i] = j + lane;
-                    s_mask[i] = static_cast<uint16_t>(bits);
-                }
-                n += __popcll(m);
-            }
-            if (threadIdx.x == 0) s_used = at;
         }
-
-        // queries, negated where the scale is negative (exact), so that the running max is
-        // over c * s with c >= 0
-        const bool col_live = col_row < nt && col_head < G && (a.tile > 1 || col_head < 16 * hg + 16);
-        const int64_t out_row = static_cast<int64_t>(t + col_row) * a.hq + h * G + col_head;
-        uint4 qreg[NK];
-        {
-            const uint32_t flip = a.s_scale < 0.f ? 0x80008000u : 0u;
-            const uint16_t* qrow = a.q + out_row * D;
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (col_live) {
-                    const uint2 y = *reinterpret_cast<const uint2*>(qrow + 32 * k + 4 * q4);
-                    const uint2 z = *reinterpret_cast<const uint2*>(qrow + 32 * k + 16 + 4 * q4);
-                    x = make_uint4(y.x, y.y, z.x, z.y);
-                }
-                qreg[k] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-            }
+        most = static_cast<int>(wave_umax(static_cast<uint32_t>(most)));
+        if (lane == 0 && most) atomicMax(&s_used, most);
+    } else {
+        // the union: a word of bits for every block of the sequence, where the windows will be
+        uint16_t* const s_bits = reinterpret_cast<uint16_t*>(lds);
+        const int nv = pos + nt - 1 < 0 ? 0 : min(((pos + nt - 1) >> bs_log2) + 1, a.maxb);
+        const int words = (nv + 1) >> 1;
+        for (int i = threadIdx.x; i < words; i += threads) reinterpret_cast<uint32_t*>(s_bits)[i] = 0;
+        __syncthreads();
+        auto entry = [&](int i, int& x, int& e, int& before) __attribute__((always_inline)) -> int {
+            x = i / a.k;
+            e = i - x * a.k;
+            before = e ? sel[x * sel_row + e - 1] : -1;
+            return sel[x * sel_row + e];
+        };
+        int x, e, before;
+        for (int i = threadIdx.x; i < nt * a.k; i += threads)
+            if (ends(entry(i, x, e, before), before)) atomicMin(&s_end[x], e);
+        __syncthreads();
+        for (int i = threadIdx.x; i < nt * a.k; i += threads) {
+            const int j = entry(i, x, e, before);
+            if (e < s_end[x] && seen(j, pos + x)) atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (j >> 1), 1u << (16 * (j & 1) + x));
         }
         __syncthreads();
-        const int used = __builtin_amdgcn_readfirstlane(nt == 1 ? min(s_used, s_end[0]) : s_used);
-        const int end = used << bs_log2;                        // tokens of the list
-        const int first_own = pos < 0 ? 0 : pos >> bs_log2;     // blocks before it every row sees whole
-        const int last_seen = pos + nt;                         // keys of the sequence that the last row sees
+        // wave w the w-th part of the blocks
+        const int part = (nv + 64 * waves - 1) / (64 * waves) * 64;
+        const int j0 = wave * part, j1 = min(j0 + part, nv);
+        int n = 0;
+        for (int j = j0; j < j1; j += 64) n += __popcll(__builtin_amdgcn_ballot_w64(j + lane < j1 && s_bits[j + lane]));
+        if (lane == 0) s_count[wave] = n;
+        __syncthreads();
+        int at = 0;
+        for (int w = 0; w < waves; ++w) {
+            if (w == wave) n = at;
+            at += s_count[w];
+        }
+        for (int j = j0; j < j1; j += 64) {
+            const uint32_t bits = j + lane < j1 ? s_bits[j + lane] : 0;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0);
+            if (bits) {
+                const int i = n + __popcll(m & ((uint64_t(1) << lane) - 1));
+                s_list[i] = block_of(j + lane);
+                s_num[i] = j + lane;
+                s_mask[i] = static_cast<uint16_t>(bits);
+            }
+            n += __popcll(m);
+        }
+        if (threadIdx.x == 0) s_used = at;
+    }
+
+    // queries, negated where the scale is negative (exact), so that the running max is
+    // over c * s with c >= 0
+    const bool col_live = col_row < nt && col_head < G && (a.tile > 1 || col_head < 16 * hg + 16);
+    const int64_t out_row = static_cast<int64_t>(t + col_row) * a.hq + h * G + col_head;
+    uint4 qreg[NK];
+    {
+        const uint32_t flip = a.s_scale < 0.f ? 0x80008000u : 0u;
+        const uint16_t* qrow = a.q + out_row * D;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (col_live) {
+                const uint2 y = *reinterpret_cast<const uint2*>(qrow + 32 * k + 4 * q4);
+                const uint2 z = *reinterpret_cast<const uint2*>(qrow + 32 * k + 16 + 4 * q4);
+                x = make_uint4(y.x, y.y, z.x, z.y);
+            }
+            qreg[k] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+        }
+    }
+    __syncthreads();
+    const int used = __builtin_amdgcn_readfirstlane(nt == 1 ? min(s_used, s_end[0]) : s_used);
+    const int end = used << bs_log2;                        // tokens of the list
+    const int first_own = pos < 0 ? 0 : pos >> bs_log2;     // blocks before it every row sees whole
+    const int last_seen = pos + nt;                         // keys of the sequence that the last row sees
 
     sa_u32x4 kbuf[NL], vbuf[NL];
     // entries of the window at token w, one a lane: cache blocks, numbers, masks
@@ -540,7 +539,10 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
             make_uint2(M::pack2(v[0], v[1]), M::pack2(v[2], v[3]));
     }
     if (a.splits > 1) {
-        // the last workgroup of the unit joins its parts, in their order
+        // The last workgroup of the unit joins its parts, in their order.  Each wave's parts
+        // have left the CU before the arrival that releases them to the other XCDs.
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (threadIdx.x == 0) {
             const int before = __hip_atomic_fetch_add(a.count + part_unit, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
@@ -583,7 +585,6 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
     if (nt > 1 && __syncthreads_or(bad))
         for (int x = 0; x < nt; ++x)
             for (int g = wave; g < G; g += waves) sparse_one<QKIND, KVKIND>(a, t + x, h, g, seq, pos + x, D, bs_log2);
-    }
 }
 
 template <int QKIND, int KVKIND, int RUN>
@@ -606,7 +607,7 @@ int32_t launch_sparse(SparseArgs a, int64_t d, hipStream_t st) {
     int waves = 4;
     // Few units: a CU draws some 13 bytes a clock from memory however much it asks for,
     // so a unit goes to several (1 row on 64 blocks, 8 kv heads, head_dim 128: one
-    // workgroup of 8 waves 13.5 us).  A capture on a stream without scratch does without.
+    // workgroup of 8 waves 13.5 us, 8 of 2 waves 9.6).  A capture on a stream without scratch does without.
     a.splits = 1;
     const int64_t windows = ((static_cast<int64_t>(a.k) << a.bs_log2) + SA_WIN - 1) / SA_WIN;
     if (units <= 128 && windows > 2) {
@@ -625,8 +626,8 @@ int32_t launch_sparse(SparseArgs a, int64_t d, hipStream_t st) {
         }
     }
     // tiles: in a chunk of several rows a sequence, where heads leave columns free, tiles
-    // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 -> 156 us),
-    // the blocks' bits fit where the windows go, and the union of the lists beside it
+    // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 us by
+    // single rows, 148 in tiles), the blocks' bits fit where the windows go, and the union of the lists beside it
     const int64_t G = a.hq / a.hkv;
     a.tile = 1;
     a.list = a.k;

@@ -73,7 +73,7 @@ constexpr int select_m_tiles(int d) { return d > 128 ? 2 : 4; }   // 16-row tile
 // hi.  Each lane loads 8 channels of its column's block, the operand as it stands.
 // Bound by HBM: the bounds are read once a row.  The heads of a block lie in a run, so
 // the waves of a workgroup read whole runs between them (64 rows of 250-2000 blocks, 8 kv
-// heads, head_dim 128: 84 us where a workgroup kept to one head).
+// heads, head_dim 128: 72 us, 4.0 TB/s; 84 where a workgroup kept to one head).
 template <int QKIND, int KVKIND, int NK>
 __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
     using M = GenMfma<QKIND>;
@@ -525,100 +525,100 @@ __device__ __forceinline__ void pick_slowly(const SelectArgs& a, int unit, int h
     uint32_t* const keys = a.keys + unit * a.pitch + base;
     uint8_t* const state = a.state + unit * a.pitch + base;
     __syncthreads();
-        int K = 0, ties = 0;
-        if (!all) {
-            int c = 0, f = 0;
-            for (int i0 = 0; i0 < a.first + a.last; i0 += NT) {
-                const int i = i0 + threadIdx.x;
-                f += wave_count(i < a.first + a.last && usable(i < a.first ? i : nv - a.last + (i - a.first)));
-            }
-            bool odd = false;
-            for (int i0 = 0; i0 < n; i0 += NT) {
-                const int i = i0 + threadIdx.x;
-                uint32_t key = 0;
-                if (i < n) {
-                    key = keys[i];
-                    state[i] = key ? MID : OUT;
-                }
-                const float x = unorder32(key);
-                odd |= key && !gen_finite(x);
-                c += wave_count(key != 0);
-            }
-            K = a.k - team.sum(f);
-            const int eligible = team.sum(c);
-            if (eligible <= K) {
-                ties = K;          // the whole middle goes in
-            } else if (K > 0) {
-                const bool any_odd = team.max(__builtin_amdgcn_ballot_w64(odd) != 0) != 0;
-                bool again = any_odd;
-                if (!any_odd) {
-                    float over, under;
-                    const float th = unorder32(kth_largest<NT>(keys, state, n, K, team));
-                    again = !select_window(th, select_error<QKIND, NT>(p, team), over, under);
-                    if (!again) {
-                        int in = 0, mid = 0;
-                        for (int i0 = 0; i0 < n; i0 += NT) {
-                            const int i = i0 + threadIdx.x;
-                            const bool was = i < n && state[i] == MID;
-                            const float x = was ? unorder32(keys[i]) : 0.f;
-                            const bool is_in = was && x > over, is_mid = was && x >= under && x <= over;
-                            if (was) state[i] = is_in ? IN : is_mid ? MID : OUT;
-                            in += wave_count(is_in);
-                            mid += wave_count(is_mid);
-                        }
-                        K -= team.sum(in);
-                        again = team.sum(mid) > K;
-                    }
-                }
-                ties = K;
-                if (again) {
-                    // the middle once more in 64 bits: upper half, and where that is equal the lower
-                    for (int half = 0; half < 2; ++half) {
-                        __syncthreads();
-                        int mid = 0;
-                        for (int i0 = 64 * wave; i0 < n; i0 += NT) {
-                            uint64_t m = __builtin_amdgcn_ballot_w64(i0 + lane < n && state[i0 + lane] == MID);
-                            mid += __popcll(m);
-                            for (; m; m &= m - 1) {
-                                const int i = i0 + __builtin_ctzll(m);
-                                const uint64_t key = order64(exact_score<QKIND, KVKIND>(a, t, h, bt[base + i]));
-                                if (lane == 0) keys[i] = static_cast<uint32_t>(half ? key : key >> 32);
-                            }
-                        }
-                        if (team.sum(mid) <= ties) break;
-                        __syncthreads();
-                        ties = settle<NT>(keys, state, n, ties, team);
-                    }
-                }
-            }
-            __syncthreads();
+    int K = 0, ties = 0;
+    if (!all) {
+        int c = 0, f = 0;
+        for (int i0 = 0; i0 < a.first + a.last; i0 += NT) {
+            const int i = i0 + threadIdx.x;
+            f += wave_count(i < a.first + a.last && usable(i < a.first ? i : nv - a.last + (i - a.first)));
         }
-        // the list, in the blocks' order; of the middle the first `ties`
-        int out = 0, mids = 0;
-        const int total = nv;
-        for (int j0 = 0; j0 < total && out < a.k; j0 += NT) {
-            const int j = j0 + threadIdx.x;
-            bool in = false, mid = false;
-            if (j < total) {
-                if (all || j < a.first || j >= nv - a.last) in = usable(j);
-                else {
-                    in = state[j - base] == IN;
-                    mid = state[j - base] == MID;
+        bool odd = false;
+        for (int i0 = 0; i0 < n; i0 += NT) {
+            const int i = i0 + threadIdx.x;
+            uint32_t key = 0;
+            if (i < n) {
+                key = keys[i];
+                state[i] = key ? MID : OUT;
+            }
+            const float x = unorder32(key);
+            odd |= key && !gen_finite(x);
+            c += wave_count(key != 0);
+        }
+        K = a.k - team.sum(f);
+        const int eligible = team.sum(c);
+        if (eligible <= K) {
+            ties = K;          // the whole middle goes in
+        } else if (K > 0) {
+            const bool any_odd = team.max(__builtin_amdgcn_ballot_w64(odd) != 0) != 0;
+            bool again = any_odd;
+            if (!any_odd) {
+                float over, under;
+                const float th = unorder32(kth_largest<NT>(keys, state, n, K, team));
+                again = !select_window(th, select_error<QKIND, NT>(p, team), over, under);
+                if (!again) {
+                    int in = 0, mid = 0;
+                    for (int i0 = 0; i0 < n; i0 += NT) {
+                        const int i = i0 + threadIdx.x;
+                        const bool was = i < n && state[i] == MID;
+                        const float x = was ? unorder32(keys[i]) : 0.f;
+                        const bool is_in = was && x > over, is_mid = was && x >= under && x <= over;
+                        if (was) state[i] = is_in ? IN : is_mid ? MID : OUT;
+                        in += wave_count(is_in);
+                        mid += wave_count(is_mid);
+                    }
+                    K -= team.sum(in);
+                    again = team.sum(mid) > K;
                 }
             }
-            int before;
-            const uint64_t below = (uint64_t(1) << lane) - 1;
-            const uint64_t mm = __builtin_amdgcn_ballot_w64(mid);
-            const int found = team.scan(__popcll(mm), before);
-            in |= mid && mids + before + __popcll(mm & below) < ties;
-            mids += found;
-            const uint64_t mi = __builtin_amdgcn_ballot_w64(in);
-            const int taken = team.scan(__popcll(mi), before);
-            const int at = out + before + __popcll(mi & below);
-            if (in && at < a.k) sel[at] = j;
-            out += taken;
+            ties = K;
+            if (again) {
+                // the middle once more in 64 bits: upper half, and where that is equal the lower
+                for (int half = 0; half < 2; ++half) {
+                    __syncthreads();
+                    int mid = 0;
+                    for (int i0 = 64 * wave; i0 < n; i0 += NT) {
+                        uint64_t m = __builtin_amdgcn_ballot_w64(i0 + lane < n && state[i0 + lane] == MID);
+                        mid += __popcll(m);
+                        for (; m; m &= m - 1) {
+                            const int i = i0 + __builtin_ctzll(m);
+                            const uint64_t key = order64(exact_score<QKIND, KVKIND>(a, t, h, bt[base + i]));
+                            if (lane == 0) keys[i] = static_cast<uint32_t>(half ? key : key >> 32);
+                        }
+                    }
+                    if (team.sum(mid) <= ties) break;
+                    __syncthreads();
+                    ties = settle<NT>(keys, state, n, ties, team);
+                }
+            }
         }
-        for (int i = out + threadIdx.x; i < a.k; i += NT) sel[i] = -1;
+        __syncthreads();
+    }
+    // the list, in the blocks' order; of the middle the first `ties`
+    int out = 0, mids = 0;
+    const int total = nv;
+    for (int j0 = 0; j0 < total && out < a.k; j0 += NT) {
+        const int j = j0 + threadIdx.x;
+        bool in = false, mid = false;
+        if (j < total) {
+            if (all || j < a.first || j >= nv - a.last) in = usable(j);
+            else {
+                in = state[j - base] == IN;
+                mid = state[j - base] == MID;
+            }
+        }
+        int before;
+        const uint64_t below = (uint64_t(1) << lane) - 1;
+        const uint64_t mm = __builtin_amdgcn_ballot_w64(mid);
+        const int found = team.scan(__popcll(mm), before);
+        in |= mid && mids + before + __popcll(mm & below) < ties;
+        mids += found;
+        const uint64_t mi = __builtin_amdgcn_ballot_w64(in);
+        const int taken = team.scan(__popcll(mi), before);
+        const int at = out + before + __popcll(mi & below);
+        if (in && at < a.k) sel[at] = j;
+        out += taken;
+    }
+    for (int i = out + threadIdx.x; i < a.k; i += NT) sel[i] = -1;
 }
 
 // Scores of up to four candidates at once, 16 lanes each: the lane's own, in all 16.
@@ -670,7 +670,8 @@ __device__ __forceinline__ void upto(int n, F& f) {
 
 // A workgroup per (row, kv head), each thread KPT candidates in registers: wave w the
 // w-th part of them, so that a list comes out in order.  Latency counts here: bits
-// that all keys share are not searched, and the search ends where K keys remain.
+// that all keys share are not searched, and the search ends where K keys remain (64 of 1250
+// blocks: 8 lists 12 us, 512 of 250-2000 18, 5632 of 1250-1650 58).
 template <int QKIND, int KVKIND, int NT, int KPT>
 __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
     constexpr int NW = NT / 64, REFINE = 64;
@@ -872,7 +873,8 @@ int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
         const int32_t rc = launch_status();
         if (rc) return rc;
     }
-    // a wave a row where rows are many and short enough, else four
+    // a wave a row where rows are many and short enough, else four (8 heads: 704 rows of 1250-1650 blocks
+    // 58 us by one wave, 69 by four; 64 rows of 250-2000 34 and 18; one of 1250 24 and 13)
     if (units >= 2048 && a.maxb <= 64 * 32)
         hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 64, 32>), dim3(static_cast<unsigned>(units)), dim3(64), 0, st, a);
     else if (a.maxb <= 256 * 8)
@@ -927,6 +929,8 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     RLLM_CHECK_ARG(selected && query && k_bounds && seq_lens && (block_tables || max_num_blocks_per_seq == 0));
     RLLM_CHECK_ARG(aligned_to(query, 16) && aligned_to(k_bounds, 16));
     const int64_t group = num_q_heads / num_kv_heads;
+    // several rows a sequence, one 16-row operand a group: rows share the bounds that they read
+    // (704 rows of 1250-1650 blocks, 32/8 heads, head_dim 128: 58 us, 536 row by row)
     const bool tiles = query_start_loc && group <= 16 && num_rows >= 2 * num_seqs;
     int64_t pitch = 0, need = 0, slab = num_rows, chunk = SELECT_CHUNK_MIN, chunks = 0;
     if (max_num_blocks_per_seq > num_selected) {       // else every list is the whole sequence

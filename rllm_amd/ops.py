@@ -700,7 +700,7 @@ def paged_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                  v_scale: float = 1.0, out: Optional[torch.Tensor] = None, validate: bool = True,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Attention of each query row over the keys it sees in the blocks that selected [num_rows, Hkv, n]
-    lists for it (as select_blocks returns them), through rllm_paged_attention_sparse."""
+    lists for it (as select_blocks returns them), through rllm_paged_attention_sparse.  ``out`` is not ``q``."""
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype:
         raise ValueError("q [*, Hq, D] and caches [nb, Hkv, D, bs] of equal shape and type required")
     rows, hq, d = q.shape
@@ -721,6 +721,8 @@ def paged_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError("out must be a contiguous tensor like q")
+    elif out.data_ptr() == q.data_ptr() and out.numel():
+        raise ValueError("out must not be q")
     _all_dense(q, k_cache, v_cache, block_tables, seq_lens, selected, out)
     if validate:
         _validate_rows(rows, block_tables, seq_lens, query_start_loc, nb, bs)

@@ -25,7 +25,7 @@ def select(L, sel=P, q=P, kb=P, bt=P, qsl=None, n=2, rows=2, hq=32, hkv=8, d=128
     return L.rllm_select_blocks(sel, q, kb, bt, P, qsl, n, rows, hq, hkv, d, bs, maxb, nb, k, first, last, dt, kv, ws, ws_bytes, 0)
 
 
-def attend(L, out=P, q=P, kc=P, sel=P, qsl=None, n=2, rows=2, hq=32, hkv=8, d=128, bs=16, maxb=40, nb=10, k=8, scale=0.1,
+def attend(L, out=2 * P, q=P, kc=P, sel=P, qsl=None, n=2, rows=2, hq=32, hkv=8, d=128, bs=16, maxb=40, nb=10, k=8, scale=0.1,
            dt=1, kv=1, ks=1.0, vs=1.0):
     return L.rllm_paged_attention_sparse(out, q, kc, P, P, P, qsl, sel, n, rows, hq, hkv, d, bs, maxb, nb, k, scale, dt, kv, ks,
                                          vs, 0)
@@ -62,7 +62,8 @@ def test_arguments_are_refused():
         assert select(L, **bad) == 1, bad
     for bad in (dict(out=None), dict(q=None), dict(kc=None), dict(sel=None), dict(rows=3), dict(hq=30), dict(k=0), dict(k=4097),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(kv=2, ks=float("nan")), dict(kv=2, vs=float("inf")),
-                dict(kv=2, ks=3e38, scale=10.0), dict(dt=0), dict(out=P + 8), dict(kc=P + 8), dict(rows=1 << 25, qsl=P)):
+                dict(kv=2, ks=3e38, scale=10.0), dict(dt=0), dict(out=P + 8), dict(kc=P + 8), dict(out=P),
+                dict(rows=1 << 25, qsl=P)):
         assert attend(L, **bad) == 1, bad
 
 
@@ -116,6 +117,8 @@ def test_the_front_end_names_what_is_wrong():
         ops.select_blocks(q, kb, bt, lens, 16, 2, out=sel)
     with pytest.raises(ValueError, match="selected"):
         ops.paged_sparse(q, kc, kc, bt, lens, sel[:2], 0.1)
+    with pytest.raises(ValueError, match="must not be q"):
+        ops.paged_sparse(q, kc, kc, bt, lens, sel, 0.1, out=q)
     with pytest.raises(ValueError, match="head_dim"):
         ops.paged_sparse(q[..., :32], kc, kc, bt, lens, sel, 0.1)
     with pytest.raises(ValueError, match="current GPU"):
