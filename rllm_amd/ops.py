@@ -614,32 +614,34 @@ def rope_and_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     tables say, and keeps the bounds of the blocks written, through rllm_rope_cache_append.  seq_lens count the
     new tokens; without query_start_loc each sequence has one.  Returns the rotated q (``q_out``, which
     may be ``q`` itself), or None when q is None."""
-    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4:
+    rows, cache, table, dtype, cache_dtype = k.shape, k_cache.shape, cos.shape, k.dtype, k_cache.dtype   # each read once
+    if len(rows) != 3 or v.shape != rows or len(cache) != 4:
         raise ValueError("k/v [num_tokens, Hkv, D] of one shape and caches [nb, Hkv, D, bs] required")
-    n, hkv, d = k.shape
-    nb, hkv2, d2, bs = k_cache.shape
-    if (hkv, d) != (hkv2, d2) or k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+    n, hkv, d = rows
+    nb, hkv2, d2, bs = cache
+    if hkv != hkv2 or d != d2 or v_cache.shape != cache or v_cache.dtype is not cache_dtype:
         raise ValueError("token rows do not match the cache layout")
-    dt = _TORCH_16.get(k.dtype)
-    if dt is None or v.dtype is not k.dtype:
+    dt = _TORCH_16.get(dtype)
+    if dt is None or v.dtype is not dtype:
         raise TypeError("k/v must be float16 or bfloat16")
     kv = _kv_code(k_cache, kv_dtype)
     if kv in (DTYPE_F16, DTYPE_BF16) and kv != dt:
         raise TypeError("16-bit cache dtype must equal the input dtype")
     _sparse_shape(d, bs)
-    _check_bounds(k_bounds, nb, hkv, d, k_cache.dtype)
+    _check_bounds(k_bounds, nb, hkv, d, cache_dtype)
     b = _check_rows(n, block_tables, seq_lens, query_start_loc, k.get_device())
-    if cos.dtype is not torch.float32 or sin.shape != cos.shape or sin.dtype is not cos.dtype \
-            or cos.dim() != 2 or cos.shape[1] != d // 2:
+    if cos.dtype is not torch.float32 or sin.shape != table or sin.dtype is not torch.float32 \
+            or len(table) != 2 or table[1] != d // 2:
         raise ValueError("cos/sin must be float32 [max_position, head_dim // 2]")
     hq = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype is not k.dtype:
+        queries = q.shape
+        if len(queries) != 3 or queries[0] != n or queries[2] != d or q.dtype is not dtype:
             raise ValueError("q must be [num_tokens, Hq, D] of the k dtype")
-        hq = q.shape[1]
+        hq = queries[1]
         if q_out is None:
             q_out = torch.empty_like(q)
-        elif q_out.shape != q.shape or q_out.dtype is not q.dtype:
+        elif q_out.shape != queries or q_out.dtype is not dtype:
             raise ValueError("q_out must match q")
         _all_dense(k, v, k_cache, v_cache, k_bounds, block_tables, seq_lens, cos, sin, q, q_out)
     elif q_out is not None:
@@ -648,9 +650,10 @@ def rope_and_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         _all_dense(k, v, k_cache, v_cache, k_bounds, block_tables, seq_lens, cos, sin)
     if validate:
         _validate_rows(n, block_tables, seq_lens, query_start_loc, nb, bs)
-    call("rllm_rope_cache_append", _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_bounds),
-         _ptr(block_tables), _ptr(seq_lens), _ptr(query_start_loc), _ptr(cos), _ptr(sin), b, n, hq, hkv, d, bs,
-         block_tables.shape[1], nb, cos.shape[0], dt, kv, k_scale, v_scale, fp8_rounding, _stream(stream))
+    call("rllm_rope_cache_append", _ptr(q_out), _ptr(q), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+         k_bounds.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), _ptr(query_start_loc), cos.data_ptr(),
+         sin.data_ptr(), b, n, hq, hkv, d, bs, block_tables.shape[1], nb, table[0], dt, kv, k_scale, v_scale, fp8_rounding,
+         _stream(stream))
     return q_out
 
 

@@ -245,6 +245,28 @@ def test_few_rows_over_several_workgroups(dev, kind, kv, hq, hkv, d, bs, k):
             assert torch.equal(ops.paged_sparse(*args, d ** -0.5, **kw), out)
 
 
+def test_few_rows_on_two_streams_at_once(dev):
+    """Each stream has scratch of its own: calls of different inputs that overlap give what they give alone."""
+    rng = np.random.default_rng(77)
+    lens = [2000, 1300]
+    bt, nb = S.tables(rng, lens, 16)
+    kc, vc = (x.to(dev) for x in pool(rng, nb, 8, 128, 16, "bf16"))
+    t, lt = bt.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    work = []
+    for _ in range(2):
+        q, sel = queries(rng, 2, 32, 128, "bf16").to(dev), lists(rng, bt, lens, None, 2, 8, 16, 60).to(dev)
+        want = ops.paged_sparse(q, kc, vc, t, lt, sel, 0.09)
+        work.append((q, sel, want, [torch.zeros_like(want) for _ in range(20)]))
+    torch.cuda.synchronize()
+    with RawStream() as a, RawStream() as b:
+        for i in range(20):
+            for st, (q, sel, _, outs) in zip((a, b), work):
+                ops.paged_sparse(q, kc, vc, t, lt, sel, 0.09, out=outs[i], validate=False, stream=st)
+        torch.cuda.synchronize()
+    for _, _, want, outs in work:
+        assert all(torch.equal(x, want) for x in outs)
+
+
 @pytest.mark.parametrize("d,hkv,rows", [(256, 1, 2), (128, 1, 2), (256, 4, 40), (128, 4, 40)])
 def test_the_longest_lists(dev, d, hkv, rows):
     """4096 entries, beside the windows of wide heads; also as a graph on a stream without scratch."""
