@@ -29,14 +29,13 @@
 #pragma once
 
 #include "sparse_blocks.h"
+#include "sparse_plan.h"
 #include "generic_mfma.h"
 #include "workspace.h"
 
 namespace rllm {
 
-constexpr int SA_WIN = 64;      // tokens of a wave's window: 4 groups of 16
-constexpr int SA_MAX_SPLITS = 8;
-constexpr int SA_MAX_LIST = RLLM_SELECT_MAX_BLOCKS;   // entries of a tile's list, 10 bytes of LDS each
+static_assert(SA_MAX_LIST >= RLLM_SELECT_MAX_BLOCKS, "a row's list fits");
 
 struct SparseArgs {
     uint16_t* out;
@@ -71,11 +70,6 @@ typedef short sa_i16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 sa_read_tr16(const uint8_t* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sa_i16x4*)(p)));
 }
-
-// two workgroups of four waves a CU up to head_dim 128; past it the registers of a window serve one
-constexpr int sa_max_waves(int d) { return d > 128 ? 4 : 8; }
-constexpr int sa_group_bytes(int d) { return d * 32 + 32; }     // of 16 tokens in LDS; the rest keeps groups on other banks
-constexpr int sa_stage_bytes(int d) { return SA_WIN / 16 * sa_group_bytes(d); }
 
 // One row and head by a wave, key by key: what a tile falls back to where its outputs are
 // not finite.
@@ -591,7 +585,7 @@ template <int QKIND, int KVKIND, int RUN>
 int32_t launch_sparse_run(const SparseArgs& a, int64_t d, int waves, hipStream_t st) {
     const int64_t tiles = a.tile > 1 ? (static_cast<int64_t>(a.rows) + a.tile - 1) / a.tile + a.num_seqs : a.rows;
     const dim3 grid(static_cast<unsigned>(tiles * a.hkv * a.head_groups * a.splits)), block(64 * waves);
-    const size_t lds = static_cast<size_t>(waves) * sa_stage_bytes(static_cast<int>(d)) + a.list * 10;
+    const size_t lds = static_cast<size_t>(waves) * sa_stage_bytes(static_cast<int>(d)) + a.list * SA_ENTRY;
     switch (d / 32) {
 #define RLLM_SPARSE(N) \
     case N: hipLaunchKernelGGL((sparse_attention_kernel<QKIND, KVKIND, N, RUN>), grid, block, lds, st, a); break;
@@ -603,46 +597,21 @@ int32_t launch_sparse_run(const SparseArgs& a, int64_t d, int waves, hipStream_t
 
 template <int QKIND, int KVKIND>
 int32_t launch_sparse(SparseArgs a, int64_t d, hipStream_t st) {
-    const int64_t units = static_cast<int64_t>(a.rows) * a.hkv * a.head_groups;
-    int waves = 4;
-    // Few units: a CU draws some 13 bytes a clock from memory however much it asks for,
-    // so a unit goes to several (1 row on 64 blocks, 8 kv heads, head_dim 128: one
-    // workgroup of 8 waves 13.5 us, 8 of 2 waves 9.6).  A capture on a stream without scratch does without.
-    a.splits = 1;
-    const int64_t windows = ((static_cast<int64_t>(a.k) << a.bs_log2) + SA_WIN - 1) / SA_WIN;
-    if (units <= 128 && windows > 2) {
-        int64_t splits = 256 / units < SA_MAX_SPLITS ? 256 / units : SA_MAX_SPLITS;
-        if (splits > (windows + 1) / 2) splits = (windows + 1) / 2;
-        void* ws = nullptr;
+    const SparseShape shape = {a.rows, a.num_seqs, a.hq, a.hkv, a.maxb, a.k, static_cast<int>(d), a.bs_log2, a.qsl != nullptr};
+    void* ws = nullptr;
+    if (sparse_few(shape)) {
         const int32_t rc = g_workspaces.get(reinterpret_cast<uintptr_t>(st), WS_SPARSE, 1024 + 256 * 16 * (d + 4) * 4, true, &ws);
         if (rc) return rc;
         if (ws) {
-            a.splits = static_cast<int32_t>(splits);
             a.count = static_cast<int32_t*>(ws);
             a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 1024);
-            waves = windows <= 2 * splits ? 2 : 4;
-        } else {
-            waves = sa_max_waves(static_cast<int>(d));
         }
     }
-    // tiles: in a chunk of several rows a sequence, where heads leave columns free, tiles
-    // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 us by
-    // single rows, 148 in tiles), the blocks' bits fit where the windows go, and the union of the lists beside it
-    const int64_t G = a.hq / a.hkv;
-    a.tile = 1;
-    a.list = a.k;
-    if (a.qsl && a.rows >= 2 * static_cast<int64_t>(a.num_seqs) && G <= 8) {
-        int tile = 16;
-        while (tile * G > 16) tile /= 2;
-        const int64_t most = static_cast<int64_t>(tile) * a.k < a.maxb ? static_cast<int64_t>(tile) * a.k : a.maxb;
-        if (units >= 256 * tile && a.splits == 1 && a.maxb <= waves * sa_stage_bytes(static_cast<int>(d)) / 2 - 2 && most <= SA_MAX_LIST) {
-            a.tile = tile;
-            a.list = static_cast<int32_t>(most > a.k ? most : a.k);
-        }
-    }
-    a.list = (a.list + 3) & ~3;
-    // long lists beside the windows of wide heads: fewer waves where the LDS of a CU ends
-    while (waves * sa_stage_bytes(static_cast<int>(d)) + a.list * 10 > 160 * 1024 - 256) waves /= 2;
+    const SparsePlan plan = sparse_plan(shape, ws != nullptr);
+    const int waves = plan.waves;
+    a.splits = plan.splits;
+    a.tile = plan.tile;
+    a.list = plan.list;
     if (a.bs_log2 == 4) return launch_sparse_run<QKIND, KVKIND, 4>(a, d, waves, st);
     if (a.bs_log2 == 5) return launch_sparse_run<QKIND, KVKIND, 5>(a, d, waves, st);
     return launch_sparse_run<QKIND, KVKIND, 6>(a, d, waves, st);

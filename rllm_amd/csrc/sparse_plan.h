@@ -1,0 +1,79 @@
+// How the attention over listed blocks (sparse_attention_kernel.h) is launched: waves and
+// rows of a workgroup and its LDS, from sizes alone.  Host code without HIP, so that it is
+// tested on the CPU over every head_dim, list and table width.
+#pragma once
+
+#include <stdint.h>
+
+namespace rllm {
+
+constexpr int SA_WIN = 64;      // tokens of a wave's window: 4 groups of 16
+constexpr int SA_MAX_SPLITS = 8;
+constexpr int SA_MAX_LIST = 4096;       // entries of a workgroup's list
+constexpr int SA_ENTRY = 10;            // bytes of LDS of an entry
+constexpr int SA_LDS = 160 * 1024 - 256;   // of a CU, beside the kernel's few static words
+
+// two workgroups of four waves a CU up to head_dim 128; past it the registers of a window serve one
+constexpr int sa_max_waves(int d) { return d > 128 ? 4 : 8; }
+constexpr int sa_group_bytes(int d) { return d * 32 + 32; }     // of 16 tokens in LDS; the rest keeps groups on other banks
+constexpr int sa_stage_bytes(int d) { return SA_WIN / 16 * sa_group_bytes(d); }
+
+struct SparseShape {
+    int64_t rows, num_seqs, hq, hkv, maxb, k;
+    int d, bs_log2;
+    bool chunk;                 // query_start_loc is given
+};
+struct SparsePlan {
+    int splits, waves;          // workgroups of a unit; waves of one
+    int tile, list;             // rows of a workgroup (1, or 16 / heads of a kv head), and the entries its list has room for
+};
+
+constexpr int64_t sparse_units(const SparseShape& s) { return s.rows * s.hkv * ((s.hq / s.hkv + 15) / 16); }
+constexpr int64_t sparse_windows(const SparseShape& s) { return ((s.k << s.bs_log2) + SA_WIN - 1) / SA_WIN; }
+
+// Few units: a CU draws some 13 bytes a clock from memory however much it asks for,
+// so a unit goes to several (1 row on 64 blocks, 8 kv heads, head_dim 128: one
+// workgroup of 8 waves 13.5 us, 8 of 2 waves 9.6).
+constexpr bool sparse_few(const SparseShape& s) { return sparse_units(s) <= 128 && sparse_windows(s) > 2; }
+
+constexpr int sa_padded(int list) { return (list + 3) & ~3; }
+// long lists beside the windows of wide heads: fewer waves where the LDS of a CU ends
+constexpr int sa_waves_beside(int waves, int d, int list) {
+    while (waves * sa_stage_bytes(d) + list * SA_ENTRY > SA_LDS) waves /= 2;
+    return waves;
+}
+
+// `scratch`: whether few units have some to join parts in; a capture on a stream that has none does without.
+inline SparsePlan sparse_plan(const SparseShape& s, bool scratch) {
+    SparsePlan p = {1, 4, 1, static_cast<int>(s.k)};
+    const int64_t units = sparse_units(s), windows = sparse_windows(s);
+    if (sparse_few(s)) {
+        if (scratch) {
+            int64_t splits = 256 / units < SA_MAX_SPLITS ? 256 / units : SA_MAX_SPLITS;
+            if (splits > (windows + 1) / 2) splits = (windows + 1) / 2;
+            p.splits = static_cast<int>(splits);
+            p.waves = windows <= 2 * splits ? 2 : 4;
+        } else {
+            p.waves = sa_max_waves(s.d);
+        }
+    }
+    p.waves = sa_waves_beside(p.waves, s.d, p.list = sa_padded(p.list));
+    // tiles: in a chunk of several rows a sequence, where heads leave columns free, tiles
+    // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 us by
+    // single rows, 148 in tiles), the union of the lists fits, and the blocks' bits fit where the
+    // windows of the waves go that are left beside it
+    const int64_t G = s.hq / s.hkv;
+    if (s.chunk && s.rows >= 2 * s.num_seqs && G <= 8 && p.splits == 1) {
+        int tile = 16;
+        while (tile * G > 16) tile /= 2;
+        const int64_t most = tile * s.k < s.maxb ? tile * s.k : s.maxb;
+        if (units >= 256 * tile && most <= SA_MAX_LIST) {
+            const int list = sa_padded(static_cast<int>(most > s.k ? most : s.k));
+            const int waves = sa_waves_beside(4, s.d, list);
+            if (4 * ((s.maxb + 1) / 2) <= waves * sa_stage_bytes(s.d)) p = {1, waves, tile, list};
+        }
+    }
+    return p;
+}
+
+}  // namespace rllm
