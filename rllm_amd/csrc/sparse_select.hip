@@ -475,7 +475,7 @@ struct Pick {
     }
 };
 
-// A bound of the f32 scores' error; and the f32 scores that are certainly above, or below,
+// A bound of the f32 scores' error (not finite: none is known); and the f32 scores that are certainly above, or below,
 // the K-th largest in 64 bits, th being the K-th largest in f32 (false: not finite).
 template <int QKIND, int NT>
 __device__ __forceinline__ float select_error(const Pick& p, Team& team) {
@@ -494,17 +494,19 @@ __device__ __forceinline__ float select_error(const Pick& p, Team& team) {
         }
         qs = fmaxf(qs, wave_sum(s));
     }
-    float km = 0.f;
+    // A chunk's largest may be of a block that this row does not see (rows of a tile share them).  NaN lies above
+    // infinity as bits do, and says, as that does, that the others' is not known.
+    uint32_t top = 0;
     const float* const kmax = a.kmax + (static_cast<int64_t>(p.widest - a.row0) * a.hkv + p.h) * a.chunks;
     const int ch0 = p.base / a.chunk, ch1 = (p.base + p.n - 1) / a.chunk;
-    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, kmax[i]);
+    for (int i = ch0 + lane; i <= ch1; i += 64) top = umax(top, __float_as_uint(kmax[i]));
     qs = __uint_as_float(team.max(__float_as_uint(qs)));
-    km = wave_max(km);
+    const float km = __uint_as_float(wave_umax(top));
     const float all = qs * km;                               // 0: every score is exactly 0
     return all == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * all + 0x1p-100f;
 }
 __device__ __forceinline__ bool select_window(float th, float eps, float& over, float& under) {
-    const float slack = 2.f * eps + (eps > 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
+    const float slack = 2.f * eps + (eps != 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
     over = th + slack;
     under = th - slack;
     return gen_finite(over) && gen_finite(under);

@@ -7,6 +7,7 @@ import torch
 import sparse_ref as S
 from gpu_util import log_case
 from rllm_amd import ops
+from test_gpu_sparse_select import check, key_like, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,77 @@ def test_tiles_under_wide_tables(dev, kind, kv, hq, hkv, d, k, width, n):
     S.check_attend(out, ref, mag, spread, kind, d, 16 * k)
     left = ref[:, 0, 0].isnan()
     assert (out.cpu()[left] == 3.0).all() and int(left.sum()) == n - sum(new)
+
+# ---------------------------------------------------------------------------
+# selection: rows of a chunk in tiles
+# ---------------------------------------------------------------------------
+
+GROUPS = [(2, 2), (4, 2), (3, 1), (8, 2), (9, 1), (16, 1)]      # heads of a group: 1, 2, 3, 4, 9, 16
+
+
+def chunks_of(rng, hq, hkv, blocks=70, bs=16):
+    """Lengths and new tokens of two sequences, two tiles of rows at least each (64 * 4 (row, head) pairs a tile, heads of a group
+    as a power of two); (lens, query_start_loc, rows, table, blocks in the pool)."""
+    tile = 256 // (1 << (hq // hkv - 1).bit_length())
+    new = [2 * tile + 3, tile + 1]
+    lens = [max(blocks * bs, new[0]) - 2, blocks * bs // 2 + new[1]]
+    bt, nb = S.tables(rng, lens, bs)
+    return lens, [1, 1 + new[0], 1 + sum(new)], sum(new) + 4, bt, nb
+
+
+def bounds_that_nearly_tie(rng, nb, hkv, d, kind):
+    """Scores that differ by far less than an f32 sum's rounding: + 6400 - 6400 + a little, for queries as near_tie_queries has
+    them."""
+    kb = np.broadcast_to(rng.standard_normal(d) * 0.1, (nb, hkv, 2, d)).copy()
+    kb[..., 0], kb[..., 1] = 100.0, -100.0
+    kb[..., 2] = rng.permutation(nb)[:, None, None] * 2.0 ** -9
+    return torch.from_numpy(kb).to(S.HALF[kind])
+
+
+def near_tie_queries(rng, n, hq, d, kind):
+    q = normal(rng, n, hq, d).to(S.HALF[kind])
+    q[..., 0], q[..., 1], q[..., 2] = 64.0, 64.0, 2.0 ** -10
+    return q
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_near_ties_before_a_block_that_is_not_finite(dev, hq, hkv):
+    """NaN or an infinity in a block that only the last rows see (and that stands among the first candidates' 64 blocks): the rows
+    before it are still the 64-bit scores'."""
+    rng = np.random.default_rng(hq + 200)
+    tile = 256 // (1 << (hq // hkv - 1).bit_length())
+    new = max(2 * tile + 3, 16 * 16)
+    lens, qsl, n = [max(62 * 16, new + 16 * 20) - 2, 500], [1, 1 + new, 1 + new + 40], new + 45
+    bt, nb = S.tables(rng, lens, 16)
+    q = near_tie_queries(rng, n, hq, 64, "bf16")
+    late = (lens[0] - 1) // 16 - 2
+    assert (lens[0] - new) // 16 + 8 < late < 64
+    for bad in (float("nan"), -float("nan"), float("inf")):
+        kb = bounds_that_nearly_tie(rng, nb, hkv, 64, "bf16")
+        kb[int(bt[0, late]), :, 1, 9] = bad
+        for k in (3, 12):
+            check(dev, q, kb, "bf16", bt, lens, 16, k, 1, 1, qsl, what=f"a late {bad}")
+
+
+@pytest.mark.parametrize("hq", [8, 24])
+def test_select_near_ties_over_several_slabs(dev, hq):
+    """Near ties and a late NaN in a call that works through its rows in parts: as under a narrow table, and by the formula."""
+    rng = np.random.default_rng(hq + 900)
+    hkv, width, new = 8, 16384, [901, 1, 1300, 40]
+    lens = [1500, 2000, 1300, 900]
+    small, nb = S.tables(rng, lens, 16)
+    qsl = np.concatenate([[0], np.cumsum(new)]).tolist()
+    n = qsl[-1]
+    kb, q = bounds_that_nearly_tie(rng, nb, hkv, 32, "bf16"), near_tie_queries(rng, n, hq, 32, "bf16")
+    kb[int(small[2, 60]), :, 1, 9] = float("nan")
+    assert n * hkv * width * 4 > ops.lib().rllm_select_blocks_workspace_size(n, hkv, width)
+    bt = torch.full((4, width), -1, dtype=torch.int32, device=dev)
+    bt[:, :small.shape[1]] = small.to(dev)
+    args = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (lens, qsl)]
+    wide, narrow = (ops.select_blocks(q.to(dev), kb.to(dev), t, args[0], 16, 8, validate=False, query_start_loc=args[1]).cpu()
+                    for t in (bt, small.to(dev)))
+    assert torch.equal(wide, narrow)
+    for t in list(range(0, n, 53)) + [900, 901, 902, 1524, 1525, 1526, 1527, n - 41, n - 1]:
+        s = int(np.searchsorted(qsl, t, side="right")) - 1
+        one = S.select(q[t:t + 1], S.values(kb, "bf16"), small[s:s + 1], [lens[s] - (qsl[s + 1] - 1 - t)], None, 16, 8, 1, 1)
+        assert torch.equal(wide[t:t + 1], one), t
