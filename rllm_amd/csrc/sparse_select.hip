@@ -502,8 +502,8 @@ __device__ __forceinline__ float select_error(const Pick& p, Team& team) {
     for (int i = ch0 + lane; i <= ch1; i += 64) top = umax(top, __float_as_uint(kmax[i]));
     qs = __uint_as_float(team.max(__float_as_uint(qs)));
     const float km = __uint_as_float(wave_umax(top));
-    const float all = qs * km;                               // 0: every score is exactly 0
-    return all == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * all + 0x1p-100f;
+    // either 0: every score is exactly 0.  The product of both may be below f32's range, as the scores may: 2^-100 stands for those
+    return qs == 0.f || km == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * (qs * km) + 0x1p-100f;
 }
 __device__ __forceinline__ bool select_window(float th, float eps, float& over, float& under) {
     const float slack = 2.f * eps + (eps != 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);

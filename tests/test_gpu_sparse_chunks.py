@@ -106,6 +106,19 @@ def test_select_near_ties_before_a_block_that_is_not_finite(dev, hq, hkv):
             check(dev, q, kb, "bf16", bt, lens, 16, k, 1, 1, qsl, what=f"a late {bad}")
 
 
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+@pytest.mark.parametrize("queries_by,bounds_by", [(-20, -120), (-40, -120), (-60, -100), (-126, -126), (60, -130), (-130, 100)])
+def test_select_scores_below_f32(dev, hq, hkv, queries_by, bounds_by):
+    """Scores below f32's range, subnormal bf16 queries and bounds: a chunk, and its last rows as decode rows."""
+    rng = np.random.default_rng(hq + 400)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    kb = key_like(rng, nb, hkv, 64, "bf16") * 2.0 ** bounds_by
+    q = queries(rng, n, hq, 64, "bf16") * 2.0 ** queries_by
+    assert bool(kb.any()) and bool(q.any())
+    check(dev, q, kb, "bf16", bt, lens, 16, 10, 1, 1, qsl, what=f"2^{queries_by} by 2^{bounds_by}")
+    check(dev, q[:2], kb, "bf16", bt, lens, 16, 10, 1, 1, what=f"2^{queries_by} by 2^{bounds_by}, a row a sequence")
+
+
 @pytest.mark.parametrize("hq", [8, 24])
 def test_select_near_ties_over_several_slabs(dev, hq):
     """Near ties and a late NaN in a call that works through its rows in parts: as under a narrow table, and by the formula."""
