@@ -88,6 +88,34 @@ def near_tie_queries(rng, n, hq, d, kind):
 
 
 @pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_ties(dev, hq, hkv):
+    rng = np.random.default_rng(hq)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    q, kb = queries(rng, n, hq, 64, "bf16"), key_like(rng, nb, hkv, 64, "bf16")
+    kb[bt[0, 5:60:3].long()] = kb[int(bt[0, 7])].clone()
+    check(dev, q, kb, "bf16", bt, lens, 16, 9, 1, 1, qsl, what="some alike")
+    check(dev, torch.zeros_like(q), kb, "bf16", bt, lens, 16, 9, 0, 1, qsl, what="zero queries")
+    kb[:] = kb[3].clone()
+    check(dev, q, kb, "bf16", bt, lens, 16, 9, 1, 2, qsl, what="all alike")
+    check(dev, q, torch.zeros_like(kb), "bf16", bt, lens, 16, 9, 0, 1, qsl, what="zero bounds")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_scores_that_f32_cannot_tell_apart(dev, kind, hq, hkv):
+    rng = np.random.default_rng(hq + 100)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    q, kb = near_tie_queries(rng, n, hq, 64, kind), bounds_that_nearly_tie(rng, nb, hkv, 64, kind)
+    for k in (3, 20, 50):
+        check(dev, q, kb, kind, bt, lens, 16, k, 1, 1, qsl, what="near ties")
+    # 250 blocks: more between the border's two sides than are scored again at once
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv, 250)
+    n = 60
+    check(dev, near_tie_queries(rng, n, hq, 64, kind), bounds_that_nearly_tie(rng, nb, hkv, 64, kind), kind, bt[:1], lens[:1], 16, 99,
+          1, 1, [1, 59], what="more near ties")
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
 def test_select_near_ties_before_a_block_that_is_not_finite(dev, hq, hkv):
     """NaN or an infinity in a block that only the last rows see (and that stands among the first candidates' 64 blocks): the rows
     before it are still the 64-bit scores'."""
@@ -107,6 +135,28 @@ def test_select_near_ties_before_a_block_that_is_not_finite(dev, hq, hkv):
 
 
 @pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_values_that_are_not_finite(dev, hq, hkv):
+    rng = np.random.default_rng(hq + 300)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    kb = key_like(rng, nb, hkv, 64, "bf16")
+    nan, inf = float("nan"), float("inf")
+    kb[int(bt[0, 50]), :, 1, 5] = nan
+    kb[int(bt[0, 20]), :, 0, 5] = nan
+    kb[int(bt[0, 10]), :, 1, 7] = inf
+    kb[int(bt[0, 11]), :, 0, 7] = -inf
+    kb[int(bt[0, 12])], kb[int(bt[0, 13])] = inf, -inf
+    q = queries(rng, n, hq, 64, "bf16")
+    for k in (3, 6, 20):
+        check(dev, q, kb, "bf16", bt, lens, 16, k, 1, 1, qsl, what="non-finite bounds")
+    q[::3, hq - 1, 7] = 0.0
+    q[1::7, 0, 9] = nan
+    q[2::7, hq // 2, 9] = inf
+    check(dev, q, kb, "bf16", bt, lens, 16, 6, 1, 1, qsl, what="non-finite queries")
+    big = key_like(rng, nb, hkv, 64, "bf16") * 2.0 ** 126
+    check(dev, queries(rng, n, hq, 64, "bf16") * 64, big, "bf16", bt, lens, 16, 20, 1, 1, qsl, what="scores past f32")
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
 @pytest.mark.parametrize("queries_by,bounds_by", [(-20, -120), (-40, -120), (-60, -100), (-126, -126), (60, -130), (-130, 100)])
 def test_select_scores_below_f32(dev, hq, hkv, queries_by, bounds_by):
     """Scores below f32's range, subnormal bf16 queries and bounds: a chunk, and its last rows as decode rows."""
@@ -117,6 +167,55 @@ def test_select_scores_below_f32(dev, hq, hkv, queries_by, bounds_by):
     assert bool(kb.any()) and bool(q.any())
     check(dev, q, kb, "bf16", bt, lens, 16, 10, 1, 1, qsl, what=f"2^{queries_by} by 2^{bounds_by}")
     check(dev, q[:2], kb, "bf16", bt, lens, 16, 10, 1, 1, what=f"2^{queries_by} by 2^{bounds_by}, a row a sequence")
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_f16_and_e5m2_subnormals(dev, hq, hkv):
+    rng = np.random.default_rng(hq + 500)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    for kv in ("f16", "e5m2"):
+        x = normal(rng, nb, hkv, 2, 64).sort(2).values * 2.0 ** -16
+        q = queries(rng, n, hq, 64, "f16")
+        check(dev, q, S.store(x, kv), kv, bt, lens, 16, 12, 1, 1, qsl, what="subnormal bounds")
+        check(dev, q * 2.0 ** -14, S.store(x * 2.0 ** 17, kv), kv, bt, lens, 16, 12, 1, 1, qsl, what="subnormal queries")
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_select_unused_entries(dev, hq, hkv):
+    rng = np.random.default_rng(hq + 600)
+    lens, qsl, n, bt, nb = chunks_of(rng, hq, hkv)
+    kb, q = key_like(rng, nb, hkv, 64, "bf16"), queries(rng, n, hq, 64, "bf16")
+    bt[0, rng.permutation(70)[:50]] = -1
+    bt[0, 3], bt[0, 40], bt[1, 0] = nb, 1 << 30, -7
+    for k in (4, 9, 30):
+        check(dev, q, kb, "bf16", bt, lens, 16, k, 2, 2, qsl)
+    check(dev, q, kb, "bf16", bt[:, :25].contiguous(), lens, 16, 6, 1, 1, qsl, what="a table narrower than the lengths")
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (16, 1)])
+def test_select_more_blocks_than_registers_hold(dev, hq, hkv):
+    rng = np.random.default_rng(hq + 700)
+    blocks, n = 8192 + 300, 40
+    lens, qsl = [blocks * 16 - 3, 60], [0, n - 6, n - 4]
+    bt, nb = S.tables(rng, lens, 16)
+    q, kb = queries(rng, n, hq, 32, "bf16"), key_like(rng, nb, hkv, 32, "bf16")
+    check(dev, q, kb, "bf16", bt, lens, 16, 100, 1, 2, qsl)
+    check(dev, near_tie_queries(rng, n, hq, 32, "bf16"), bounds_that_nearly_tie(rng, nb, hkv, 32, "bf16"), "bf16", bt, lens, 16, 100, 1,
+          2, qsl, what="near ties")
+    kb[int(bt[0, 8200]), 0, 1, 3] = float("nan")
+    check(dev, q, kb, "bf16", bt, lens, 16, 100, 1, 2, qsl, what="NaN")
+
+
+def test_select_lists_of_one_wave_each(dev):
+    """2048 lists and more, of up to 2047 blocks: every register of a lane."""
+    rng = np.random.default_rng(800)
+    hq, hkv, n = 8, 8, 262
+    lens, qsl = [2047 * 16 - 1, 1000 * 16, 33], [0, 200, 258, 260]
+    bt, nb = S.tables(rng, lens, 16)
+    q, kb = queries(rng, n, hq, 32, "bf16"), key_like(rng, nb, hkv, 32, "bf16")
+    check(dev, q, kb, "bf16", bt, lens, 16, 64, 1, 2, qsl)
+    check(dev, near_tie_queries(rng, n, hq, 32, "bf16"), bounds_that_nearly_tie(rng, nb, hkv, 32, "bf16"), "bf16", bt, lens, 16, 64, 1,
+          2, qsl, what="near ties")
 
 
 @pytest.mark.parametrize("hq", [8, 24])
