@@ -1,11 +1,80 @@
-// How the attention over listed blocks (sparse_attention_kernel.h) is launched: waves and
-// rows of a workgroup and its LDS, from sizes alone.  Host code without HIP, so that it is
-// tested on the CPU over every head_dim, list and table width.
+// How the selection (sparse_select.hip) and the attention over listed blocks
+// (sparse_attention_kernel.h) are launched: rows of a launch and of a workgroup, its waves
+// and LDS, from sizes alone.  Host code without HIP, so that it is tested on the CPU over
+// every head_dim, list and table width.
 #pragma once
 
 #include <stdint.h>
 
 namespace rllm {
+
+constexpr int64_t MAX_WORKGROUPS = ((int64_t(1) << 32) - 1) / 256;   // of a launch, of 256 threads each
+
+// ---------------------------------------------------------------------------
+// selection
+// ---------------------------------------------------------------------------
+
+constexpr int64_t SELECT_SLAB = int64_t(1) << 30;    // bytes of scratch of one pair of launches (a row's, where that is more)
+constexpr int64_t SELECT_CHUNK_MIN = 16, SELECT_CHUNK_MAX = 512;
+constexpr int select_m_tiles(int64_t d) { return d > 128 ? 2 : 4; }   // 16-row tiles of a wave, in a chunk
+
+// bytes of scratch of a row: never fewer for a wider table
+inline int64_t select_row_bytes(int64_t hkv, int64_t maxb, int64_t& pitch) {
+    pitch = (maxb + SELECT_CHUNK_MAX - 1) / SELECT_CHUNK_MAX * SELECT_CHUNK_MAX;
+    return hkv * (pitch * 4 + pitch / SELECT_CHUNK_MIN * 4 + pitch);
+}
+inline int64_t select_bytes(int64_t num_rows, int64_t row_bytes) {
+    const int64_t slab = row_bytes > SELECT_SLAB ? row_bytes : SELECT_SLAB;
+    return row_bytes == 0 ? 0 : num_rows <= slab / row_bytes ? num_rows * row_bytes : slab;   // (the product may pass 64 bits)
+}
+
+struct SelectPlan {
+    int64_t pitch, need, slab;  // keys of a list in scratch; bytes of it; rows of a pair of launches
+    int64_t chunk, chunks;      // blocks of a scoring workgroup, and such parts of a table (0: nothing is scored)
+    bool tiles;                 // rows are scored in tiles
+    int group_log2;             // heads of a group, as a power of two, where they are
+};
+
+// tiles of a chunk's rows, up to a row of the call (each sequence's last may be cut short)
+inline int64_t select_tiles(int64_t rows, int64_t num_seqs, int64_t d, int group_log2) {
+    const int64_t tile = 64 * select_m_tiles(d) >> group_log2;
+    return (rows + tile - 1) / tile + num_seqs;
+}
+
+inline SelectPlan select_plan(int64_t num_rows, int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d, int64_t maxb, int64_t k,
+                              bool chunk) {
+    SelectPlan p = {0, 0, num_rows, SELECT_CHUNK_MIN, 0, false, 0};
+    const int64_t group = hq / hkv;
+    while ((1 << p.group_log2) < group) ++p.group_log2;
+    // several rows a sequence, one 16-row operand a group: rows share the bounds that they read
+    // (704 rows of 1250-1650 blocks, 32/8 heads, head_dim 128: 58 us, 536 row by row)
+    p.tiles = chunk && group <= 16 && num_rows >= 2 * num_seqs;
+    p.slab = num_rows < MAX_WORKGROUPS / hkv ? num_rows : MAX_WORKGROUPS / hkv;      // a workgroup a list
+    if (maxb <= k) return p;                         // every list is the whole sequence
+    const int64_t row_bytes = select_row_bytes(hkv, maxb, p.pitch);
+    p.need = select_bytes(num_rows, row_bytes);
+    if (p.slab > p.need / row_bytes) p.slab = p.need / row_bytes;
+    // Row by row, small chunks keep a block's heads together in time and fill the card
+    // with few rows (64 rows of 250-2000 blocks: 16 blocks 72 us, 64 92, 128 109); a tile
+    // of rows loads its queries for each chunk (704 rows: 32 blocks 79 us, 64 58, 128 67).
+    // Not many more workgroups than it takes.
+    auto cut = [&] {
+        p.chunk = p.tiles ? 64 : SELECT_CHUNK_MIN;
+        while (p.chunk < SELECT_CHUNK_MAX && p.slab * ((maxb + p.chunk - 1) / p.chunk) > 32768) p.chunk *= 2;
+        p.chunks = (maxb + p.chunk - 1) / p.chunk;
+    };
+    cut();
+    if (p.tiles && select_tiles(num_rows, num_seqs, d, p.group_log2) > MAX_WORKGROUPS / (hkv * p.chunks)) {
+        p.tiles = false;
+        cut();
+    }
+    if (!p.tiles && p.slab > MAX_WORKGROUPS / p.chunks) p.slab = MAX_WORKGROUPS / p.chunks;
+    return p;
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
 
 constexpr int SA_WIN = 64;      // tokens of a wave's window: 4 groups of 16
 constexpr int SA_MAX_SPLITS = 8;

@@ -12,6 +12,7 @@
 // one below T - 2E is out, and only those between are scored again in f64.  Equal
 // ones go to the lowest block.
 #include "sparse_blocks.h"
+#include "sparse_plan.h"
 #include "generic_mfma.h"
 #include "workspace.h"
 
@@ -66,7 +67,6 @@ __device__ __forceinline__ void split_signs(const uint4& x, uint4& neg, uint4& p
     neg = make_uint4(n[0], n[1], n[2], n[3]);
     pos = make_uint4(p[0], p[1], p[2], p[3]);
 }
-constexpr int select_m_tiles(int d) { return d > 128 ? 2 : 4; }   // 16-row tiles of a wave, in a chunk
 
 // A workgroup per (row, chunk of its blocks), a wave kv heads w, w + 4, ..., 16 blocks at
 // a time: v_mfma_16x16x32, rows = heads, columns = blocks, k = channels of lo, then of
@@ -850,12 +850,11 @@ __global__ __launch_bounds__(NT) void select_pick_kernel(SelectArgs a) {
 }
 
 template <int QKIND, int KVKIND>
-int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
+int32_t launch_select(const SelectArgs& a, hipStream_t st) {
     const int64_t units = static_cast<int64_t>(a.rows) * a.hkv;
     if (a.chunks > 0) {
-        if (tiles) {
-            const int tile = 64 * select_m_tiles(a.d) >> a.group_log2;
-            const int64_t count = (static_cast<int64_t>(a.row0) + a.rows + tile - 1) / tile + a.num_seqs;
+        if (a.tiles) {
+            const int64_t count = select_tiles(static_cast<int64_t>(a.row0) + a.rows, a.num_seqs, a.d, a.group_log2);
             const dim3 grid(static_cast<unsigned>(count * a.hkv * a.chunks));
             switch (a.d / 32) {
 #define RLLM_SCORE(N) \
@@ -884,19 +883,6 @@ int32_t launch_select(const SelectArgs& a, bool tiles, hipStream_t st) {
     else
         hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 256, 32>), dim3(static_cast<unsigned>(units)), dim3(256), 0, st, a);
     return launch_status();
-}
-
-constexpr int64_t SELECT_SLAB = int64_t(1) << 30;    // bytes of scratch of one pair of launches (a row's, where that is more)
-constexpr int64_t SELECT_CHUNK_MIN = 16, SELECT_CHUNK_MAX = 512;
-
-// bytes of scratch of a row: never fewer for a wider table
-int64_t select_row_bytes(int64_t hkv, int64_t maxb, int64_t& pitch) {
-    pitch = (maxb + SELECT_CHUNK_MAX - 1) / SELECT_CHUNK_MAX * SELECT_CHUNK_MAX;
-    return hkv * (pitch * 4 + pitch / SELECT_CHUNK_MIN * 4 + pitch);
-}
-int64_t select_bytes(int64_t num_rows, int64_t row_bytes) {
-    const int64_t slab = row_bytes > SELECT_SLAB ? row_bytes : SELECT_SLAB;
-    return num_rows * row_bytes < slab ? num_rows * row_bytes : slab;
 }
 
 }  // namespace
@@ -930,31 +916,14 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     RLLM_CHECK_ARG(num_first >= 0 && num_last >= 1 && num_first <= num_selected && num_last <= num_selected - num_first);
     RLLM_CHECK_ARG(selected && query && k_bounds && seq_lens && (block_tables || max_num_blocks_per_seq == 0));
     RLLM_CHECK_ARG(aligned_to(query, 16) && aligned_to(k_bounds, 16));
-    const int64_t group = num_q_heads / num_kv_heads;
-    // several rows a sequence, one 16-row operand a group: rows share the bounds that they read
-    // (704 rows of 1250-1650 blocks, 32/8 heads, head_dim 128: 58 us, 536 row by row)
-    const bool tiles = query_start_loc && group <= 16 && num_rows >= 2 * num_seqs;
-    int64_t pitch = 0, need = 0, slab = num_rows, chunk = SELECT_CHUNK_MIN, chunks = 0;
-    if (max_num_blocks_per_seq > num_selected) {       // else every list is the whole sequence
-        const int64_t row_bytes = select_row_bytes(num_kv_heads, max_num_blocks_per_seq, pitch);
-        need = select_bytes(num_rows, row_bytes);
-        slab = need / row_bytes;
-        // Row by row, small chunks keep a block's heads together in time and fill the card
-        // with few rows (64 rows of 250-2000 blocks: 16 blocks 72 us, 64 92, 128 109); a tile
-        // of rows loads its queries for each chunk (704 rows: 32 blocks 79 us, 64 60, 128 67).
-        // Not many more workgroups than it takes.
-        chunk = tiles ? 64 : SELECT_CHUNK_MIN;
-        while (chunk < SELECT_CHUNK_MAX && slab * ((max_num_blocks_per_seq + chunk - 1) / chunk) > 32768) chunk *= 2;
-        chunks = (max_num_blocks_per_seq + chunk - 1) / chunk;
-        if (slab > INT32_MAX / (num_kv_heads * chunks)) slab = INT32_MAX / (num_kv_heads * chunks);   // workgroups of a launch
-        if (tiles) RLLM_CHECK_ARG((num_rows + num_seqs) * num_kv_heads * chunks <= INT32_MAX);
-    }
+    const SelectPlan p = select_plan(num_rows, num_seqs, num_q_heads, num_kv_heads, head_dim, max_num_blocks_per_seq,
+                                     num_selected, query_start_loc != nullptr);
     WorkspaceHold hold;
     void* ws = workspace;
     if (workspace) {
-        RLLM_CHECK_ARG(workspace_bytes >= need && aligned_to(workspace, 16));
-    } else if (need > 0) {
-        const int32_t rc = g_workspaces.get(stream, WS_SELECT, need, false, &ws, &hold);
+        RLLM_CHECK_ARG(workspace_bytes >= p.need && aligned_to(workspace, 16));
+    } else if (p.need > 0) {
+        const int32_t rc = g_workspaces.get(stream, WS_SELECT, p.need, false, &ws, &hold);
         if (rc) return rc;
         if (!ws) return static_cast<int32_t>(hipErrorStreamCaptureUnsupported);
     }
@@ -975,28 +944,28 @@ int32_t rllm_select_blocks(int32_t* selected, const void* query, const void* k_b
     a.k = static_cast<int32_t>(num_selected);
     a.first = static_cast<int32_t>(num_first);
     a.last = static_cast<int32_t>(num_last);
-    a.chunk = static_cast<int32_t>(chunk);
-    a.chunks = static_cast<int32_t>(chunks);
+    a.chunk = static_cast<int32_t>(p.chunk);
+    a.chunks = static_cast<int32_t>(p.chunks);
     a.num_blocks = num_blocks;
-    a.pitch = pitch;
-    a.tiles = tiles;
-    while ((1 << a.group_log2) < group) ++a.group_log2;
+    a.pitch = p.pitch;
+    a.tiles = p.tiles;
+    a.group_log2 = p.group_log2;
     const hipStream_t st = as_stream(stream);
-    for (int64_t r = 0; r < num_rows; r += slab) {
+    for (int64_t r = 0; r < num_rows; r += p.slab) {
         a.row0 = static_cast<int32_t>(r);
-        a.rows = static_cast<int32_t>(num_rows - r < slab ? num_rows - r : slab);
-        const int64_t units = slab * num_kv_heads;     // the scratch's layout is that of a whole slab
-        a.kmax = reinterpret_cast<float*>(a.keys + units * pitch);
-        a.state = reinterpret_cast<uint8_t*>(a.kmax + units * (pitch / SELECT_CHUNK_MIN));
+        a.rows = static_cast<int32_t>(num_rows - r < p.slab ? num_rows - r : p.slab);
+        const int64_t units = p.slab * num_kv_heads;     // the scratch's layout is that of a whole slab
+        a.kmax = reinterpret_cast<float*>(a.keys + units * p.pitch);
+        a.state = reinterpret_cast<uint8_t*>(a.kmax + units * (p.pitch / SELECT_CHUNK_MIN));
         int32_t rc;
         if (q_dtype == RLLM_DTYPE_BF16)
-            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_BF16, KIND_FP8_E4M3>(a, tiles, st)
-                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_BF16, KIND_FP8_E5M2>(a, tiles, st)
-                                                   : launch_select<KIND_BF16, KIND_BF16>(a, tiles, st);
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_BF16, KIND_FP8_E4M3>(a, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_BF16, KIND_FP8_E5M2>(a, st)
+                                                   : launch_select<KIND_BF16, KIND_BF16>(a, st);
         else
-            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_F16, KIND_FP8_E4M3>(a, tiles, st)
-                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_F16, KIND_FP8_E5M2>(a, tiles, st)
-                                                   : launch_select<KIND_F16, KIND_F16>(a, tiles, st);
+            rc = kv_dtype == RLLM_DTYPE_FP8_E4M3   ? launch_select<KIND_F16, KIND_FP8_E4M3>(a, st)
+                 : kv_dtype == RLLM_DTYPE_FP8_E5M2 ? launch_select<KIND_F16, KIND_FP8_E5M2>(a, st)
+                                                   : launch_select<KIND_F16, KIND_F16>(a, st);
         if (rc) return rc;
     }
     return 0;

@@ -240,3 +240,17 @@ def test_select_near_ties_over_several_slabs(dev, hq):
         s = int(np.searchsorted(qsl, t, side="right")) - 1
         one = S.select(q[t:t + 1], S.values(kb, "bf16"), small[s:s + 1], [lens[s] - (qsl[s + 1] - 1 - t)], None, 16, 8, 1, 1)
         assert torch.equal(wide[t:t + 1], one), t
+
+
+def test_select_more_lists_than_a_launch_has_threads_for(dev):
+    """2^26 lists and some, under a table no wider than they are."""
+    n, hkv = (1 << 23) + 3, 8
+    q = torch.ones((n, hkv, 32), dtype=torch.bfloat16, device=dev)
+    kb = torch.zeros((1, hkv, 2, 32), dtype=torch.bfloat16, device=dev)
+    bt = torch.zeros((n, 1), dtype=torch.int32, device=dev)
+    lens = torch.arange(n, dtype=torch.int32, device=dev) % 3       # 0, 1 and 2 keys
+    out = torch.full((n, hkv, 1), -7, dtype=torch.int32, device=dev)
+    log_case(f"select rows={n} hkv={hkv} d=32 width=1")
+    ops.select_blocks(q, kb, bt, lens, 16, 1, num_first=0, out=out, validate=False)
+    want = torch.where(lens > 0, 0, -1)
+    assert bool((out[:, :, 0] == want[:, None]).all())
