@@ -659,8 +659,10 @@ int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,
  * 0 .. seq_len - n + i.  Rows that no sequence has are left as they were, in every
  * output; the entries must not fall or pass num_rows.
  * Shapes: head_dim a multiple of 32 up to 256, block_size 16, 32, 64 or 128, at most
- * 1024 heads, block_size * max_num_blocks_per_seq below 2^31, all arrays of elements 16-byte
- * aligned; anything else returns hipErrorInvalidValue.  dtype / q_dtype is
+ * 1024 heads, block_size * max_num_blocks_per_seq below 2^31, at most 2^24 rows, all arrays of
+ * elements 16-byte aligned; anything else returns hipErrorInvalidValue, and so do an append and an
+ * attention whose launch would pass 2^32 - 1 threads (2^24 workgroups: a row, kv head and 16 of its
+ * heads each in the attention, 16 tokens and a kv head, or a token's queries, in the append).  dtype / q_dtype is
  * RLLM_DTYPE_F16 or RLLM_DTYPE_BF16, kv_dtype the same or an FP8 one.  Table entries
  * outside [0, num_blocks) are unused: nothing is written for them, they are in
  * no list, and lists that name them attend nothing there. */

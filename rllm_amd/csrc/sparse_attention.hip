@@ -36,7 +36,7 @@ int32_t rllm_paged_attention_sparse(void* output, const void* query, const void*
     const float s_scale = scale * k_scale * 1.44269504088896340736f;
     RLLM_CHECK_ARG(std::isfinite(scale) && std::isfinite(k_scale) && std::isfinite(v_scale) && std::isfinite(s_scale));
     const int64_t head_groups = (num_q_heads / num_kv_heads + 15) / 16;
-    RLLM_CHECK_ARG(num_rows * num_kv_heads * head_groups <= INT32_MAX);
+    RLLM_CHECK_ARG(num_rows * num_kv_heads * head_groups <= INT32_MAX);   // (and what is launched: MAX_WORKGROUPS)
     SparseArgs a = {};
     a.out = static_cast<uint16_t*>(output);
     a.q = static_cast<const uint16_t*>(query);

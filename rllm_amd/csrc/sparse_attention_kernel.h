@@ -584,7 +584,9 @@ __global__ __launch_bounds__(64 * sa_max_waves(32 * NK), (sa_max_waves(32 * NK) 
 template <int QKIND, int KVKIND, int RUN>
 int32_t launch_sparse_run(const SparseArgs& a, int64_t d, int waves, hipStream_t st) {
     const int64_t tiles = a.tile > 1 ? (static_cast<int64_t>(a.rows) + a.tile - 1) / a.tile + a.num_seqs : a.rows;
-    const dim3 grid(static_cast<unsigned>(tiles * a.hkv * a.head_groups * a.splits)), block(64 * waves);
+    const int64_t count = tiles * a.hkv * a.head_groups * a.splits;
+    RLLM_CHECK_ARG(count <= MAX_WORKGROUPS);                  // (of 512 threads where units are few)
+    const dim3 grid(static_cast<unsigned>(count)), block(64 * waves);
     const size_t lds = static_cast<size_t>(waves) * sa_stage_bytes(static_cast<int>(d)) + a.list * SA_ENTRY;
     switch (d / 32) {
 #define RLLM_SPARSE(N) \

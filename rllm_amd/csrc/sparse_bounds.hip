@@ -4,6 +4,7 @@
 // K[row, h, d].  Stored elements are compared as integers in the order of their
 // values (ordered2), so a bound is one of the stored keys, in the cache's type.
 #include "sparse_blocks.h"
+#include "sparse_plan.h"
 
 #include <type_traits>
 
@@ -462,7 +463,7 @@ int32_t rllm_rope_cache_append(void* q_out, const void* q, const void* k, const 
                     static_cast<int32_t>(max_position), group,
                     static_cast<int32_t>(num_kv_heads) + (num_q_heads > 0 ? group : 0), num_blocks, k_scale, v_scale,
                     fp8_rounding == RLLM_FP8_ROUND_NEAREST_EVEN};
-    RLLM_CHECK_ARG((num_tokens + group - 1) / group * a.roles <= INT32_MAX);
+    RLLM_CHECK_ARG((num_tokens + group - 1) / group * a.roles <= MAX_WORKGROUPS);
     const hipStream_t st = as_stream(stream);
     if (dtype == RLLM_DTYPE_BF16) {
         if (kv_dtype == RLLM_DTYPE_FP8_E4M3) return launch_append<KIND_BF16, KIND_FP8_E4M3>(a, st);
