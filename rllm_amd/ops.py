@@ -697,6 +697,13 @@ def select_blocks(q: torch.Tensor, k_bounds: torch.Tensor, block_tables: torch.T
     return out
 
 
+def _validate_lists(selected: torch.Tensor) -> None:
+    s = selected.detach().cpu()
+    before, after = s[..., :-1], s[..., 1:]
+    if bool(((after >= 0) & ((after <= before) | (before < 0))).any()):
+        raise ValueError("the blocks of a list must rise, with nothing but -1 after them")
+
+
 def paged_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                  seq_lens: torch.Tensor, selected: torch.Tensor, scale: float, *,
                  query_start_loc: Optional[torch.Tensor] = None, kv_dtype: Optional[int] = None, k_scale: float = 1.0,
@@ -729,9 +736,7 @@ def paged_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     _all_dense(q, k_cache, v_cache, block_tables, seq_lens, selected, out)
     if validate:
         _validate_rows(rows, block_tables, seq_lens, query_start_loc, nb, bs)
-        s = selected.detach().cpu()
-        if bool(((s[..., 1:] >= 0) & (s[..., 1:] <= s[..., :-1])).any()):
-            raise ValueError("the blocks of a list must rise")
+        _validate_lists(selected)
     call("rllm_paged_attention_sparse", _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
          _ptr(seq_lens), _ptr(query_start_loc), _ptr(selected), b, rows, hq, hkv, d, bs, block_tables.shape[1], nb,
          selected.shape[2], scale, dt, kv, k_scale, v_scale, _stream(stream))

@@ -1,5 +1,9 @@
-"""Sizes of the operators over selected blocks that the host refuses before any launch."""
+"""Sizes and lists of the operators over selected blocks that the host refuses before any launch."""
+import pytest
+import torch
+
 import rllm_amd
+from rllm_amd import ops
 
 P = 0x1000   # never dereferenced: validation fails first
 INVALID = 1
@@ -21,3 +25,11 @@ def test_launches_past_the_limit_of_threads_are_refused():
         assert attend(rows, hq, hkv, n=rows // 2 + 1) == INVALID, (rows, hq, hkv)
     for rows, hq, hkv in ((1 << 24, 32, 8), (1 << 24, 0, 17), (1 << 23, 1, 17), (1 << 20, 1024, 1024)):
         assert append(rows, hq, hkv) == INVALID, (rows, hq, hkv)
+
+
+def test_lists_that_do_not_rise_or_go_on_after_their_end_are_refused():
+    for good in ([0, 3, 9], [4, -1, -1], [-1, -1, -1], [7, 8, -1], [5]):
+        ops._validate_lists(torch.tensor(good, dtype=torch.int32)[None, None])
+    for bad in ([-1, 3, -1], [2, -1, 3], [-7, -7, 0], [3, 3, -1], [4, 2, 5], [0, 1, 0]):
+        with pytest.raises(ValueError, match="must rise"):
+            ops._validate_lists(torch.tensor([[1, 2, 3], bad], dtype=torch.int32)[:, None])
