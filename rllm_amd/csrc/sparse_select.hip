@@ -25,7 +25,7 @@ struct SelectArgs {
     const void* kb;
     const int32_t *bt, *seq_lens, *qsl;
     uint32_t* keys;     // [rows of the launch, hkv, pitch]: scores in their order, 0 = not to be chosen
-    uint8_t* state;     // the same, where they do not fit in LDS
+    uint8_t* state;     // OUT, MID or IN of each, for lists whose candidates are not held in registers
     float* kmax;        // [rows of the launch, hkv, chunks]: largest |bound| of a chunk, at a sequence's last row of the launch
     int32_t num_seqs, row0, rows, hq, hkv, d, bs_log2, maxb, k, first, last, chunk, chunks;
     int32_t tiles;      // whether rows were scored in tiles
@@ -66,6 +66,13 @@ __device__ __forceinline__ void split_signs(const uint4& x, uint4& neg, uint4& p
     }
     neg = make_uint4(n[0], n[1], n[2], n[3]);
     pos = make_uint4(p[0], p[1], p[2], p[3]);
+}
+// A chunk's largest magnitude, which lies highest as 16 bits do.  It may be of a block that a row which reads it does
+// not see (rows of a tile share them): NaN is an infinity there, so that the others' size counts as not known.
+template <class TAG>
+__device__ __forceinline__ float chunk_max(uint32_t bits) {
+    const float x = to_f32<TAG>(static_cast<uint16_t>(bits));
+    return x == x ? x : INFINITY;
 }
 
 // A workgroup per (row, chunk of its blocks), a wave kv heads w, w + 4, ..., 16 blocks at
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
             if (kq == 0 && j >= c0 && j < c1) keys[j] = here ? best : 0;
         }
         const uint32_t t16 = wave_umax(umax(top & 0xffffu, top >> 16));
-        if (lane == 0) a.kmax[unit * a.chunks + chunk] = to_f32<typename M::tag>(static_cast<uint16_t>(t16));
+        if (lane == 0) a.kmax[unit * a.chunks + chunk] = chunk_max<typename M::tag>(t16);
     }
 }
 
@@ -169,8 +176,8 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
 // 128) of one sequence and kv head, a quarter a wave, their queries in registers.  The
 // bounds of 16 blocks at a time go to LDS in whole runs, the next ones on their way,
 // and serve every row of the tile.  704 rows of 1250-1650
-// blocks, 32/8 heads, head_dim 128: 60 us, 26 of them vector instructions; a
-// workgroup's start (its queries) is as long as its four steps.
+// blocks, 32/8 heads, head_dim 128: 58 us; vector instructions are busy for 39% of them
+// (1339 a wave, 101 of them products), and half of a wave's cycles go in waiting.
 template <int QKIND, int KVKIND, int NK>
 __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a) {
     using M = GenMfma<QKIND>;
@@ -331,7 +338,7 @@ __global__ __launch_bounds__(256, 2) void select_score_tile_kernel(SelectArgs a)
     t16 = umax(umax(s_max[0], s_max[1]), umax(s_max[2], s_max[3]));
     if (widest && threadIdx.x == 0)
         a.kmax[(static_cast<int64_t>(x.row + nt - 1 - a.row0) * a.hkv + h) * a.chunks + chunk] =
-            to_f32<typename M::tag>(static_cast<uint16_t>(t16));
+            chunk_max<typename M::tag>(t16);
 }
 
 enum : uint8_t { OUT = 0, MID = 1, IN = 2 };
@@ -494,19 +501,17 @@ __device__ __forceinline__ float select_error(const Pick& p, Team& team) {
         }
         qs = fmaxf(qs, wave_sum(s));
     }
-    // A chunk's largest may be of a block that this row does not see (rows of a tile share them).  NaN lies above
-    // infinity as bits do, and says, as that does, that the others' is not known.
-    uint32_t top = 0;
+    float km = 0.f;
     const float* const kmax = a.kmax + (static_cast<int64_t>(p.widest - a.row0) * a.hkv + p.h) * a.chunks;
     const int ch0 = p.base / a.chunk, ch1 = (p.base + p.n - 1) / a.chunk;
-    for (int i = ch0 + lane; i <= ch1; i += 64) top = umax(top, __float_as_uint(kmax[i]));
+    for (int i = ch0 + lane; i <= ch1; i += 64) km = fmaxf(km, kmax[i]);
     qs = __uint_as_float(team.max(__float_as_uint(qs)));
-    const float km = __uint_as_float(wave_umax(top));
+    km = wave_max(km);
     // either 0: every score is exactly 0.  The product of both may be below f32's range, as the scores may: 2^-100 stands for those
     return qs == 0.f || km == 0.f ? 0.f : (a.d + 32) * 0x1p-23f * (qs * km) + 0x1p-100f;
 }
 __device__ __forceinline__ bool select_window(float th, float eps, float& over, float& under) {
-    const float slack = 2.f * eps + (eps != 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
+    const float slack = 2.f * eps + (eps > 0.f ? __builtin_fabsf(th) * 0x1p-22f : 0.f);
     over = th + slack;
     under = th - slack;
     return gen_finite(over) && gen_finite(under);
@@ -874,8 +879,9 @@ int32_t launch_select(const SelectArgs& a, hipStream_t st) {
         const int32_t rc = launch_status();
         if (rc) return rc;
     }
-    // a wave a row where rows are many and short enough, else four (8 heads: 704 rows of 1250-1650 blocks
-    // 58 us by one wave, 69 by four; 64 rows of 250-2000 34 and 18; one of 1250 24 and 13)
+    // a wave a row where rows are many and short enough, else four (8 heads, 1250-1650 blocks, with the scores,
+    // in a graph, by one wave and by four: one row 31.5 and 20.6 us, 128 158 and 147, 256, the border, 279 and
+    // 277, 384 358 and 359, 512 465 and 472; 704 of two chunks 121 and 127; 256 of 60-250 44.2 and 49.5)
     if (units >= 2048 && a.maxb <= 64 * 32)
         hipLaunchKernelGGL((select_pick_kernel<QKIND, KVKIND, 64, 32>), dim3(static_cast<unsigned>(units)), dim3(64), 0, st, a);
     else if (a.maxb <= 256 * 8)
