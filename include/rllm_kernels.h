@@ -669,7 +669,8 @@ int32_t rllm_paged_attention_prefill_mxfp4(void *output, const void *query,
 
 /* Bounds of the blocks that sequences' keys 0 .. seq_lens[s] - 1 reach, from a cache that
  * other entry points filled.  first_positions (may be NULL): blocks that end
- * at or before first_positions[s] keep the bounds they have. */
+ * at or before first_positions[s] keep the bounds they have.  Sequences that share a block
+ * must hold the same number of its rows. */
 int32_t rllm_key_bounds(void *k_bounds, const void *key_cache, const int32_t *block_tables,
                         const int32_t *seq_lens, const int32_t *first_positions, int64_t num_seqs,
                         int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
@@ -711,8 +712,9 @@ int32_t rllm_rope_cache_append(void *q_out, const void *q, const void *k, const 
  * content; one sized for a number of rows and a table width serves every call of as many
  * kv heads with no more rows and no wider table.  Calls that share it must not overlap in
  * time.  NULL: a library-owned buffer per (device, stream); a call that would have to grow
- * it while the stream is being captured returns hipErrorStreamCaptureUnsupported,
- * and graphs captured on one stream share it. */
+ * it while the stream is being captured returns hipErrorStreamCaptureUnsupported.  Graphs
+ * captured on one stream share it with each other and with its eager calls, and must not
+ * overlap with them in time. */
 #define RLLM_SELECT_MAX_BLOCKS 4096   /* most blocks of a list */
 int32_t rllm_select_blocks(int32_t *selected, const void *query, const void *k_bounds,
                            const int32_t *block_tables, const int32_t *seq_lens,
@@ -731,9 +733,12 @@ int64_t rllm_select_blocks_workspace_size(int64_t num_rows, int64_t num_kv_heads
  * nothing to attend get zeros.  scale, k_scale and v_scale as rllm_paged_attention_decode_ex.
  * output must not be query.  Sums, maxima and partials are f32, the weights 16 bits or more.  Blocks not listed
  * and keys past the row are not looked at; a key or value that is attended and not finite makes the
- * outputs it reaches not finite.  Calls of few rows (rows * num_kv_heads at most 128) use a
- * library-owned buffer per (device, stream), which graphs captured on one stream share; a capture
- * on a stream that has none runs without (results within rounding). */
+ * outputs it reaches not finite (an infinity or NaN, whichever the call's split gives), as do values
+ * whose sum over the row's keys passes f32.  Calls of few rows (num_rows * num_kv_heads * ceil(q heads
+ * of a kv head / 16) at most 128, and num_selected * block_size above 128) use a
+ * library-owned buffer per (device, stream); graphs captured on one stream share it with each other and with
+ * its eager calls, and must not overlap with them in time.  A capture on a stream that has
+ * none (no such call ran on it) runs without (results within rounding). */
 int32_t rllm_paged_attention_sparse(void *output, const void *query, const void *key_cache,
                                     const void *value_cache, const int32_t *block_tables,
                                     const int32_t *seq_lens, const int32_t *query_start_loc,

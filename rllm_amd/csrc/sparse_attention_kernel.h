@@ -22,10 +22,12 @@
 //                 the scores of a lane are the weights it needs, V's operand two 8-byte
 //                 LDS reads.
 // Loads that gave every lane the 8 x 8 tile it transposes itself read 16 bytes here
-// and there: one lane a clock, 13.5 bytes a clock and CU, whatever was in flight (64
-// rows on 128 blocks, head_dim 128, 103 us, 99 so, 5.4 TB/s; 704 rows of two chunks on 64,
-// 340, 148 so).
-// Weights enter as two 16-bit terms (generic_mfma.h).
+// and there, without LDS: no faster for 64 rows on 128 blocks (head_dim 128, 99 us either way, 5.4
+// TB/s), and 311 us for 704 rows of two chunks on 64, where whole runs and tiles take 148.
+// Weights enter as two 16-bit terms (generic_mfma.h), in bf16 16 bits of them, in f16 22.
+// A third term in bf16 made 167 of 262144 outputs of the 64 rows differ from f32 weights' by a
+// last bit instead of 524, with the same error against 64 bits (the output's rounding,
+// 2^-9, hides both), and the chunks 150 us instead of 144: left out.
 #pragma once
 
 #include "sparse_blocks.h"

@@ -452,8 +452,10 @@ int32_t rllm_rope_cache_append(void* q_out, const void* q, const void* k, const 
         RLLM_CHECK_ARG(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale > 0.f && v_scale > 0.f);
         RLLM_CHECK_ARG(fp8_rounding == RLLM_FP8_ROUND_TOWARD_ZERO || fp8_rounding == RLLM_FP8_ROUND_NEAREST_EVEN);
     }
-    // few tokens: fewer a workgroup, whose runs go one after the other (32/8 heads, head_dim 128:
-    // 64 tokens 7.2 us with 4, 14.5 with 16; 4096 into FP8 38 and 33; 9250 78 and 55)
+    // few tokens: fewer a workgroup, whose runs go one after the other (32/8 heads, head_dim 128, in
+    // a graph, 4 and 16 a workgroup: 64 sequences' one token 8.0 and 15.5 us, 512 14.4 and 20.5, 1024
+    // 23.5 and 28.8; one sequence's 512 7.8 and 8.6, 640 9.1 both, 1024 11.6 and 10.0; 8 x 512 31 and
+    // 24, into E4M3 39 and 31; 9250 of 8 59 and 45)
     const int32_t group = num_tokens <= 512 ? 4 : APPEND_GROUP;
     AppendArgs a = {static_cast<uint16_t*>(q_out), static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                     static_cast<const uint16_t*>(v), key_cache, value_cache, k_bounds, block_tables, seq_lens,

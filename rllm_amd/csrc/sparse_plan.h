@@ -100,9 +100,10 @@ struct SparsePlan {
 constexpr int64_t sparse_units(const SparseShape& s) { return s.rows * s.hkv * ((s.hq / s.hkv + 15) / 16); }
 constexpr int64_t sparse_windows(const SparseShape& s) { return ((s.k << s.bs_log2) + SA_WIN - 1) / SA_WIN; }
 
-// Few units: a CU draws some 13 bytes a clock from memory however much it asks for,
-// so a unit goes to several (1 row on 64 blocks, 8 kv heads, head_dim 128: one
-// workgroup of 8 waves 13.5 us, 8 of 2 waves 9.6).
+// Few units: a unit's keys come faster to several CUs than to one, so a unit goes to several.
+// 8 kv heads, head_dim 128, in a graph, split and not: 1 row on 64 blocks 10.5 and 14.7 us, 4
+// rows 13.4 and 14.9; 1 row on 256 14.8 and 36, 8 rows 26.5 and 38.  Where lists are short the
+// joining shows before the 128th unit (8 rows on 64 blocks 16.7 and 15.1, 16 19.0 and 15.2).
 constexpr bool sparse_few(const SparseShape& s) { return sparse_units(s) <= 128 && sparse_windows(s) > 2; }
 
 constexpr int sa_padded(int list) { return (list + 3) & ~3; }
@@ -128,9 +129,10 @@ inline SparsePlan sparse_plan(const SparseShape& s, bool scratch) {
     }
     p.waves = sa_waves_beside(p.waves, s.d, p.list = sa_padded(p.list));
     // tiles: in a chunk of several rows a sequence, where heads leave columns free, tiles
-    // fill the card (704 rows on 64 blocks each, 32/8 heads, head_dim 128: 281 us by
-    // single rows, 148 in tiles), the union of the lists fits, and the blocks' bits fit where the
-    // windows of the waves go that are left beside it
+    // fill the card (on 64 blocks each, 32/8 heads, head_dim 128, in a graph, by single rows and
+    // in tiles: 64 rows 24 and 33 us, 96 35 and 33, 128 42 and 33, the rule's border, 704 198 and
+    // 116), the union of the lists fits, and the blocks' bits fit where the windows of the
+    // waves go that are left beside it
     const int64_t G = s.hq / s.hkv;
     if (s.chunk && s.rows >= 2 * s.num_seqs && G <= 8 && p.splits == 1) {
         int tile = 16;
